@@ -1,0 +1,57 @@
+/*
+ * istnet_vocab.h -- C ABI (library libistnet_pn2.so, conventions of istnet_pn2.h) of the operators at the two ends of a model
+ * with discrete classes: a scaled table lookup and its gradient, and the distance to a teacher's top logits.
+ *
+ * Element types: ISTNET_VOCAB_F32 / _BF16 / _F16 (`dtype`, all floating tensors of a call that are not said to be float).
+ * Indices are int32 (idx64 == 0) or int64 (idx64 != 0).  Rows are contiguous (last stride 1); a leading dimension `ld*` is the
+ * distance of two rows in elements.  Every function enqueues on `stream` and returns 0, a hipError_t or ISTNET_PN2_EINVAL; the
+ * *_scratch_kib functions return the size of the caller's scratch memory `ws` in KiB (-1 for invalid sizes), which nothing has to
+ * clear and which may be reused as soon as the call's work on `stream` is done.  Sums are float or double, in an order that the
+ * sizes alone decide: the same inputs give the same bits.
+ */
+#ifndef ISTNET_VOCAB_H_
+#define ISTNET_VOCAB_H_
+
+#include "istnet_pn2.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define ISTNET_VOCAB_F32 0
+#define ISTNET_VOCAB_BF16 1
+#define ISTNET_VOCAB_F16 2
+
+/* out (n, d) = scale * weight[ids], weight (v, d) with leading dimension ldw, ids (n): float product, rounded once.  A row whose
+ * index is outside [0, v) is filled with NaN. */
+ISTNET_PN2_API int istnet_embed_forward(long long n, int v, int d, int dtype, int idx64, const void *weight, long long ldw,
+                                        const void *ids, float scale, void *out, void *stream);
+/* dw (v, d) = scale * sum of the rows of grad (n, d; leading dimension ldg) per index, added in float in the order of the rows
+ * and rounded once; rows that no index names, the row `padding` (-1: none) and indices outside [0, v) get / give nothing.
+ * All of dw is written.  n <= 2^30, v < 2^31 - 257. */
+ISTNET_PN2_API int istnet_embed_scratch_kib(long long n, int v, int d);
+ISTNET_PN2_API int istnet_embed_backward(long long n, int v, int d, int dtype, int idx64, const void *grad, long long ldg,
+                                         const void *ids, long long padding, float scale, void *ws, void *dw, void *stream);
+
+/* Distance of a student's logits z (n, v; leading dimension ldz) to a teacher of whom each row keeps k <= 256 logits
+ * top (n, k) of the classes idx (n, k); slots with idx == -1 are unused, rows without a used slot do not count:
+ *   q = softmax over the used slots of top / T,  p = softmax over all classes of z / T,
+ *   row = T^2 * sum_k q_k (log q_k - log p_idx(k)),  loss = per row (reduction 0), sum (2) or mean over the counted rows (1).
+ * An index outside [-1, v) or a NaN among the used logits makes its row NaN.  Kept for the backward: stats (n, 2) = (row maximum,
+ * 1 / sum of exp((z - maximum) / T), 0 where the row does not count), q (n, k) = the weight of a slot's class (the slots of a row
+ * that name the same class all hold their sum) and count (1) = number of counted rows (written for reductions 1 and 2).
+ * ttype: element type of top.  n <= 2^23. */
+ISTNET_PN2_API int istnet_distill_scratch_kib(long long n, int v, int k);
+ISTNET_PN2_API int istnet_distill_forward(long long n, int v, int k, int dtype, int ttype, int idx64, const void *z,
+                                          long long ldz, const void *top, const void *idx, float temperature, int reduction,
+                                          float *loss, float *stats, float *q, float *count, void *ws, void *stream);
+/* dz (n, v; contiguous) = T * g * (p - q) with g = gout (n) for reduction 0, gout (1) for 2, gout (1) / count for 1; rows that do
+ * not count get zeros. */
+ISTNET_PN2_API int istnet_distill_backward(long long n, int v, int k, int dtype, int idx64, const void *z, long long ldz,
+                                           const void *idx, float temperature, int reduction, const float *gout,
+                                           const float *stats, const float *q, const float *count, void *dz, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* ISTNET_VOCAB_H_ */

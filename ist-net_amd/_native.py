@@ -12,7 +12,8 @@ INCLUDE_DIR = os.path.join(_HERE, "..", "include")
 HEADER_PATH = os.path.join(INCLUDE_DIR, "istnet_pn2.h")
 HEADER_PATHS = [HEADER_PATH, os.path.join(INCLUDE_DIR, "istnet_pw.h"), os.path.join(INCLUDE_DIR, "istnet_preproc.h"),
                 os.path.join(INCLUDE_DIR, "istnet_optim.h"), os.path.join(INCLUDE_DIR, "istnet_rgb.h"),
-                os.path.join(INCLUDE_DIR, "istnet_heads.h"), os.path.join(INCLUDE_DIR, "istnet_conv.h")]
+                os.path.join(INCLUDE_DIR, "istnet_heads.h"), os.path.join(INCLUDE_DIR, "istnet_conv.h"),
+                os.path.join(INCLUDE_DIR, "istnet_vocab.h")]
 ABI_VERSION = 2
 
 _i, _f, _p, _d, _l = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_double, ctypes.c_longlong
@@ -146,6 +147,13 @@ SIGNATURES = {
     "istnet_smooth_l1_backward": [_l, _f, _p, _p, _p, _p, _p],
     "istnet_mse_parts": [_l],
     "istnet_mse_value_grad": [_l, _p, _p, _p, _p, _p, _p],
+    # include/istnet_vocab.h (csrc/vocab/)
+    "istnet_embed_forward": [_l, _i, _i, _i, _i, _p, _l, _p, _f, _p, _p],
+    "istnet_embed_scratch_kib": [_l, _i, _i],
+    "istnet_embed_backward": [_l, _i, _i, _i, _i, _p, _l, _p, _l, _f, _p, _p, _p],
+    "istnet_distill_scratch_kib": [_l, _i, _i],
+    "istnet_distill_forward": [_l, _i, _i, _i, _i, _i, _p, _l, _p, _p, _f, _i] + [_p] * 6,
+    "istnet_distill_backward": [_l, _i, _i, _i, _i, _p, _l, _p, _f, _i] + [_p] * 6,
     # compact-column form of a set-abstraction scale (csrc/sa_compact.hip)
     "istnet_sa_compact": [_i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p],
     "istnet_sa_compact_pair": [_i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i, _p],

@@ -15,10 +15,19 @@ ARCH = "gfx950"
 # -ffp-contract per source.  "off" for the index ops is part of their numerical contract (the
 # squared distances that decide an index are IEEE f32 in the reference's source order, no FMA contraction).
 FP_CONTRACT = {"pn2_index_ops.hip": "off", "preproc.hip": "off"}
+# csrc/vocab/: plain float code there must not be turned into packed-float instructions, some forms of which have given wrong
+# results now and then (the host pass of hipcc warns that it does not know the feature: harmless).
+SUBDIR_FLAGS = {"vocab": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
 
 
 def sources():
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
+    dirs = [CSRC] + [os.path.join(CSRC, d) for d in SUBDIR_FLAGS]
+    return [os.path.join(d, f) for d in dirs for f in sorted(os.listdir(d)) if f.endswith(".hip")]
+
+
+def headers():
+    dirs = [os.path.join(HERE, "..", "include")] + [os.path.join(CSRC, d) for d in SUBDIR_FLAGS]
+    return [os.path.join(d, f) for d in dirs for f in os.listdir(d) if f.endswith(".h")]
 
 
 def hipcc():
@@ -31,8 +40,7 @@ def hipcc():
 def needs_build():
     if not os.path.exists(LIB_PATH):
         return True
-    newest = max(os.path.getmtime(p) for p in sources() + [
-        os.path.join(HERE, "..", "include", f) for f in os.listdir(os.path.join(HERE, "..", "include"))])
+    newest = max(os.path.getmtime(p) for p in sources() + headers())
     return os.path.getmtime(LIB_PATH) < newest
 
 
@@ -50,6 +58,7 @@ def build(force=False, verbose=False):
         contract = os.environ.get("ISTNET_FP_CONTRACT_" + os.path.basename(src)[:-4].upper(),
                                   FP_CONTRACT.get(os.path.basename(src), "off"))
         extra = os.environ.get("ISTNET_HIPCC_FLAGS", "").split()      # experiments (e.g. -DISTNET_BWD_SMALL_WAVES=3)
+        extra = SUBDIR_FLAGS.get(os.path.basename(os.path.dirname(src)), []) + extra
         cmd = common + extra + [f"-ffp-contract={contract}", "-c", src, "-o", obj]
         if verbose:
             print(" ".join(cmd))

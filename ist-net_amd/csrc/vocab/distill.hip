@@ -1,0 +1,337 @@
+// Distance of a student's logits to a teacher's top logits, forward and backward (include/istnet_vocab.h).  gfx950 only, wave64.
+//
+//   q_k = softmax over the used slots of t_k / T          p_v = softmax over all classes of z_v / T
+//   row = T^2 sum_k q_k (log q_k - log p_idx(k))          dz_v = T g (p_v - sum_{k: idx(k) = v} q_k)
+//
+// Bound by bytes: z is read once forward (one pass with a running maximum and sum), read once and dz written once backward; the
+// teacher's k values are noise beside a row.  A row is one workgroup's, or several workgroups' where there are few rows.
+#include <algorithm>
+
+#include "vocab_common.h"
+
+namespace {
+
+constexpr int kMaxSlots = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNaN = __builtin_nanf("");
+
+struct Stat { float m, s; };      // maximum, sum of exp2((x - maximum) c)
+
+__device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
+  const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;      // nothing seen yet: exp2(-inf) = 0, not NaN
+  return {m, a.s * exp2_raw((a.m - ref) * c) + b.s * exp2_raw((b.m - ref) * c)};
+}
+
+template <int THREADS> __device__ __forceinline__ float block_max(float x, float* tmp) {
+  x = wave_max(x);
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = tmp[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) x = fmaxf(x, tmp[w]);
+    __syncthreads();
+  }
+  return x;
+}
+template <int THREADS> __device__ __forceinline__ float block_sum(float x, float* tmp) {
+  x = wave_sum(x);
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = tmp[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) x += tmp[w];
+    __syncthreads();
+  }
+  return x;
+}
+
+// any used slot in the row?  (every thread gets the answer)
+template <int THREADS>
+__device__ __forceinline__ bool row_counts(const void* idx, long long row, int k, int idx64, float* tmp) {
+  float any = 0.f;
+  for (int j = threadIdx.x; j < k; j += THREADS) any = load_index(idx, row * k + j, idx64) != -1 ? 1.f : any;
+  return block_max<THREADS>(any, tmp) > 0.f;
+}
+
+// running maximum and sum of z[a, e) over the workgroup's threads
+template <typename T, int THREADS>
+__device__ __forceinline__ Stat scan_row(const T* __restrict__ z, int a, int e, float c, float* tmp) {
+  constexpr int V = kVec<T>, U = 4;      // four sixteen-byte loads in flight per thread
+  Stat st = {-INFINITY, 0.f};
+  int at = a + threadIdx.x * V;
+  for (; at + (U - 1) * THREADS * V + V <= e; at += U * THREADS * V) {
+    float f[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) unpack<T>(load16(z + at + u * THREADS * V), f[u]);
+    float m = st.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = fmaxf(m, f[u][i]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = st.s * exp2_raw((st.m - ref) * c);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += exp2_raw((f[u][i] - ref) * c);
+    st = {m, s};
+  }
+  for (; at < e; at += THREADS * V) {
+    const int left = e - at;
+    float f[V];
+    load_part(z + at, left, f);
+    float m = st.m;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = i < left ? fmaxf(m, f[i]) : m;
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = st.s * exp2_raw((st.m - ref) * c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += i < left ? exp2_raw((f[i] - ref) * c) : 0.f;
+    st = {m, s};
+  }
+  const float m = block_max<THREADS>(st.m, tmp), ref = m == -INFINITY ? 0.f : m;
+  return {m, block_sum<THREADS>(st.s * exp2_raw((st.m - ref) * c), tmp)};
+}
+
+// the row's loss from its statistics: teacher's softmax, the k picked logits, weights of the slots for the backward
+template <typename T, int THREADS>
+__device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k, int ttype, int idx64, const void* __restrict__ top,
+                                           const void* __restrict__ idx, long long row, float temp, Stat st, bool counts,
+                                           float* __restrict__ row_loss, float* __restrict__ stats, float* __restrict__ q, float* tmp,
+                                           float* lq, int* lidx) {
+  const int tid = threadIdx.x;
+  if (!counts) {
+    for (int j = tid; j < k; j += THREADS) q[row * k + j] = 0.f;
+    if (tid == 0) { stats[2 * row] = 0.f; stats[2 * row + 1] = 0.f; row_loss[row] = 0.f; }
+    return;
+  }
+  float tm = -INFINITY, bad = 0.f;
+  for (int j = tid; j < k; j += THREADS) {
+    const long long id = load_index(idx, row * k + j, idx64);
+    float t = -INFINITY;
+    if (id != -1) {
+      t = (ttype == ISTNET_VOCAB_F32 ? ((const float*)top)[row * k + j]
+           : ttype == ISTNET_VOCAB_BF16 ? to_f32(((const bf16*)top)[row * k + j]) : (float)((const f16*)top)[row * k + j]) / temp;
+      if (id < -1 || id >= v || t != t) bad = 1.f;
+    }
+    lq[j] = t;
+    lidx[j] = (id < 0 || id >= v) ? -1 : (int)id;
+    tm = fmaxf(tm, t);
+  }
+  bad = block_max<THREADS>(bad, tmp);
+  tm = block_max<THREADS>(tm, tmp);
+  float ts = 0.f;
+  for (int j = tid; j < k; j += THREADS) ts += lidx[j] >= 0 ? expf(lq[j] - tm) : 0.f;
+  ts = block_sum<THREADS>(ts, tmp);
+  const float log_ts = logf(ts), log_s = logf(st.s);
+  float loss = 0.f;
+  for (int j = tid; j < k; j += THREADS) {
+    const float t = lq[j];
+    float qj = 0.f;
+    if (lidx[j] >= 0) {
+      qj = expf(t - tm) / ts;
+      // a slot of the teacher's logit -inf weighs nothing, whatever the student says
+      if (!(qj == 0.f)) loss += qj * ((t - tm - log_ts) - ((to_f32(z[lidx[j]]) - st.m) / temp - log_s));
+    }
+    lq[j] = qj;      // each thread overwrites only what it alone has read since the barrier
+  }
+  loss = block_sum<THREADS>(loss, tmp);
+  __syncthreads();
+  for (int j = tid; j < k; j += THREADS) {      // slots of the same class share their weights' sum, in slot order
+    float sum = 0.f;
+    for (int i = 0; i < k; ++i) sum += lidx[i] == lidx[j] ? lq[i] : 0.f;
+    q[row * k + j] = lidx[j] >= 0 ? sum : 0.f;
+  }
+  if (tid == 0) {
+    stats[2 * row] = st.m;
+    stats[2 * row + 1] = bad > 0.f ? kNaN : 1.f / st.s;
+    row_loss[row] = bad > 0.f ? kNaN : temp * temp * loss;
+  }
+}
+
+// splits == 1: the whole row and its loss; else one of `splits` parts of the row, (maximum, sum) to part
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_rows_kernel(int v, int k, int ttype, int idx64, const T* __restrict__ z,
+                                                               long long ldz, const void* __restrict__ top,
+                                                               const void* __restrict__ idx, float temp, int splits, int width,
+                                                               Stat* __restrict__ part, float* __restrict__ row_loss,
+                                                               float* __restrict__ stats, float* __restrict__ q) {
+  __shared__ float tmp[THREADS / 64];
+  __shared__ float lq[kMaxSlots];
+  __shared__ int lidx[kMaxSlots];
+  const long long row = blockIdx.x / splits;
+  const int a = (int)(blockIdx.x % splits) * width, e = min(v, a + width);
+  const bool counts = row_counts<THREADS>(idx, row, k, idx64, tmp);
+  Stat st = {-INFINITY, 0.f};
+  if (counts) st = scan_row<T, THREADS>(z + row * ldz, a, e, kLog2e / temp, tmp);
+  if (splits == 1)
+    finish_row<T, THREADS>(z + row * ldz, v, k, ttype, idx64, top, idx, row, temp, st, counts, row_loss, stats, q, tmp, lq, lidx);
+  else if (threadIdx.x == 0)
+    part[blockIdx.x] = st;
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(int v, int k, int ttype, int idx64, const T* __restrict__ z, long long ldz,
+                                                          const void* __restrict__ top, const void* __restrict__ idx, float temp,
+                                                          int splits, const Stat* __restrict__ part, float* __restrict__ row_loss,
+                                                          float* __restrict__ stats, float* __restrict__ q) {
+  __shared__ float tmp[1];
+  __shared__ float lq[kMaxSlots];
+  __shared__ int lidx[kMaxSlots];
+  const long long row = blockIdx.x;
+  const float c = kLog2e / temp;
+  const bool counts = row_counts<64>(idx, row, k, idx64, tmp);
+  Stat st = {-INFINITY, 0.f};
+  if (counts) {
+    for (int p = threadIdx.x; p < splits; p += 64) st = merge(st, part[row * splits + p], c);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) st = merge(st, {__shfl_xor(st.m, o), __shfl_xor(st.s, o)}, c);
+  }
+  finish_row<T, 64>(z + row * ldz, v, k, ttype, idx64, top, idx, row, temp, st, counts, row_loss, stats, q, tmp, lq, lidx);
+}
+
+// sum of the rows' losses and number of counted rows, in double, one workgroup
+__global__ __launch_bounds__(1024) void distill_total_kernel(long long n, int mean, const float* __restrict__ row_loss,
+                                                             const float* __restrict__ stats, float* __restrict__ loss,
+                                                             float* __restrict__ count) {
+  __shared__ double tmp[2][16];
+  double sum = 0.0, rows = 0.0;
+  for (long long i = threadIdx.x; i < n; i += 1024) {
+    sum += row_loss[i];
+    rows += stats[2 * i + 1] == 0.f ? 0.0 : 1.0;      // 1 / sum of exponentials: zero only where nothing was counted
+  }
+  sum = wave_sum(sum);
+  rows = wave_sum(rows);
+  if ((threadIdx.x & 63) == 0) { tmp[0][threadIdx.x >> 6] = sum; tmp[1][threadIdx.x >> 6] = rows; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = rows = 0.0;
+    for (int w = 0; w < 16; ++w) { sum += tmp[0][w]; rows += tmp[1][w]; }
+    *loss = (float)(mean ? sum / rows : sum);
+    *count = (float)rows;
+  }
+}
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int idx64, const T* __restrict__ z, long long ldz,
+                                                               const void* __restrict__ idx, float temp, int reduction,
+                                                               const float* __restrict__ gout, const float* __restrict__ stats,
+                                                               const float* __restrict__ q, const float* __restrict__ count,
+                                                               int splits, int width, T* __restrict__ dz) {
+  constexpr int V = kVec<T>;
+  const long long row = blockIdx.x / splits;
+  const int a = (int)(blockIdx.x % splits) * width, e = min(v, a + width);
+  const float m = stats[2 * row], inv_s = stats[2 * row + 1], c = kLog2e / temp;
+  T* out = dz + row * v;
+  if (inv_s == 0.f) {      // a row without a teacher: its logits are not looked at
+    const float zero[V] = {};
+    for (int at = a + threadIdx.x * V; at < e; at += THREADS * V) store_part(out + at, e - at, zero);
+    return;
+  }
+  const float g = temp * (reduction == 0 ? gout[row] : reduction == 1 ? gout[0] / count[0] : gout[0]);
+  const float gp = g * inv_s;
+  const T* in = z + row * ldz;
+  constexpr int U = 2;
+  int at = a + threadIdx.x * V;
+  for (; at + (U - 1) * THREADS * V + V <= e; at += U * THREADS * V) {
+    float f[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) unpack<T>(load16(in + at + u * THREADS * V), f[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[u][i] = gp * exp2_raw((f[u][i] - m) * c);
+      store16(out + at + u * THREADS * V, pack<T>(f[u]));
+    }
+  }
+  for (; at < e; at += THREADS * V) {
+    float f[V];
+    load_part(in + at, e - at, f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = gp * exp2_raw((f[i] - m) * c);
+    store_part(out + at, e - at, f);
+  }
+  // the teacher's classes: p - q is formed before it is rounded.  The barrier orders these stores behind the row's.
+  __syncthreads();
+  for (int j = threadIdx.x; j < k; j += THREADS) {
+    const long long id = load_index(idx, row * k + j, idx64);
+    if (id >= a && id < e) out[id] = from_f32<T>(g * (inv_s * exp2_raw((to_f32(in[id]) - m) * c) - q[row * k + j]));
+  }
+}
+
+struct DistillPlan { int threads, splits, width; };
+// One wave per row up to 4 KB, four waves above; parts of a row (of whole 4 KB blocks) where the rows alone are too few workgroups
+// for the chip's 256 compute units.
+inline DistillPlan distill_plan(long long n, int v, int elt) {
+  DistillPlan p;
+  const long long bytes = (long long)v * elt;
+  p.threads = bytes <= 4096 ? 64 : 256;
+  const int block = 4096 / elt;
+  const long long blocks = (v + block - 1) / block;
+  p.splits = (int)std::min(blocks, std::max(1ll, 2048 / n));
+  p.width = (int)((blocks + p.splits - 1) / p.splits) * block;
+  p.splits = (int)((v + (long long)p.width - 1) / p.width);
+  return p;
+}
+inline bool distill_ok(long long n, int v, int k) {
+  // a launch holds fewer than 2^32 threads
+  return n >= 1 && n <= (1ll << 23) && v >= 1 && v < 0x7fffffff - 65536 && k >= 1 && k <= kMaxSlots;
+}
+
+}  // namespace
+
+extern "C" int istnet_distill_scratch_kib(long long n, int v, int k) {
+  if (!distill_ok(n, v, k)) return -1;
+  const DistillPlan a = distill_plan(n, v, 2), b = distill_plan(n, v, 4);
+  const long long parts = n * std::max(a.splits, b.splits);
+  return (int)((4 * n + 8 * parts + 2047) / 1024);
+}
+
+extern "C" int istnet_distill_forward(long long n, int v, int k, int dtype, int ttype, int idx64, const void* z, long long ldz,
+                                      const void* top, const void* idx, float temperature, int reduction, float* loss, float* stats,
+                                      float* q, float* count, void* ws, void* stream) {
+  if (!distill_ok(n, v, k) || dtype < 0 || dtype > 2 || ttype < 0 || ttype > 2 || !z || !top || !idx || !loss || !stats || !q ||
+      !count || !ws || ldz < v || !(temperature > 0.f) || reduction < 0 || reduction > 2)
+    return ISTNET_PN2_EINVAL;
+  const hipStream_t st = (hipStream_t)stream;
+  const DistillPlan p = distill_plan(n, v, dtype == ISTNET_VOCAB_F32 ? 4 : 2);
+  Stat* part = (Stat*)ws;
+  float* row_loss = reduction == 0 ? loss : (float*)((char*)ws + (p.splits > 1 ? 8 * n * p.splits : 0));
+  const dim3 grid((unsigned)(n * p.splits));
+  VOCAB_DISPATCH(dtype, T, {
+    if (p.threads == 64)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_rows_kernel<T, 64>), grid, dim3(64), 0, st, v, k, ttype, idx64, (const T*)z, ldz, top,
+                         idx, temperature, p.splits, p.width, part, row_loss, stats, q);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_rows_kernel<T, 256>), grid, dim3(256), 0, st, v, k, ttype, idx64, (const T*)z, ldz,
+                         top, idx, temperature, p.splits, p.width, part, row_loss, stats, q);
+    if (p.splits > 1)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_join_kernel<T>), dim3((unsigned)n), dim3(64), 0, st, v, k, ttype, idx64, (const T*)z,
+                         ldz, top, idx, temperature, p.splits, part, row_loss, stats, q);
+  });
+  if (reduction != 0)
+    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, st, n, reduction == 1, row_loss, stats, loss, count);
+  return launch_status();
+}
+
+extern "C" int istnet_distill_backward(long long n, int v, int k, int dtype, int idx64, const void* z, long long ldz, const void* idx,
+                                       float temperature, int reduction, const float* gout, const float* stats, const float* q,
+                                       const float* count, void* dz, void* stream) {
+  if (!distill_ok(n, v, k) || dtype < 0 || dtype > 2 || !z || !idx || !gout || !stats || !q || !count || !dz || ldz < v ||
+      !(temperature > 0.f) || reduction < 0 || reduction > 2)
+    return ISTNET_PN2_EINVAL;
+  const hipStream_t st = (hipStream_t)stream;
+  const DistillPlan p = distill_plan(n, v, dtype == ISTNET_VOCAB_F32 ? 4 : 2);
+  const dim3 grid((unsigned)(n * p.splits));
+  VOCAB_DISPATCH(dtype, T, {
+    if (p.threads == 64)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_grad_kernel<T, 64>), grid, dim3(64), 0, st, v, k, idx64, (const T*)z, ldz, idx,
+                         temperature, reduction, gout, stats, q, count, p.splits, p.width, (T*)dz);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_grad_kernel<T, 256>), grid, dim3(256), 0, st, v, k, idx64, (const T*)z, ldz, idx,
+                         temperature, reduction, gout, stats, q, count, p.splits, p.width, (T*)dz);
+  });
+  return launch_status();
+}

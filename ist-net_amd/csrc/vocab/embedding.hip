@@ -1,0 +1,499 @@
+// Scaled table lookup and its gradient (include/istnet_vocab.h).  gfx950 only, wave64, no matrix work: both directions move bytes.
+//
+//   out_i = s * w_id(i)                       reads the touched rows and n indices, writes n rows
+//   dw_v  = s * sum_{i: id(i) = v} g_i        reads n rows and n indices, writes ALL v rows (zeros where no index points)
+//
+// The gradient is a sum over the tokens of each index in the order of the tokens, so it is the same bits on every run: the tokens
+// are sorted by index (stable, least significant digit first), every table row then owns a run of the sorted list and one team of
+// lanes adds it up in registers -- no atomics, dw written once.  A run longer than L tokens would leave one team with a long chain
+// of loads; it is cut where the sorted list is cut into pieces of L, the pieces are summed side by side and joined in order.
+#include <algorithm>
+
+#include "vocab_common.h"
+
+namespace {
+
+constexpr int kSmallSort = 8192;      // tokens that one workgroup sorts in LDS
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallDigit = 6;        // bits of a digit there: 64 digits x 16 waves = one counter per thread
+constexpr int kDigit = 9;             // most bits of a digit of the sort over many workgroups
+constexpr int kSortThreads = 256;
+constexpr int kSortItems = 16;        // tokens per thread and workgroup of that sort
+
+__device__ __forceinline__ uint32_t key_of(const void* ids, long long i, int idx64, int v, long long padding) {
+  const long long id = load_index(ids, i, idx64);
+  return (id < 0 || id >= v || id == padding) ? (uint32_t)v : (uint32_t)id;      // key v: nobody's gradient, sorted last
+}
+
+// lanes of the wave that are active and hold the same digit
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool active) {
+  uint64_t m = __ballot(active);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1u;
+    const uint64_t has = __ballot(one);
+    m &= one ? has : ~has;
+  }
+  return m;
+}
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+}
+// position of this lane's key among the keys of its digit that the wave has seen so far; counts the wave's keys in cnt[digit]
+__device__ __forceinline__ int rank_and_count(uint32_t digit, int bits, bool active, int* cnt, int lane) {
+  const uint64_t m = same_digit(digit, bits, active);
+  const int lead = active ? __builtin_ctzll(m) : lane;
+  int base = 0;
+  if (active && lane == lead) base = atomicAdd(&cnt[digit], (int)__popcll(m));
+  base = __shfl(base, lead);
+  return base + lanes_below(m);
+}
+
+// exclusive scan of one int per thread over the workgroup; tmp: one int per wave
+template <int THREADS> __device__ __forceinline__ int block_exclusive(int x, int* tmp, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(s, o);
+    if (lane >= o) s += y;
+  }
+  if (lane == 63) tmp[wave] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int t = tmp[w];
+    if (w < wave) before += t;
+    all += t;
+  }
+  __syncthreads();
+  *total = all;
+  return before + s - x;
+}
+
+// up to kSmallSort tokens: every pass in LDS, one launch
+__global__ __launch_bounds__(kSmallThreads) void embed_sort_small_kernel(int n, int v, const void* __restrict__ ids, int idx64,
+                                                                         long long padding, int bits, int passes,
+                                                                         uint32_t* __restrict__ keys, uint32_t* __restrict__ perm) {
+  constexpr int WAVES = kSmallThreads / 64, ROUNDS = kSmallSort / kSmallThreads;
+  __shared__ uint32_t skey[2][kSmallSort];
+  __shared__ uint16_t sperm[2][kSmallSort];
+  __shared__ int cnt[1 << kSmallDigit][WAVES];      // digit-major: the scan order is the sort order
+  __shared__ int wcnt[WAVES][1 << kSmallDigit];
+  __shared__ int tmp[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rounds = (n + kSmallThreads - 1) / kSmallThreads, first = wave * rounds * 64;
+  for (int r = 0; r < rounds; ++r) {
+    const int i = first + r * 64 + lane;
+    if (i < n) {
+      skey[0][i] = key_of(ids, i, idx64, v, padding);
+      sperm[0][i] = (uint16_t)i;
+    }
+  }
+  const int radix = 1 << bits;
+  for (int p = 0; p < passes; ++p) {
+    const int from = p & 1, shift = p * bits;
+    for (int d = lane; d < radix; d += 64) wcnt[wave][d] = 0;
+    __syncthreads();
+    int rank[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      if (r < rounds) {
+        const int i = first + r * 64 + lane;
+        const bool active = i < n;
+        const uint32_t digit = active ? (skey[from][i] >> shift) & (uint32_t)(radix - 1) : 0u;
+        rank[r] = rank_and_count(digit, bits, active, wcnt[wave], lane);
+      }
+    }
+    for (int d = lane; d < radix; d += 64) cnt[d][wave] = wcnt[wave][d];
+    __syncthreads();
+    int all;
+    int* flat = &cnt[0][0];
+    const int mine = tid < radix * WAVES ? flat[tid] : 0;
+    const int before = block_exclusive<kSmallThreads>(mine, tmp, &all);
+    if (tid < radix * WAVES) flat[tid] = before;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const int i = first + r * 64 + lane;
+      if (r < rounds && i < n) {
+        const uint32_t k = skey[from][i];
+        const int pos = cnt[(k >> shift) & (uint32_t)(radix - 1)][wave] + rank[r];
+        skey[from ^ 1][pos] = k;
+        sperm[from ^ 1][pos] = sperm[from][i];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += kSmallThreads) {
+    keys[i] = skey[passes & 1][i];
+    perm[i] = sperm[passes & 1][i];
+  }
+}
+
+// One pass of the sort over many workgroups: digit counts per workgroup, scan of the counts digit by digit, stable scatter.
+// Wave w of workgroup b owns tokens [b * tile + w * 64 * items, ...): the order of (workgroup, wave, round, lane) is token order.
+__global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(int n, int v, const void* __restrict__ ids, int idx64,
+                                                                  long long padding, const uint32_t* __restrict__ keys_in, int shift,
+                                                                  int bits, int items, int nb, int* __restrict__ hist) {
+  __shared__ int cnt[1 << kDigit];
+  const int radix = 1 << bits, b = blockIdx.x;
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) cnt[d] = 0;
+  __syncthreads();
+  const long long base = (long long)b * kSortThreads * items;
+  for (int r = 0; r < items; ++r) {
+    const long long i = base + r * kSortThreads + threadIdx.x;
+    if (i < n) {
+      const uint32_t k = keys_in ? keys_in[i] : key_of(ids, i, idx64, v, padding);
+      atomicAdd(&cnt[(k >> shift) & (uint32_t)(radix - 1)], 1);
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[(long long)d * nb + b] = cnt[d];
+}
+
+__global__ __launch_bounds__(1024) void embed_scan_kernel(long long count, int* __restrict__ hist) {
+  __shared__ int tmp[16];
+  int carry = 0;
+  for (long long base = 0; base < count; base += 4096) {
+    const long long i = base + 4 * threadIdx.x;
+    int x[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = i + j < count ? hist[i + j] : 0;
+      sum += x[j];
+    }
+    int all;
+    int at = carry + block_exclusive<1024>(sum, tmp, &all);
+    carry += all;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j < count) hist[i + j] = at;
+      at += x[j];
+    }
+  }
+}
+
+__global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int v, const void* __restrict__ ids, int idx64,
+                                                                     long long padding, const uint32_t* __restrict__ keys_in,
+                                                                     const uint32_t* __restrict__ perm_in, int shift, int bits,
+                                                                     int items, int nb, const int* __restrict__ hist,
+                                                                     uint32_t* __restrict__ keys_out, uint32_t* __restrict__ perm_out) {
+  constexpr int WAVES = kSortThreads / 64;
+  __shared__ int cnt[WAVES][1 << kDigit];
+  const int radix = 1 << bits, b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = lane; d < radix; d += 64) cnt[wave][d] = 0;
+  __syncthreads();
+  const long long first = ((long long)b * WAVES + wave) * 64 * items;
+  int rank[kSortItems];
+  uint32_t key[kSortItems];
+#pragma unroll
+  for (int r = 0; r < kSortItems; ++r) {
+    if (r < items) {
+      const long long i = first + r * 64 + lane;
+      const bool active = i < n;
+      key[r] = active ? (keys_in ? keys_in[i] : key_of(ids, i, idx64, v, padding)) : 0u;
+      rank[r] = rank_and_count((key[r] >> shift) & (uint32_t)(radix - 1), bits, active, cnt[wave], lane);
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) {
+    int at = hist[(long long)d * nb + b];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const int c = cnt[w][d];
+      cnt[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kSortItems; ++r) {
+    const long long i = first + r * 64 + lane;
+    if (r < items && i < n) {
+      const int pos = cnt[wave][(key[r] >> shift) & (uint32_t)(radix - 1)] + rank[r];
+      keys_out[pos] = key[r];
+      perm_out[pos] = perm_in ? perm_in[i] : (uint32_t)i;
+    }
+  }
+}
+
+// start[t] = number of sorted keys below t, t = 0 .. v
+__global__ __launch_bounds__(256) void embed_starts_kernel(int n, int v, const uint32_t* __restrict__ keys, int* __restrict__ start) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t > v) return;
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (keys[mid] < (uint32_t)t) lo = mid + 1; else hi = mid;
+  }
+  start[t] = lo;
+}
+
+// sum of the gradient rows of sorted tokens [a, e), elements [col, col + left), four loads in flight, added in order
+template <typename T>
+__device__ __forceinline__ void sum_run(const T* __restrict__ grad, long long ldg, const uint32_t* __restrict__ perm, int a, int e,
+                                        int col, int left, float (&acc)[kVec<T>]) {
+  int p = a;
+  for (; p + 4 <= e; p += 4) {
+    float f[4][kVec<T>];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_part(grad + (long long)perm[p + j] * ldg + col, left, f[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) acc[i] += f[j][i];
+  }
+  for (; p < e; ++p) {
+    float f[kVec<T>];
+    load_part(grad + (long long)perm[p] * ldg + col, left, f);
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) acc[i] += f[i];
+  }
+}
+
+constexpr int kTeamRows = 4;      // consecutive table rows per team of lanes
+
+template <typename T>
+__global__ __launch_bounds__(256) void embed_rows_kernel(int v, int d, int lanes_log, int longest, const T* __restrict__ grad,
+                                                         long long ldg, const uint32_t* __restrict__ perm,
+                                                         const int* __restrict__ start, float scale, T* __restrict__ dw) {
+  const int lanes = 1 << lanes_log, at = threadIdx.x & (lanes - 1);
+  const long long step = (long long)gridDim.x * kTeamRows << (8 - lanes_log);
+  for (long long row0 = (((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log)) * kTeamRows; row0 < v; row0 += step) {
+    int s[kTeamRows + 1];
+#pragma unroll
+    for (int r = 0; r <= kTeamRows; ++r) s[r] = start[row0 + r < v ? row0 + r : v];
+    for (int col = at * kVec<T>; col < d; col += lanes * kVec<T>) {
+#pragma unroll
+      for (int r = 0; r < kTeamRows; ++r) {
+        if (row0 + r < v && s[r + 1] - s[r] <= longest) {
+          float acc[kVec<T>] = {};
+          sum_run(grad, ldg, perm, s[r], s[r + 1], col, d - col, acc);
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i) acc[i] *= scale;
+          store_part(dw + (row0 + r) * d + col, d - col, acc);
+        }
+      }
+    }
+  }
+}
+
+// the teams of a workgroup hold partial sums of the same columns: team 0 gets them added in team order
+template <typename T>
+__device__ __forceinline__ void join_teams(float (&acc)[kVec<T>], float* lds, int lanes_log, int teams) {
+  const int at = threadIdx.x & ((1 << lanes_log) - 1), team = threadIdx.x >> lanes_log;
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) lds[(i << 8) + threadIdx.x] = acc[i];
+  __syncthreads();
+  if (team == 0) {
+    for (int t = 1; t < teams; ++t)
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) acc[i] += lds[(i << 8) + (t << lanes_log) + at];
+  }
+  __syncthreads();
+}
+
+// Piece p holds sorted tokens [p L, (p + 1) L).  At most two runs longer than L touch it: the one of its first token (slot 0) and
+// the one of its last (slot 1, if that is another one).
+template <typename T>
+__global__ __launch_bounds__(256) void embed_pieces_kernel(int n, int v, int d, int lanes_log, int longest, const T* __restrict__ grad,
+                                                           long long ldg, const uint32_t* __restrict__ keys,
+                                                           const uint32_t* __restrict__ perm, const int* __restrict__ start,
+                                                           float* __restrict__ part) {
+  __shared__ float lds[256 * kVec<T>];
+  const int lanes = 1 << lanes_log, teams = 256 >> lanes_log, at = threadIdx.x & (lanes - 1), team = threadIdx.x >> lanes_log;
+  const int p0 = blockIdx.x * longest, p1 = min(n, p0 + longest);
+  const uint32_t ka = keys[p0], kb = keys[p1 - 1];
+  for (int slot = 0; slot < 2; ++slot) {
+    const uint32_t k = slot ? kb : ka;
+    if (k >= (uint32_t)v || (slot && kb == ka)) continue;
+    const int s = start[k], e = start[k + 1];
+    if (e - s <= longest) continue;
+    const int a0 = max(s, p0), a1 = min(e, p1), per = (a1 - a0 + teams - 1) / teams;
+    const int a = min(a1, a0 + team * per), b = min(a1, a + per);
+    for (int c0 = 0; c0 < d; c0 += lanes * kVec<T>) {
+      const int col = c0 + at * kVec<T>;
+      float acc[kVec<T>] = {};
+      if (col < d) sum_run(grad, ldg, perm, a, b, col, d - col, acc);
+      join_teams<T>(acc, lds, lanes_log, teams);
+      if (team == 0 && col < d) {
+        float* o = part + ((long long)blockIdx.x * 2 + slot) * d + col;
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i)
+          if (col + i < d) o[i] = acc[i];
+      }
+    }
+  }
+}
+
+// the run longer than L that STARTS in piece p (there is at most one, that of the piece's last token): its partial sums in order
+template <typename T>
+__global__ __launch_bounds__(256) void embed_join_kernel(int n, int v, int d, int lanes_log, int longest,
+                                                         const uint32_t* __restrict__ keys, const int* __restrict__ start,
+                                                         const float* __restrict__ part, float scale, T* __restrict__ dw) {
+  __shared__ float lds[256 * kVec<T>];
+  const int lanes = 1 << lanes_log, teams = 256 >> lanes_log, at = threadIdx.x & (lanes - 1), team = threadIdx.x >> lanes_log;
+  const int p0 = blockIdx.x * longest, p1 = min(n, p0 + longest);
+  const uint32_t k = keys[p1 - 1];
+  if (k >= (uint32_t)v) return;
+  const int s = start[k], e = start[k + 1];
+  if (e - s <= longest || s < p0) return;
+  const int q0 = blockIdx.x, q1 = (e - 1) / longest + 1, per = (q1 - q0 + teams - 1) / teams;
+  const int a = min(q1, q0 + team * per), b = min(q1, a + per);
+  for (int c0 = 0; c0 < d; c0 += lanes * kVec<T>) {
+    const int col = c0 + at * kVec<T>;
+    float acc[kVec<T>] = {};
+    if (col < d) {
+      for (int q = a; q < b; ++q) {
+        const float* o = part + ((long long)q * 2 + (s > q * longest ? 1 : 0)) * d + col;
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) acc[i] += col + i < d ? o[i] : 0.f;
+      }
+    }
+    join_teams<T>(acc, lds, lanes_log, teams);
+    if (team == 0 && col < d) {
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) acc[i] *= scale;
+      store_part(dw + (long long)k * d + col, d - col, acc);
+    }
+  }
+}
+
+constexpr int kLookupRows = 4;      // rows per team of lanes: their loads are in flight together
+
+template <typename T>
+__global__ __launch_bounds__(256) void embed_lookup_kernel(long long n, int v, int d, int lanes_log, int idx64,
+                                                           const T* __restrict__ weight, long long ldw, const void* __restrict__ ids,
+                                                           float scale, T* __restrict__ out) {
+  const int lanes = 1 << lanes_log, at = threadIdx.x & (lanes - 1);
+  const long long step = (long long)gridDim.x * kLookupRows << (8 - lanes_log);
+  for (long long row0 = (((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log)) * kLookupRows; row0 < n; row0 += step) {
+    long long id[kLookupRows];
+#pragma unroll
+    for (int r = 0; r < kLookupRows; ++r) {
+      const long long i = row0 + r < n ? load_index(ids, row0 + r, idx64) : -1;
+      id[r] = (i < 0 || i >= v) ? -1 : i;
+    }
+    for (int col = at * kVec<T>; col < d; col += lanes * kVec<T>) {
+      float f[kLookupRows][kVec<T>];
+#pragma unroll
+      for (int r = 0; r < kLookupRows; ++r) {
+        if (id[r] >= 0) {
+          load_part(weight + id[r] * ldw + col, d - col, f[r]);
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i) f[r][i] *= scale;
+        } else {
+#pragma unroll
+          for (int i = 0; i < kVec<T>; ++i) f[r][i] = __uint_as_float(0x7fc00000u);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kLookupRows; ++r)
+        if (row0 + r < n) store_part(out + (row0 + r) * d + col, d - col, f[r]);
+    }
+  }
+}
+
+constexpr long long kMaxGrid = 1 << 22;      // a launch holds fewer than 2^32 threads; the kernels over rows stride beyond it
+
+inline int log2_ceil(long long x) {
+  int l = 0;
+  while ((1ll << l) < x) ++l;
+  return l;
+}
+// lanes that share a row: enough for sixteen bytes each, a workgroup at most
+inline int lanes_log_of(int d, int dtype) {
+  const int vec = dtype == ISTNET_VOCAB_F32 ? 4 : 8, l = log2_ceil((d + vec - 1) / vec);
+  return l > 8 ? 8 : l;
+}
+inline bool embed_ok(long long n, int v, int d, int dtype) {
+  return n >= 1 && n <= (1ll << 30) && v >= 1 && v < 0x7fffffff - 256 && d >= 1 && dtype >= 0 && dtype <= 2;
+}
+
+struct EmbedPlan {
+  int bits, passes, items, nb, longest, pieces;
+  long long keys[2], perm[2], hist, start, part, bytes;      // offsets into the scratch memory
+};
+inline EmbedPlan embed_plan(long long n, int v, int d) {
+  EmbedPlan p = {};
+  const int key_bits = log2_ceil((long long)v + 1), most = n <= kSmallSort ? kSmallDigit : kDigit;
+  p.passes = (key_bits + most - 1) / most;
+  p.bits = (key_bits + p.passes - 1) / p.passes;
+  p.items = n <= 256 * 1024 ? 4 : kSortItems;
+  p.nb = (int)((n + kSortThreads * p.items - 1) / (kSortThreads * p.items));
+  // pieces short enough that one is a few rounds of loads, long enough that the partial sums of one row stay about as many
+  p.longest = 1 << ((log2_ceil(n) + 1) / 2);
+  if (p.longest < 128) p.longest = 128;
+  p.pieces = n > p.longest ? (int)((n + p.longest - 1) / p.longest) : 0;
+  long long at = 0;
+  auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
+  const bool small = n <= kSmallSort;
+  for (int i = 0; i < (small ? 1 : 2); ++i) { p.keys[i] = take(4 * n); p.perm[i] = take(4 * n); }
+  p.hist = small ? 0 : take(4ll * p.nb << p.bits);
+  p.start = take(4ll * (v + 1ll));
+  p.part = p.pieces ? take(8ll * p.pieces * d) : 0;
+  p.bytes = at;
+  return p;
+}
+
+}  // namespace
+
+extern "C" int istnet_embed_forward(long long n, int v, int d, int dtype, int idx64, const void* weight, long long ldw,
+                                    const void* ids, float scale, void* out, void* stream) {
+  if (!embed_ok(n, v, d, dtype) || !weight || !ids || !out || ldw < d) return ISTNET_PN2_EINVAL;
+  const int ll = lanes_log_of(d, dtype);
+  const long long rows = (256 >> ll) * (long long)kLookupRows, grid = std::min((n + rows - 1) / rows, kMaxGrid);
+  VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_lookup_kernel<T>), dim3((unsigned)grid), dim3(256), 0,
+                                              (hipStream_t)stream, n, v, d, ll, idx64, (const T*)weight, ldw, ids, scale, (T*)out));
+  return launch_status();
+}
+
+extern "C" int istnet_embed_scratch_kib(long long n, int v, int d) {
+  if (!embed_ok(n, v, d, 0)) return -1;
+  return (int)((embed_plan(n, v, d).bytes + 1023) / 1024);
+}
+
+extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int idx64, const void* grad, long long ldg,
+                                     const void* ids, long long padding, float scale, void* ws, void* dw, void* stream) {
+  if (!embed_ok(n, v, d, dtype) || !grad || !ids || !ws || !dw || ldg < d) return ISTNET_PN2_EINVAL;
+  const hipStream_t st = (hipStream_t)stream;
+  const EmbedPlan p = embed_plan(n, v, d);
+  char* base = (char*)ws;
+  uint32_t *keys[2], *perm[2];
+  for (int i = 0; i < 2; ++i) { keys[i] = (uint32_t*)(base + p.keys[i]); perm[i] = (uint32_t*)(base + p.perm[i]); }
+  int* start = (int*)(base + p.start);
+  float* part = (float*)(base + p.part);
+  int last = 0;
+  if (n <= kSmallSort) {
+    hipLaunchKernelGGL(embed_sort_small_kernel, dim3(1), dim3(kSmallThreads), 0, st, (int)n, v, ids, idx64, padding, p.bits,
+                       p.passes, keys[0], perm[0]);
+  } else {
+    int* hist = (int*)(base + p.hist);
+    for (int i = 0; i < p.passes; ++i) {
+      const uint32_t* kin = i ? keys[last] : nullptr;
+      const uint32_t* pin = i ? perm[last] : nullptr;
+      const int to = i ? last ^ 1 : 0;
+      hipLaunchKernelGGL(embed_hist_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, i * p.bits,
+                         p.bits, p.items, p.nb, hist);
+      hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, st, (long long)p.nb << p.bits, hist);
+      hipLaunchKernelGGL(embed_scatter_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, pin,
+                         i * p.bits, p.bits, p.items, p.nb, hist, keys[to], perm[to]);
+      last = to;
+    }
+  }
+  hipLaunchKernelGGL(embed_starts_kernel, dim3((unsigned)(v / 256 + 1)), dim3(256), 0, st, (int)n, v, keys[last], start);
+  const int ll = lanes_log_of(d, dtype);
+  const long long rows = (256 >> ll) * (long long)kTeamRows, grid = std::min((v + rows - 1) / rows, kMaxGrid);
+  VOCAB_DISPATCH(dtype, T, {
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, v, d, ll, p.longest,
+                       (const T*)grad, ldg, perm[last], start, scale, (T*)dw);
+    if (p.pieces) {
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_pieces_kernel<T>), dim3(p.pieces), dim3(256), 0, st, (int)n, v, d, ll, p.longest,
+                         (const T*)grad, ldg, keys[last], perm[last], start, part);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_join_kernel<T>), dim3(p.pieces), dim3(256), 0, st, (int)n, v, d, ll, p.longest,
+                         keys[last], start, part, scale, (T*)dw);
+    }
+  });
+  return launch_status();
+}

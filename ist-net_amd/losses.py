@@ -34,6 +34,62 @@ def PoseDis(r1, t1, s1, r2, t2, s2):
             + torch.mean(torch.norm(s1 - s2, dim=1)))
 
 
+def _reduce_rows(rows, counted, reduction):
+    if reduction == "none":
+        return rows
+    return rows.sum() if reduction == "sum" else rows.sum() / counted.sum()
+
+
+def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="mean"):
+    """Distance of a student's ``logits`` (..., V) to a teacher of whom only the K <= 256 largest logits ``top_logits`` (..., K) of
+    the classes ``top_index`` (..., K) were kept:
+
+        q = softmax(top_logits / T) over the used slots,   p = softmax(logits / T) over all V classes,
+        row = T^2 * sum_k q_k (log q_k - log p[top_index_k])
+
+    float32 loss: per row ("none"), their "sum" or their "mean" over the rows that count.  Slots with index -1 are unused
+    (their logits are not looked at); a row without a used slot does not count: loss 0, gradient 0, its logits are not looked at;
+    the mean over no row is NaN.  Slots may repeat a class.  A row with an index outside [-1, V) or with a NaN among its used
+    logits is NaN, loss and gradient.  Differentiable w.r.t. ``logits`` (once).  ``logits`` may be a slice with a row stride, of
+    float32, bfloat16 or float16; the gradient has its type, everything between is float32."""
+    from . import vocab_native as vn
+    vn.require(reduction in vn.REDUCTIONS, f"reduction must be one of {sorted(vn.REDUCTIONS)}, got {reduction!r}", ValueError)
+    temperature = float(temperature)
+    vn.require(0.0 < temperature < float("inf"), f"temperature must be positive and finite, got {temperature}", ValueError)
+    vn.require(logits.dim() >= 1 and top_index.dim() >= 1 and logits.shape[:-1] == top_index.shape[:-1]
+               and top_logits.shape == top_index.shape,
+               f"shapes do not agree: logits {tuple(logits.shape)}, top_logits {tuple(top_logits.shape)}, "
+               f"top_index {tuple(top_index.shape)}", ValueError)
+    v, k = logits.shape[-1], top_index.shape[-1]
+    vn.require(v >= 1 and 1 <= k <= 256, f"needs at least one class and 1 to 256 kept logits, got {v} and {k}", ValueError)
+    vn.require_index(top_index, "top_index")
+    vn.require(not top_logits.requires_grad, "top_logits must not require a gradient: the teacher is fixed", ValueError)
+    vn.require_device(logits, "logits", top_logits=top_logits, top_index=top_index)
+    lead = logits.shape[:-1]
+    z, top, idx = logits.reshape(-1, v), top_logits.reshape(-1, k), top_index.reshape(-1, k)
+    n = z.shape[0]
+    if logits.is_cuda and n:
+        vn.require_float(logits, "logits")
+        vn.require_float(top_logits, "top_logits")
+        vn.require(n <= 1 << 23 and v < 2 ** 31 - 65536, "more than 2^23 rows or too many classes", ValueError)
+        loss = vn.DistillFunction.apply(z, top, idx, temperature, vn.REDUCTIONS[reduction])
+    else:                                            # host: the definition as it is written
+        z = z if z.dtype == torch.float64 else z.float()
+        used, idx = idx != -1, idx.long()
+        counted = used.any(1)
+        t = torch.where(used, top.to(z.dtype) / temperature, -float("inf"))
+        bad = (used & ((idx < 0) | (idx >= v) | t.isnan())).any(1)
+        t = torch.where((counted & ~bad).unsqueeze(1), t, 0.0)
+        log_q = torch.log_softmax(t, 1)
+        live = torch.where(counted.unsqueeze(1), z, 0.0)
+        log_p = torch.log_softmax(live / temperature, 1).gather(1, idx.clamp(0, v - 1))
+        q = log_q.exp()
+        rows = temperature ** 2 * torch.where(used & (q != 0), q * (log_q - log_p), 0.0).sum(1)
+        rows = rows * torch.where(bad, float("nan"), 1.0)
+        loss = _reduce_rows(rows, counted, reduction)
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
 class _WeightedSumFn(torch.autograd.Function):
     """sum_i w_i s_i of scalar terms as one node: stack + dot forward, one scaled copy of the weights backward -- the
     reference's chain ``loss = a + b + g1 * c + g2 * d + e`` (model/ist_net.py:95-110) is four adds and two multiplies

@@ -15,6 +15,7 @@ import torch
 import torch.nn as nn
 from torch.autograd import Function
 
+from .. import vocab_native
 from . import _ext
 
 
@@ -129,6 +130,46 @@ class GroupingOperation(Function):
 
 
 grouping_operation = GroupingOperation.apply
+
+
+def embedding_operation(weight, idx, scale=1.0, padding_idx=None):
+    """weight (V,D), idx (...) i32 or i64 -> scale * weight[idx] (...,D), in weight's type (float32, bfloat16, float16).
+
+    An extension of the reference's operators: the row-major sibling of ``gather_operation`` for tables indexed by category, cell
+    or token.  The product is formed in float32 and rounded once.  Differentiable w.r.t. ``weight``: the gradient (V,D) is dense,
+    its rows are summed in float32 in the order of the indices (deterministic) and rounded once; row ``padding_idx`` gets none.
+    An index outside [0, V) is not looked up: its output row is NaN and its gradient is dropped (nothing synchronises to raise).
+    ``idx`` may repeat, be empty and have any shape; ``weight`` may be a slice with a row stride.  CUDA only."""
+    if not weight.is_cuda:
+        raise RuntimeError("CPU not supported")
+    vocab_native.require(weight.dim() == 2 and weight.shape[0] >= 1 and weight.shape[1] >= 1,
+                         f"weight must be a non-empty (V, D) tensor, got {tuple(weight.shape)}", ValueError)
+    vocab_native.require_float(weight, "weight")
+    vocab_native.require_index(idx, "idx")
+    vocab_native.require(idx.is_cuda, "idx must be a CUDA tensor")
+    vocab_native.require_device(weight, "weight", idx=idx)
+    vocab_native.require(idx.numel() <= 1 << 30, "idx holds more than 2^30 indices", ValueError)
+    vocab_native.require(weight.shape[0] < 2 ** 31 - 257 and weight.shape[1] < 2 ** 31 - 2048, "weight is too large", ValueError)
+    if padding_idx is not None:
+        vocab_native.require(0 <= padding_idx < weight.shape[0], f"padding_idx must be a row of weight, got {padding_idx}", ValueError)
+    return vocab_native.EmbeddingFunction.apply(weight, idx, float(scale), padding_idx)
+
+
+class ScaledEmbedding(nn.Module):
+    """A (num_rows, width) table with normal(0, width ** -0.5) rows looked up by ``embedding_operation``; ``scale`` defaults to
+    sqrt(width), so that looked-up rows have unit variance.  Row ``padding_idx`` starts at zero and stays there."""
+
+    def __init__(self, num_rows, width, scale=None, padding_idx=None):
+        super().__init__()
+        self.scale = float(width) ** 0.5 if scale is None else float(scale)
+        self.padding_idx = padding_idx
+        self.weight = nn.Parameter(torch.empty(num_rows, width).normal_(0.0, float(width) ** -0.5))
+        if padding_idx is not None:
+            with torch.no_grad():
+                self.weight[padding_idx].zero_()
+
+    def forward(self, idx):
+        return embedding_operation(self.weight, idx, self.scale, self.padding_idx)
 
 
 class BallQuery(Function):

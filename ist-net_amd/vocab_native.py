@@ -1,0 +1,131 @@
+"""Native operators at the two ends of a model with discrete classes (csrc/vocab/, include/istnet_vocab.h): the scaled table
+lookup with its gradient by sorted indices (``pointnet2_utils.embedding_operation``) and the distance to a teacher's top logits
+(``losses.TopLogitsDistill``).
+
+CUDA tensors of float32, bfloat16 or float16 run the kernels or raise; there is no fallback on the GPU.  CPU tensors (host-logic
+tests) take the literal torch composition in the callers.  Nothing synchronises and nothing is kept between calls: every call
+takes its scratch memory from torch's allocator on the current stream, so calls on several streams and captured graphs do not
+share any.
+"""
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def require(cond, msg, kind=RuntimeError):
+    if not cond:
+        raise kind(msg)
+
+
+def require_float(t, name):
+    require(t.dtype in DTYPES, f"{name} must be a float32, bfloat16 or float16 tensor, got {t.dtype}", TypeError)
+
+
+def require_index(t, name):
+    require(t.dtype in (torch.int32, torch.int64), f"{name} must be an int32 or int64 tensor, got {t.dtype}", TypeError)
+
+
+def require_device(lead, name, **others):
+    for other, t in others.items():
+        require(t.device == lead.device, f"{other} must be on the same device as {name}")
+
+
+def _st(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _rows(t):
+    """(tensor, leading dimension) of a 2-D operand with contiguous rows that do not overlap; anything else is copied."""
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    if t.shape[1] == 1 and t.stride(0) >= 1:
+        return t, t.stride(0)
+    if t.shape[0] == 1 and t.stride(1) == 1:
+        return t, t.shape[1]
+    t = t.contiguous()
+    return t, t.shape[1]
+
+
+def _scratch(kib, dev):
+    return torch.empty(max(kib, 1) * 1024, dtype=torch.uint8, device=dev)
+
+
+class EmbeddingFunction(Function):
+    """weight (V, D), idx (...) -> scale * weight[idx] (..., D); gradient for weight."""
+
+    @staticmethod
+    def forward(ctx, weight, idx, scale, padding):
+        dev, (v, d), n = weight.device, weight.shape, idx.numel()
+        out = torch.empty((*idx.shape, d), dtype=weight.dtype, device=dev)
+        ids = idx.contiguous()
+        if n:
+            w, ldw = _rows(weight)
+            with torch.cuda.device(dev):
+                _native.check(_native.lib().istnet_embed_forward(
+                    n, v, d, DTYPES[weight.dtype], int(ids.dtype == torch.int64), w.data_ptr(), ldw, ids.data_ptr(), scale,
+                    out.data_ptr(), _st(dev)), "embed_forward")
+        ctx.save_for_backward(ids)
+        ctx.args = (v, d, scale, padding, weight.dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        (ids,) = ctx.saved_tensors
+        v, d, scale, padding, dtype = ctx.args
+        dev, n = ids.device, ids.numel()
+        if n == 0:
+            return torch.zeros((v, d), dtype=dtype, device=dev), None, None, None
+        g, ldg = _rows(grad_out.reshape(n, d))
+        dw = torch.empty((v, d), dtype=dtype, device=dev)
+        lib = _native.lib()
+        ws = _scratch(lib.istnet_embed_scratch_kib(n, v, d), dev)
+        with torch.cuda.device(dev):
+            _native.check(lib.istnet_embed_backward(
+                n, v, d, DTYPES[dtype], int(ids.dtype == torch.int64), g.data_ptr(), ldg, ids.data_ptr(),
+                -1 if padding is None else padding, scale, ws.data_ptr(), dw.data_ptr(), _st(dev)), "embed_backward")
+        return dw, None, None, None
+
+
+class DistillFunction(Function):
+    """logits (N, V), top (N, K), idx (N, K) -> loss (N,) or scalar, float32; gradient for logits."""
+
+    @staticmethod
+    def forward(ctx, logits, top, idx, temperature, reduction):
+        dev, (n, v), k = logits.device, logits.shape, idx.shape[1]
+        lib = _native.lib()
+        z, ldz = _rows(logits)
+        top, ids = top.contiguous(), idx.contiguous()
+        loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+        keep = torch.empty(n * (2 + k) + 1, dtype=torch.float32, device=dev)      # stats (n, 2), q (n, k), count
+        ws = _scratch(lib.istnet_distill_scratch_kib(n, v, k), dev)
+        at = keep.data_ptr()
+        with torch.cuda.device(dev):
+            _native.check(lib.istnet_distill_forward(
+                n, v, k, DTYPES[z.dtype], DTYPES[top.dtype], int(ids.dtype == torch.int64), z.data_ptr(), ldz, top.data_ptr(),
+                ids.data_ptr(), temperature, reduction, loss.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), ws.data_ptr(),
+                _st(dev)), "distill_forward")
+        ctx.save_for_backward(logits, ids, keep)
+        ctx.args = (temperature, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        logits, ids, keep = ctx.saved_tensors
+        temperature, reduction = ctx.args
+        dev, (n, v), k = logits.device, logits.shape, ids.shape[1]
+        z, ldz = _rows(logits)
+        gout = gout.contiguous()
+        dz = torch.empty((n, v), dtype=logits.dtype, device=dev)
+        at = keep.data_ptr()
+        with torch.cuda.device(dev):
+            _native.check(_native.lib().istnet_distill_backward(
+                n, v, k, DTYPES[z.dtype], int(ids.dtype == torch.int64), z.data_ptr(), ldz, ids.data_ptr(), temperature, reduction,
+                gout.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), dz.data_ptr(), _st(dev)), "distill_backward")
+        return dz, None, None, None, None

@@ -1,0 +1,120 @@
+"""Host logic of the vocabulary operators: refusals, empty calls, and the definitions as the CPU composition evaluates them
+(float64 inputs are evaluated in float64, so the formulas are checked to rounding and their gradients against differences)."""
+import math
+
+import pytest
+import torch
+
+from istnet_amd import losses
+from istnet_amd.pointnet2 import pointnet2_utils
+
+INF = float("inf")
+
+
+def _distill_rows(z, top, idx, temp):
+    """The definition, one row and one slot at a time."""
+    out = []
+    for zr, tr, ir in zip(z.tolist(), top.tolist(), idx.tolist()):
+        used = [(t, i) for t, i in zip(tr, ir) if i != -1]
+        if not used:
+            out.append(0.0)
+            continue
+        zmax, tmax = max(zr), max(t for t, _ in used)
+        zsum = sum(math.exp((x - zmax) / temp) for x in zr)
+        tsum = sum(math.exp((t - tmax) / temp) for t, _ in used)
+        row = 0.0
+        for t, i in used:
+            log_q = (t - tmax) / temp - math.log(tsum)
+            log_p = (zr[i] - zmax) / temp - math.log(zsum)
+            row += math.exp(log_q) * (log_q - log_p) if t > -INF else 0.0
+        out.append(temp * temp * row)
+    return torch.tensor(out, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("n,v,k,temp", [(1, 1, 1, 1.0), (1, 7, 3, 2.0), (5, 33, 8, 0.5), (4, 9, 9, 1.0)])
+def test_distill_composition_is_the_definition(n, v, k, temp):
+    g = torch.Generator().manual_seed(n + v + k)
+    z = torch.randn(n, v, generator=g, dtype=torch.float64).requires_grad_()
+    top = torch.randn(n, k, generator=g, dtype=torch.float64)
+    idx = torch.randint(0, v, (n, k), generator=g)                 # repeats a class now and then
+    idx[0, k // 2:] = -1
+    top[0, k // 2:] = float("nan")                                 # unused: not looked at
+    want = _distill_rows(z.detach(), top, idx, temp)
+    torch.testing.assert_close(losses.TopLogitsDistill(z, top, idx, temp, "none"), want, rtol=1e-12, atol=1e-12)
+    counted = (idx != -1).any(1).sum()
+    torch.testing.assert_close(losses.TopLogitsDistill(z, top, idx, temp, "sum"), want.sum(), rtol=1e-12, atol=1e-12)
+    mean = losses.TopLogitsDistill(z, top, idx, temp)
+    if counted:
+        torch.testing.assert_close(mean, want.sum() / counted, rtol=1e-12, atol=1e-12)
+        assert torch.autograd.gradcheck(lambda x: losses.TopLogitsDistill(x, top, idx, temp, "none"), (z,))
+    else:
+        assert mean.isnan()
+
+
+def test_distill_composition_odd_rows():
+    z = torch.tensor([[1.0, 2.0, -INF], [float("nan")] * 3, [0.0, 1.0, 2.0], [0.0, 1.0, 2.0], [0.0, 1.0, 2.0]],
+                     dtype=torch.float64, requires_grad=True)
+    top = torch.tensor([[1.0, 0.0], [1.0, 1.0], [1.0, -INF], [1.0, 2.0], [float("nan"), 0.0]], dtype=torch.float64)
+    idx = torch.tensor([[0, 1], [-1, -1], [2, 0], [0, 3], [1, 2]])
+    rows = losses.TopLogitsDistill(z, top, idx, 1.0, "none")
+    assert rows[0].isfinite() and rows[1] == 0.0 and rows[2].isfinite() and rows[3].isnan() and rows[4].isnan()
+    rows[:3].sum().backward()
+    assert z.grad[0].isfinite().all() and (z.grad[1] == 0).all() and z.grad[2].isfinite().all()
+    # a class of weight zero changes nothing
+    alone = losses.TopLogitsDistill(z[2:3], top[2:3, :1], idx[2:3, :1], 1.0, "none")
+    torch.testing.assert_close(rows[2:3], alone)
+
+
+def test_distill_refusals():
+    z, top, idx = torch.randn(4, 10), torch.randn(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    call = losses.TopLogitsDistill
+    with pytest.raises(ValueError, match="reduction"):
+        call(z, top, idx, reduction="batchmean")
+    for bad in (0.0, -1.0, INF, float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            call(z, top, idx, bad)
+    with pytest.raises(ValueError, match="shapes"):
+        call(z, top[:, :2], idx)
+    with pytest.raises(ValueError, match="shapes"):
+        call(z[:3], top, idx)
+    with pytest.raises(ValueError, match="1 to 256"):
+        call(z, top[:, :0], idx[:, :0])
+    with pytest.raises(ValueError, match="1 to 256"):
+        call(z, torch.randn(4, 257), torch.zeros(4, 257, dtype=torch.int64))
+    with pytest.raises(TypeError, match="top_index"):
+        call(z, top, idx.float())
+    with pytest.raises(ValueError, match="teacher"):
+        call(z, top.requires_grad_(), idx)
+
+
+def test_distill_without_rows():
+    z = torch.zeros(0, 5, requires_grad=True)
+    top, idx = torch.zeros(0, 2), torch.zeros(0, 2, dtype=torch.int32)
+    assert losses.TopLogitsDistill(z, top, idx, reduction="none").shape == (0,)
+    assert losses.TopLogitsDistill(z, top, idx, reduction="sum") == 0.0
+    assert losses.TopLogitsDistill(z, top, idx).isnan()
+
+
+def test_embedding_refuses_the_cpu():
+    with pytest.raises(RuntimeError, match="CPU not supported"):
+        pointnet2_utils.embedding_operation(torch.randn(3, 4), torch.zeros(2, dtype=torch.int64))
+
+
+def test_entry_points_reject_invalid_arguments():
+    """Sizes, types and pointers are checked before anything touches a device."""
+    from istnet_amd import _native
+    lib = _native.lib()
+    bad, one = 100001, 16
+    assert lib.istnet_embed_forward(0, 4, 4, 0, 0, one, 4, one, 1.0, one, None) == bad
+    assert lib.istnet_embed_forward(4, 4, 4, 3, 0, one, 4, one, 1.0, one, None) == bad
+    assert lib.istnet_embed_forward(4, 4, 4, 0, 0, one, 3, one, 1.0, one, None) == bad
+    assert lib.istnet_embed_forward(4, 4, 4, 0, 0, None, 4, one, 1.0, one, None) == bad
+    assert lib.istnet_embed_backward(4, 4, 4, 0, 0, one, 4, one, -1, 1.0, None, one, None) == bad
+    assert lib.istnet_embed_backward((1 << 30) + 1, 4, 4, 0, 0, one, 4, one, -1, 1.0, one, one, None) == bad
+    assert lib.istnet_embed_scratch_kib(0, 4, 4) == -1 and lib.istnet_embed_scratch_kib(1, 1, 1) >= 1
+    forward = lambda n, v, k, t, red, z=one: lib.istnet_distill_forward(n, v, k, 0, 0, 0, z, v, one, one, t, red, one, one, one, one,
+                                                                        one, None)
+    assert forward(0, 4, 2, 1.0, 1) == forward(4, 0, 2, 1.0, 1) == forward(4, 4, 0, 1.0, 1) == forward(4, 4, 257, 1.0, 1) == bad
+    assert forward(4, 4, 2, 0.0, 1) == forward(4, 4, 2, 1.0, 3) == forward(4, 4, 2, 1.0, 1, None) == bad
+    assert lib.istnet_distill_backward(4, 4, 2, 0, 0, one, 3, one, 1.0, 1, one, one, one, one, one, None) == bad
+    assert lib.istnet_distill_scratch_kib(1, 1, 257) == -1 and lib.istnet_distill_scratch_kib(1, 1, 1) >= 1
