@@ -18,6 +18,7 @@ constexpr int kSmallThreads = 1024;
 constexpr int kSmallDigit = 6;        // bits of a digit there: 64 digits x 16 waves = one counter per thread
 constexpr int kDigit = 9;             // most bits of a digit of the sort over many workgroups
 constexpr int kSortThreads = 256;
+constexpr int kFewBlocks = 64;        // workgroups up to which the scatter adds up the digit counts of all of them (saves a launch)
 constexpr int kSortItems = 16;        // tokens per thread and workgroup of that sort
 
 __device__ __forceinline__ uint32_t key_of(const void* ids, long long i, int idx64, int v, long long padding) {
@@ -149,7 +150,8 @@ __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(int n, int v, 
     }
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[(long long)d * nb + b] = cnt[d];
+  // few workgroups: counts of one workgroup side by side, added up by the scatter itself; many: digit by digit, for the scan
+  for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[nb <= kFewBlocks ? (long long)b * radix + d : (long long)d * nb + b] = cnt[d];
 }
 
 __global__ __launch_bounds__(1024) void embed_scan_kernel(long long count, int* __restrict__ hist) {
@@ -181,6 +183,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int 
                                                                      uint32_t* __restrict__ keys_out, uint32_t* __restrict__ perm_out) {
   constexpr int WAVES = kSortThreads / 64;
   __shared__ int cnt[WAVES][1 << kDigit];
+  __shared__ int tmp[WAVES];
   const int radix = 1 << bits, b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int d = lane; d < radix; d += 64) cnt[wave][d] = 0;
   __syncthreads();
@@ -197,13 +200,48 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int 
     }
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += kSortThreads) {
-    int at = hist[(long long)d * nb + b];
+  constexpr int PER = (1 << kDigit) / kSortThreads;      // digits of a thread: PER consecutive ones
+  int at[PER];
+  if (nb <= kFewBlocks) {
+    int before[PER] = {}, total[PER] = {};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const int c = cnt[w][d];
-      cnt[w][d] = at;
-      at += c;
+    for (int j = 0; j < PER; ++j) {
+      const int d = threadIdx.x * PER + j;
+      if (d < radix) {
+#pragma unroll 8
+        for (int o = 0; o < nb; ++o) {
+          const int c = hist[(long long)o * radix + d];
+          total[j] += c;
+          before[j] += o < b ? c : 0;
+        }
+      }
+    }
+    int mine = 0, all;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine += total[j];
+    int from = block_exclusive<kSortThreads>(mine, tmp, &all);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      at[j] = from + before[j];
+      from += total[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int d = threadIdx.x * PER + j;
+      at[j] = d < radix ? hist[(long long)d * nb + b] : 0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int d = threadIdx.x * PER + j;
+    if (d < radix) {
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const int c = cnt[w][d];
+        cnt[w][d] = at[j];
+        at[j] += c;
+      }
     }
   }
   __syncthreads();
@@ -230,19 +268,25 @@ __global__ __launch_bounds__(256) void embed_starts_kernel(int n, int v, const u
   start[t] = lo;
 }
 
-// sum of the gradient rows of sorted tokens [a, e), elements [col, col + left), four loads in flight, added in order
+// sum of the gradient rows of sorted tokens [a, e), elements [col, col + left), eight loads in flight, added in order
 template <typename T>
 __device__ __forceinline__ void sum_run(const T* __restrict__ grad, long long ldg, const uint32_t* __restrict__ perm, int a, int e,
                                         int col, int left, float (&acc)[kVec<T>]) {
+  constexpr int U = 8;
   int p = a;
-  for (; p + 4 <= e; p += 4) {
-    float f[4][kVec<T>];
+  if (left >= kVec<T>) {
+    for (; p + U <= e; p += U) {
+      u32x4 raw[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load_part(grad + (long long)perm[p + j] * ldg + col, left, f[j]);
+      for (int j = 0; j < U; ++j) raw[j] = load16(grad + (long long)perm[p + j] * ldg + col);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < U; ++j) {
+        float f[kVec<T>];
+        unpack<T>(raw[j], f);
 #pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) acc[i] += f[j][i];
+        for (int i = 0; i < kVec<T>; ++i) acc[i] += f[i];
+      }
+    }
   }
   for (; p < e; ++p) {
     float f[kVec<T>];
@@ -252,27 +296,33 @@ __device__ __forceinline__ void sum_run(const T* __restrict__ grad, long long ld
   }
 }
 
-constexpr int kTeamRows = 4;      // consecutive table rows per team of lanes
+constexpr int kTeamRows = 4;      // table rows per team of lanes
 
+// The rows of a team are far apart: frequent indices are often neighbours, and one team would have to add up several of them.
 template <typename T>
 __global__ __launch_bounds__(256) void embed_rows_kernel(int v, int d, int lanes_log, int longest, const T* __restrict__ grad,
                                                          long long ldg, const uint32_t* __restrict__ perm,
                                                          const int* __restrict__ start, float scale, T* __restrict__ dw) {
   const int lanes = 1 << lanes_log, at = threadIdx.x & (lanes - 1);
-  const long long step = (long long)gridDim.x * kTeamRows << (8 - lanes_log);
-  for (long long row0 = (((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log)) * kTeamRows; row0 < v; row0 += step) {
-    int s[kTeamRows + 1];
+  const long long teams = (long long)gridDim.x << (8 - lanes_log);
+  for (long long row0 = ((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log); row0 < v; row0 += teams * kTeamRows) {
+    int s[kTeamRows], e[kTeamRows];
 #pragma unroll
-    for (int r = 0; r <= kTeamRows; ++r) s[r] = start[row0 + r < v ? row0 + r : v];
+    for (int r = 0; r < kTeamRows; ++r) {
+      const long long row = row0 + r * teams;
+      s[r] = start[row < v ? row : v];
+      e[r] = start[row < v ? row + 1 : v];
+    }
     for (int col = at * kVec<T>; col < d; col += lanes * kVec<T>) {
 #pragma unroll
       for (int r = 0; r < kTeamRows; ++r) {
-        if (row0 + r < v && s[r + 1] - s[r] <= longest) {
+        const long long row = row0 + r * teams;
+        if (row < v && e[r] - s[r] <= longest) {
           float acc[kVec<T>] = {};
-          sum_run(grad, ldg, perm, s[r], s[r + 1], col, d - col, acc);
+          sum_run(grad, ldg, perm, s[r], e[r], col, d - col, acc);
 #pragma unroll
           for (int i = 0; i < kVec<T>; ++i) acc[i] *= scale;
-          store_part(dw + (row0 + r) * d + col, d - col, acc);
+          store_part(dw + row * d + col, d - col, acc);
         }
       }
     }
@@ -345,6 +395,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(int n, int v, int d, in
     const int col = c0 + at * kVec<T>;
     float acc[kVec<T>] = {};
     if (col < d) {
+#pragma unroll 8
       for (int q = a; q < b; ++q) {
         const float* o = part + ((long long)q * 2 + (s > q * longest ? 1 : 0)) * d + col;
 #pragma unroll
@@ -422,9 +473,8 @@ inline EmbedPlan embed_plan(long long n, int v, int d) {
   p.bits = (key_bits + p.passes - 1) / p.passes;
   p.items = n <= 256 * 1024 ? 4 : kSortItems;
   p.nb = (int)((n + kSortThreads * p.items - 1) / (kSortThreads * p.items));
-  // pieces short enough that one is a few rounds of loads, long enough that the partial sums of one row stay about as many
-  p.longest = 1 << ((log2_ceil(n) + 1) / 2);
-  if (p.longest < 128) p.longest = 128;
+  // pieces short enough that one is a few rounds of loads, long enough that the partial sums of one row do not become many
+  p.longest = std::max(32, (1 << ((log2_ceil(n) + 1) / 2)) / 8);
   p.pieces = n > p.longest ? (int)((n + p.longest - 1) / p.longest) : 0;
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
@@ -476,7 +526,8 @@ extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int i
       const int to = i ? last ^ 1 : 0;
       hipLaunchKernelGGL(embed_hist_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, i * p.bits,
                          p.bits, p.items, p.nb, hist);
-      hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, st, (long long)p.nb << p.bits, hist);
+      if (p.nb > kFewBlocks)
+        hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, st, (long long)p.nb << p.bits, hist);
       hipLaunchKernelGGL(embed_scatter_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, pin,
                          i * p.bits, p.bits, p.items, p.nb, hist, keys[to], perm[to]);
       last = to;

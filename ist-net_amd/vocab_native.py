@@ -35,8 +35,13 @@ def require_device(lead, name, **others):
         require(t.device == lead.device, f"{other} must be on the same device as {name}")
 
 
-def _st(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+def _launch(dev, what, fn, *args):
+    """fn(*args, current stream of dev) with dev as the current device, which it nearly always is already."""
+    if torch.cuda.current_device() == dev.index:
+        _native.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+    else:
+        with torch.cuda.device(dev):
+            _native.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
 
 
 def _rows(t):
@@ -65,10 +70,8 @@ class EmbeddingFunction(Function):
         ids = idx.contiguous()
         if n:
             w, ldw = _rows(weight)
-            with torch.cuda.device(dev):
-                _native.check(_native.lib().istnet_embed_forward(
-                    n, v, d, DTYPES[weight.dtype], int(ids.dtype == torch.int64), w.data_ptr(), ldw, ids.data_ptr(), scale,
-                    out.data_ptr(), _st(dev)), "embed_forward")
+            _launch(dev, "embed_forward", _native.lib().istnet_embed_forward, n, v, d, DTYPES[weight.dtype],
+                    ids.dtype == torch.int64, w.data_ptr(), ldw, ids.data_ptr(), scale, out.data_ptr())
         ctx.save_for_backward(ids)
         ctx.args = (v, d, scale, padding, weight.dtype)
         return out
@@ -85,10 +88,8 @@ class EmbeddingFunction(Function):
         dw = torch.empty((v, d), dtype=dtype, device=dev)
         lib = _native.lib()
         ws = _scratch(lib.istnet_embed_scratch_kib(n, v, d), dev)
-        with torch.cuda.device(dev):
-            _native.check(lib.istnet_embed_backward(
-                n, v, d, DTYPES[dtype], int(ids.dtype == torch.int64), g.data_ptr(), ldg, ids.data_ptr(),
-                -1 if padding is None else padding, scale, ws.data_ptr(), dw.data_ptr(), _st(dev)), "embed_backward")
+        _launch(dev, "embed_backward", lib.istnet_embed_backward, n, v, d, DTYPES[dtype], ids.dtype == torch.int64, g.data_ptr(),
+                ldg, ids.data_ptr(), -1 if padding is None else padding, scale, ws.data_ptr(), dw.data_ptr())
         return dw, None, None, None
 
 
@@ -105,11 +106,9 @@ class DistillFunction(Function):
         keep = torch.empty(n * (2 + k) + 1, dtype=torch.float32, device=dev)      # stats (n, 2), q (n, k), count
         ws = _scratch(lib.istnet_distill_scratch_kib(n, v, k), dev)
         at = keep.data_ptr()
-        with torch.cuda.device(dev):
-            _native.check(lib.istnet_distill_forward(
-                n, v, k, DTYPES[z.dtype], DTYPES[top.dtype], int(ids.dtype == torch.int64), z.data_ptr(), ldz, top.data_ptr(),
-                ids.data_ptr(), temperature, reduction, loss.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), ws.data_ptr(),
-                _st(dev)), "distill_forward")
+        _launch(dev, "distill_forward", lib.istnet_distill_forward, n, v, k, DTYPES[z.dtype], DTYPES[top.dtype],
+                ids.dtype == torch.int64, z.data_ptr(), ldz, top.data_ptr(), ids.data_ptr(), temperature, reduction,
+                loss.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), ws.data_ptr())
         ctx.save_for_backward(logits, ids, keep)
         ctx.args = (temperature, reduction)
         return loss
@@ -124,8 +123,7 @@ class DistillFunction(Function):
         gout = gout.contiguous()
         dz = torch.empty((n, v), dtype=logits.dtype, device=dev)
         at = keep.data_ptr()
-        with torch.cuda.device(dev):
-            _native.check(_native.lib().istnet_distill_backward(
-                n, v, k, DTYPES[z.dtype], int(ids.dtype == torch.int64), z.data_ptr(), ldz, ids.data_ptr(), temperature, reduction,
-                gout.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), dz.data_ptr(), _st(dev)), "distill_backward")
+        _launch(dev, "distill_backward", _native.lib().istnet_distill_backward, n, v, k, DTYPES[z.dtype],
+                ids.dtype == torch.int64, z.data_ptr(), ldz, ids.data_ptr(), temperature, reduction, gout.data_ptr(), at,
+                at + 8 * n, at + 4 * n * (2 + k), dz.data_ptr())
         return dz, None, None, None, None
