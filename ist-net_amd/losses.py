@@ -90,6 +90,49 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
     return loss.reshape(lead) if reduction == "none" else loss
 
 
+def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of a linear head -- ``nn.functional.cross_entropy(features @ weight.T + bias, target)`` -- that never
+    holds the logits: ``features`` (..., D), ``weight`` (V, D), ``bias`` (V), all of one type (float32, bfloat16, float16), ``target``
+    (...) int32 or int64.
+
+    float32 loss: per row ("none"), their "sum" or their "mean" over the rows that count.  Rows whose target is ``ignore_index`` do
+    not count: loss 0, gradient 0, their features are not looked at; the mean over no row is NaN.  A target outside [0, V) makes its
+    row NaN, and with it the gradients it enters (nothing synchronises to raise).  Differentiable (once) w.r.t. features, weight and
+    bias; the gradients have their types.  Sums are float32; the derivative of the logits is rounded to the operands' type (float32
+    operands: both are held as two float16 numbers to a common power of two, 22 bits, with an absolute error of 2^-39 of the
+    largest entry below that).  The backward forms the logits a second time instead of keeping them."""
+    from . import vocab_native as vn
+    vn.require(reduction in vn.REDUCTIONS, f"reduction must be one of {sorted(vn.REDUCTIONS)}, got {reduction!r}", ValueError)
+    vn.require(features.dim() >= 1 and weight.dim() == 2 and features.shape[-1] == weight.shape[1]
+               and target.shape == features.shape[:-1] and (bias is None or bias.shape == weight.shape[:1]),
+               f"shapes do not agree: features {tuple(features.shape)}, weight {tuple(weight.shape)}, target {tuple(target.shape)}"
+               + ("" if bias is None else f", bias {tuple(bias.shape)}"), ValueError)
+    v, d = weight.shape
+    vn.require(v >= 1 and d >= 1, f"weight must not be empty, got {(v, d)}", ValueError)
+    vn.require_index(target, "target")
+    vn.require(weight.dtype == features.dtype and (bias is None or bias.dtype == features.dtype),
+               f"features ({features.dtype}), weight ({weight.dtype}) and bias must have one type", TypeError)
+    vn.require_device(features, "features", weight=weight, target=target, **({} if bias is None else {"bias": bias}))
+    ignore_index = int(ignore_index)
+    x, t = features.reshape(-1, d), target.reshape(-1)
+    n = x.shape[0]
+    if features.is_cuda and n:
+        vn.require_float(features, "features")
+        vn.require(n <= 1 << 22 and d <= 1 << 20 and v <= 1 << 28 and -(-n // 128) * -(-v // 256) <= 1 << 23,
+                   f"{n} rows of {d} features and {v} classes are too many for one call", ValueError)
+        loss = vn.LinearCEFunction.apply(x, weight, bias, t, ignore_index, vn.REDUCTIONS[reduction])
+    else:                                            # host: the definition as it is written
+        kind = torch.float64 if features.dtype == torch.float64 else torch.float32
+        counted = t != ignore_index
+        bad = counted & ((t < 0) | (t >= v))
+        z = torch.where(counted.unsqueeze(1), x.to(kind), 0.0) @ weight.to(kind).t()
+        z = z if bias is None else z + bias.to(kind)
+        rows = -torch.log_softmax(z, 1).gather(1, t.long().clamp(0, v - 1).unsqueeze(1)).squeeze(1)
+        rows = torch.where(counted, rows, 0.0) * torch.where(bad, float("nan"), 1.0)
+        loss = _reduce_rows(rows, counted, reduction)
+    return loss.reshape(target.shape) if reduction == "none" else loss
+
+
 class _WeightedSumFn(torch.autograd.Function):
     """sum_i w_i s_i of scalar terms as one node: stack + dot forward, one scaled copy of the weights backward -- the
     reference's chain ``loss = a + b + g1 * c + g2 * d + e`` (model/ist_net.py:95-110) is four adds and two multiplies

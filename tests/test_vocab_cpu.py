@@ -118,3 +118,75 @@ def test_entry_points_reject_invalid_arguments():
     assert forward(4, 4, 2, 0.0, 1) == forward(4, 4, 2, 1.0, 3) == forward(4, 4, 2, 1.0, 1, None) == bad
     assert lib.istnet_distill_backward(4, 4, 2, 0, 0, one, 3, one, 1.0, 1, one, one, one, one, one, None) == bad
     assert lib.istnet_distill_scratch_kib(1, 1, 257) == -1 and lib.istnet_distill_scratch_kib(1, 1, 1) >= 1
+
+
+@pytest.mark.parametrize("n,d,v", [(1, 1, 1), (4, 3, 7), (9, 5, 2)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_linear_ce_composition_is_the_definition(n, d, v, with_bias):
+    g = torch.Generator().manual_seed(n + d + v)
+    x = torch.randn(n, d, generator=g, dtype=torch.float64).requires_grad_()
+    w = torch.randn(v, d, generator=g, dtype=torch.float64).requires_grad_()
+    b = torch.randn(v, generator=g, dtype=torch.float64).requires_grad_() if with_bias else None
+    t = torch.randint(0, v, (n,), generator=g)
+    t[n // 2] = 255                                                # does not count
+    rows = []
+    for i in range(n):
+        z = [sum(float(x[i, c] * w[k, c]) for c in range(d)) + (float(b[k]) if with_bias else 0.0) for k in range(v)]
+        rows.append(0.0 if t[i] == 255 else math.log(sum(math.exp(a) for a in z)) - z[int(t[i])])
+    want = torch.tensor(rows, dtype=torch.float64)
+    call = lambda *a, r: losses.LinearCrossEntropy(a[0], a[1], t, a[2] if with_bias else None, 255, r)
+    args = (x, w, b) if with_bias else (x, w)
+    torch.testing.assert_close(call(*args, r="none"), want, rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(call(*args, r="sum"), want.sum(), rtol=1e-12, atol=1e-12)
+    if n > 1:
+        torch.testing.assert_close(call(*args, r="mean"), want.sum() / (n - 1), rtol=1e-12, atol=1e-12)
+    else:
+        assert call(*args, r="mean").isnan()
+    assert torch.autograd.gradcheck(lambda *a: call(*a, r="none"), args)
+
+
+def test_linear_ce_composition_odd_rows():
+    x = torch.randn(4, 3, dtype=torch.float64)
+    x[1] = float("nan")
+    w = torch.randn(5, 3, dtype=torch.float64)
+    x.requires_grad_()
+    rows = losses.LinearCrossEntropy(x, w, torch.tensor([2, -100, 5, -7]), reduction="none")
+    assert rows[0].isfinite() and rows[1] == 0.0 and rows[2].isnan() and rows[3].isnan()
+    rows[:2].sum().backward()
+    assert x.grad[0].isfinite().all() and (x.grad[1] == 0).all()
+    empty = losses.LinearCrossEntropy(torch.zeros(0, 3), torch.zeros(5, 3), torch.zeros(0, dtype=torch.int64))
+    assert empty.isnan() and losses.LinearCrossEntropy(torch.zeros(0, 3), torch.zeros(5, 3), torch.zeros(0, dtype=torch.int64),
+                                                       reduction="none").shape == (0,)
+
+
+def test_linear_ce_refusals():
+    x, w, t = torch.randn(4, 6), torch.randn(5, 6), torch.zeros(4, dtype=torch.int64)
+    call = losses.LinearCrossEntropy
+    with pytest.raises(ValueError, match="reduction"):
+        call(x, w, t, reduction="batch")
+    with pytest.raises(ValueError, match="shapes"):
+        call(x, w[:, :5], t)
+    with pytest.raises(ValueError, match="shapes"):
+        call(x, w, t[:3])
+    with pytest.raises(ValueError, match="shapes"):
+        call(x, w, t, torch.randn(4))
+    with pytest.raises(ValueError, match="empty"):
+        call(x, w[:0], t)
+    with pytest.raises(TypeError, match="target"):
+        call(x, w, t.float())
+    with pytest.raises(TypeError, match="one type"):
+        call(x, w.half(), t)
+    with pytest.raises(TypeError, match="one type"):
+        call(x, w, t, torch.randn(5).half())
+
+
+def test_linear_ce_entry_points_reject_invalid_arguments():
+    from istnet_amd import _native
+    lib = _native.lib()
+    bad, one = 100001, 16
+    forward = lambda n=4, d=8, v=5, dt=0, x=one, ldx=8, ldw=8, red=1: lib.istnet_linear_ce_forward(
+        n, d, v, dt, 1, x, ldx, one, ldw, None, one, -100, red, one, one, one, None)
+    assert forward(n=0) == forward(d=0) == forward(v=0) == forward(dt=3) == forward(x=None) == forward(ldx=7) == forward(ldw=7) == bad
+    assert forward(red=3) == forward(n=(1 << 22) + 1) == forward(n=1 << 22, v=1 << 28) == bad
+    assert lib.istnet_linear_ce_backward(4, 8, 5, 0, one, 8, one, 8, 0, 1, None, one, one, one, one, None, None) == bad
+    assert lib.istnet_linear_ce_keep_kib(0, 8, 5, 0, one, 8) == -1 and lib.istnet_linear_ce_scratch_kib(4, 8, 5, 0, 3, 1) == -1

@@ -309,3 +309,221 @@ def test_distill_refusals():
     (dz,) = torch.autograd.grad(losses.TopLogitsDistill(z, top, idx), z, create_graph=True)
     with pytest.raises(RuntimeError):
         dz.sum().backward()
+
+
+# ---- cross entropy of a linear head ------------------------------------------------------------------------------------
+
+IGNORE = -100
+
+
+def _ce_inputs(n, d, v, dtype, seed, bias=True, ignored=0.25, index=torch.int64):
+    g = _gen(seed)
+    w = (torch.randn(v, d, device=DEV, generator=g) / math.sqrt(d)).to(dtype)
+    t = torch.randint(0, v, (n,), device=DEV, generator=g)
+    x = (torch.randn(n, d, device=DEV, generator=g) + 6.0 * torch.rand(n, 1, device=DEV, generator=g) * w[t].float()).to(dtype)
+    b = torch.randn(v, device=DEV, generator=g).to(dtype) if bias else None
+    t[torch.rand(n, device=DEV, generator=g) < ignored] = IGNORE
+    return x, w, b, t.to(index)
+
+
+def _ce_reference(x, w, b, t, reduction, gout):
+    """float64 loss and gradients, and entrywise bounds.
+
+    A logit: products of 16-bit numbers are exact in float32, their sum of d terms is off by at most 2 d U sum |x w| (2: whatever the
+    matrix instruction does inside).  float32 operands are hi + lo of float16, each off by 2^-22 of itself, the product lo lo of
+    2^-22 is left out: 12 U |x w| more, and entries below 2^-17 of the largest have an absolute error of 2^-39 of it.
+    p = 2^(z2 - lse2): both logs of size L are off by a few roundings, the sum of exponentials goes through 64 additions per lane and
+    tile and about tiles / 16 + 20 merges of some eight roundings.  p - [v = t] is rounded once more, to the operands' type (float32:
+    2^-22), with float16 scaled by 2^14: absolute 2^-39."""
+    t64 = t.long()
+    keep = t64 != IGNORE
+    kind, d, v = x.dtype, x.shape[1], w.shape[0]
+    X, W = x.detach().double().masked_fill(~keep.unsqueeze(1), 0.0), w.detach().double()
+    z = X @ W.t()
+    mass = X.abs() @ W.abs().t()
+    dz = (2 * d + 2) * U * mass
+    if kind == F32:
+        dz = dz + 12 * U * mass + 2.0 ** -39 * (float(X.abs().max()) * W.abs().sum(1) + float(W.abs().max()) * X.abs().sum(1, keepdim=True))
+    if b is not None:
+        z = z + b.detach().double()
+    lse = torch.logsumexp(z, 1)
+    pick = t64.clamp(0, v - 1).unsqueeze(1)
+    wrong = keep & ((t64 < 0) | (t64 >= v))
+    rows = torch.where(keep, lse - z.gather(1, pick).squeeze(1), 0.0).masked_fill(wrong, NAN)
+    fin = z.masked_fill(~z.isfinite(), 0.0)
+    size = fin.abs().amax(1) / math.log(2) + lse.abs().nan_to_num(0, 0, 0) / math.log(2)
+    rel = 2 * dz.nan_to_num(0, 0, 0).amax(1) + U * (6 * size + 64 + 8 * (v / 4096 + 20))
+    rows_bound = (rel + 2 * U * rows.abs().nan_to_num(0, 0, 0)) * keep
+    n = keep.sum().double()
+    if reduction == "none":
+        loss, loss_bound, factor = rows, rows_bound, gout.double()
+    else:
+        share = 1.0 / n if reduction == "mean" else torch.ones((), device=DEV, dtype=torch.float64)
+        loss, loss_bound = rows.sum() * share, rows_bound.sum() * share + 2 * U * (rows.abs().sum() * share).nan_to_num(0, 0, 0)
+        factor = (gout.double() * share).expand(x.shape[0])
+    p = torch.exp(z - lse.unsqueeze(1))
+    y = p.scatter_add(1, pick, -torch.ones_like(pick, dtype=torch.float64))
+    y = y.masked_fill(~keep.unsqueeze(1), 0.0).masked_fill(wrong.unsqueeze(1), NAN)
+    unit = 4 * U if kind == F32 else _round(kind)
+    dy = (rel.unsqueeze(1) * p + unit * y.abs() + (0.0 if kind == BF16 else 2.0 ** -39) + 2.0 ** -120) * keep.unsqueeze(1)
+    f = torch.where(keep, factor, 0.0).unsqueeze(1)
+    extra = 12 * U if kind == F32 else 0.0
+    gx, gw, gb = f * (y @ W), (f * y).t() @ X, (f * y).sum(0)
+    bx = f.abs() * (dy @ W.abs() + ((2 * v + 2) * U + extra) * (y.abs() @ W.abs()))
+    # weights of the rows are taken into the rows of x, which are rounded again
+    again = unit if reduction == "none" else 0.0
+    bw = (f.abs() * dy).t() @ X.abs() + ((2 * x.shape[0] + 2) * U + extra + again) * ((f * y).abs().t() @ X.abs())
+    bb = (f.abs() * dy).sum(0) + (x.shape[0] + 4) * U * (f * y).abs().sum(0)
+    if kind == F32:
+        bx = bx + f.abs() * 2.0 ** -39 * float(W.abs().max()) * y.abs().sum(1, keepdim=True)
+        bw = bw + 2.0 ** -39 * float(X.abs().max()) * (f * y).abs().sum(0).unsqueeze(1)
+    if kind == F16 and reduction == "none":      # weighted rows of x below the normal range of float16
+        bw = bw + 2.0 ** -25 * float(f.abs().max()) * (y.abs().sum(0)).unsqueeze(1)
+    end = lambda bound, ref: (bound + (_round(kind) + 8 * U) * ref.abs() + _tiny(kind)).nan_to_num(INF)
+    # For the error as a whole: the d roundings of a logit's partial sums, each at most U times a partial sum of at most sum |x w|, have
+    # random signs and the partial sums grow with the square root of their length, so that they add up to a few U sum |x w|.  What is
+    # left of p's relative error is an absolute error of p - [v = t], which near p = 1 is as small as its error: it is counted
+    # against p, not against p - [v = t].
+    few = (2 * (4 + (12 if kind == F32 else 0)) * U * mass.amax(1) + U * (6 * size + 64 + 8 * (v / 4096 + 20))).unsqueeze(1)
+    q = (f.abs() * few * p).nan_to_num(0, 0, 0)
+    whole = [float((q @ W.abs()).norm()), float((q.t() @ X.abs()).norm()), float(q.sum(0).norm())]
+    return loss, loss_bound + 2.0 ** -100, (gx, end(bx, gx), whole[0]), (gw, end(bw, gw), whole[1]), (gb, end(bb, gb), whole[2])
+
+
+def _check_ce(x, w, b, t, reduction, ignore=IGNORE, norms=True):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    b = None if b is None else b.detach().requires_grad_()
+    loss = losses.LinearCrossEntropy(x, w, t, b, ignore, reduction)
+    gout = 0.5 + torch.rand(loss.shape, device=DEV, generator=_gen(13))
+    wrt = (x, w) if b is None else (x, w, b)
+    grads = torch.autograd.grad(loss, wrt, gout)
+    assert loss.dtype == F32 and all(g.dtype == a.dtype and g.shape == a.shape for g, a in zip(grads, wrt))
+    want, bound, *pairs = _ce_reference(x, w, b, torch.where(t == ignore, IGNORE, t), reduction, gout)
+    _within(loss, want, bound, "loss")
+    # the bounds are for the worst case; roundings of many terms rarely agree in sign, so that the error as a whole stays within a few
+    # units of the roundings of p - t and of the result, beside that of p
+    unit = (4 * U if x.dtype == F32 else _round(x.dtype)) * 2
+    for name, got, (ref, gb, of_p) in zip(("dx", "dw", "db"), grads, pairs):
+        _within(got, ref, gb, name)
+        if norms and ref.isfinite().all() and float(ref.norm()) > 0:
+            off = float((got.double() - ref).norm())
+            assert off <= (4 * unit + 64 * U) * float(ref.norm()) + of_p + ref.numel() ** 0.5 * _tiny(x.dtype), (name, off, float(ref.norm()))
+    return loss, grads
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,d,v", [(1, 1, 1), (1, 7, 2), (3, 32, 257), (130, 33, 6), (129, 64, 300), (257, 100, 1025), (64, 387, 4001),
+                                   (1000, 128, 64), (2500, 40, 500), (5, 1024, 3000), (300, 512, 20000), (1, 96, 70001)])
+def test_linear_ce(n, d, v, dtype):
+    for i, reduction in enumerate(("mean", "none", "sum")):
+        x, w, b, t = _ce_inputs(n, d, v, dtype, n + d + v + i, bias=i != 1, ignored=(0.25, 0.0, 0.6)[i],
+                                index=(torch.int64, torch.int32)[i % 2])
+        if (t == IGNORE).all():
+            t[0] = v - 1
+        _check_ce(x, w, b, t, reduction)
+
+
+@pytest.mark.parametrize("dtype,n,v", [(BF16, 4100, 66000), (F32, 4100, 33000), (F32, 17000, 300)])
+def test_linear_ce_several_pieces_and_many_rows(dtype, n, v):
+    x, w, b, t = _ce_inputs(n, 24, v, dtype, 9)
+    _check_ce(x, w, b, t, "mean")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_ce_strides_and_partial_gradients(dtype):
+    x, w, b, t = _ce_inputs(60, 96, 333, dtype, 4)
+    wide = torch.cat((w, w[:, :32]), 1)
+    wide_x = torch.cat((x, x[:, :5]), 1)
+    first, grads = _check_ce(x, w, b, t, "mean")
+    for xx, ww in ((x, wide[:, :96]), (x, torch.cat((w[:, :1], wide), 1)[:, 1:97]), (wide_x[:, :96], w), (x, w.t().contiguous().t()),
+                   (x.t().contiguous().t(), w)):
+        loss, g = _check_ce(xx, ww, b, t, "mean")
+        assert torch.equal(loss, first) and all(torch.equal(p, q) for p, q in zip(g, grads))
+    three = losses.LinearCrossEntropy(x.reshape(3, 4, 5, 96), w, t.reshape(3, 4, 5), b, reduction="none")
+    assert three.shape == (3, 4, 5)
+    a = x.detach().requires_grad_()
+    only_x = torch.autograd.grad(losses.LinearCrossEntropy(a, w, t, b), a, torch.ones((), device=DEV))[0]
+    c = w.detach().requires_grad_()
+    only_w = torch.autograd.grad(losses.LinearCrossEntropy(x, c, t, b), c, torch.ones((), device=DEV))[0]
+    e = b.detach().requires_grad_()
+    only_b = torch.autograd.grad(losses.LinearCrossEntropy(x, w, t, e), e, torch.ones((), device=DEV))[0]
+    every = [a.detach().requires_grad_(), c.detach().requires_grad_(), e.detach().requires_grad_()]
+    full = torch.autograd.grad(losses.LinearCrossEntropy(every[0], every[1], t, every[2]), every, torch.ones((), device=DEV))
+    assert torch.equal(only_x, full[0]) and torch.equal(only_w, full[1]) and torch.equal(only_b, full[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_linear_ce_masks(dtype, reduction):
+    """Rows that do not count may hold anything; classes may be excluded by a bias of -inf; weights of zero."""
+    x, w, b, t = _ce_inputs(140, 48, 600, dtype, 21)
+    t[5], t[139], t[7] = IGNORE, IGNORE, 599
+    x[5], x[139] = NAN, INF
+    b[:256], b[300] = -INF, -INF                    # a whole tile of classes, and one
+    t = torch.where((t >= 0) & ((t < 256) | (t == 300)), 450, t)
+    loss, grads = _check_ce(x, w, b, t, reduction)
+    assert all(g.isfinite().all() for g in grads) and (grads[0][5] == 0).all()
+    x, w, b, t = _ce_inputs(20, 48, 600, dtype, 22, ignored=0.0)
+    loss, grads = _check_ce(x * 0, w, b, torch.full_like(t, 7), reduction, ignore=7)      # nothing counts
+    assert (loss == 0).all() if reduction != "mean" else loss.isnan()
+    assert all((g == 0).all() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_linear_ce_rows_that_cannot_be_right_are_nan(dtype):
+    x, w, b, t = _ce_inputs(6, 40, 300, dtype, 23, ignored=0.0)
+    t[1], t[2], t[3] = 300, -1, IGNORE
+    x = x.detach().requires_grad_()
+    loss = losses.LinearCrossEntropy(x, w, t, b, reduction="none")
+    (dx,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    assert loss.isnan().tolist() == [False, True, True, False, False, False]
+    assert dx.isnan().all(1).tolist() == [False, True, True, False, False, False] and dx[[0, 3, 4, 5]].isfinite().all()
+    x2 = x.detach().clone()
+    x2[0, 3] = NAN
+    assert losses.LinearCrossEntropy(x2, w, t.clamp(min=0, max=299), b, reduction="none").isnan()[0]
+    none = losses.LinearCrossEntropy(x[:0], w, t[:0], b)
+    assert none.isnan()
+
+
+def test_linear_ce_large_logits_offsets_and_outliers():
+    """Logits in the thousands, one class far ahead, one row of features a thousand times the others: float32 keeps what its own
+    products keep."""
+    x, w, b, t = _ce_inputs(70, 64, 500, F32, 31, ignored=0.0)
+    _check_ce(x * 300.0, w, b, t, "none", norms=False)
+    b = b.clone()
+    b[3] = 4000.0
+    _check_ce(x, w, b, t, "mean", norms=False)
+    x[11] *= 1000.0
+    w[17] *= 1e-3
+    _check_ce(x, w, None, t, "none", norms=False)
+
+
+def test_linear_ce_gradient_against_differences():
+    x, w, b, t = _ce_inputs(2, 5, 7, F32, 3, ignored=0.0)
+    x, w, b = (a.detach().requires_grad_() for a in (x, w, b))
+    grads = torch.autograd.grad(losses.LinearCrossEntropy(x, w, t, b, reduction="sum"), (x, w, b))
+    h = 2.0 ** -6
+    for a, g in zip((x, w, b), grads):
+        for i in range(a.numel()):
+            with torch.no_grad():
+                keep = a.reshape(-1)[i].clone()
+                a.view(-1)[i] = keep + h
+                hi = float(losses.LinearCrossEntropy(x, w, t, b, reduction="sum"))
+                a.view(-1)[i] = keep - h
+                lo = float(losses.LinearCrossEntropy(x, w, t, b, reduction="sum"))
+                a.view(-1)[i] = keep
+            # third derivative along one coordinate: at most the cube of the largest factor it meets
+            reach = max(1.0, float(x.detach().abs().max()), float(w.detach().abs().max())) ** 3
+            assert abs((hi - lo) / (2 * h) - float(g.reshape(-1)[i])) < 2 * reach * h * h / 6 + 256 * U * (1 + abs(hi)) / h
+
+
+def test_linear_ce_refusals():
+    x, w, b, t = _ce_inputs(4, 8, 9, F32, 1)
+    with pytest.raises(TypeError, match="features"):
+        losses.LinearCrossEntropy(x.double(), w.double(), t)
+    with pytest.raises(RuntimeError, match="same device"):
+        losses.LinearCrossEntropy(x, w.cpu(), t)
+    x.requires_grad_()
+    (dx,) = torch.autograd.grad(losses.LinearCrossEntropy(x, w, t, b), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
