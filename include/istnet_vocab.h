@@ -38,7 +38,7 @@ ISTNET_PN2_API int istnet_embed_backward(long long n, int v, int d, int dtype, i
  *   q = softmax over the used slots of top / T,  p = softmax over all classes of z / T,
  *   row = T^2 * sum_k q_k (log q_k - log p_idx(k)),  loss = per row (reduction 0), sum (2) or mean over the counted rows (1).
  * An index outside [-1, v) or a NaN among the used logits makes its row NaN.  Kept for the backward: stats (n, 2) = (row maximum,
- * 1 / sum of exp((z - maximum) / T), 0 where the row does not count), q (n, k) = the weight of a slot's class (the slots of a row
+ * sum of exp((z - maximum) / T) beside the largest itself, -1 where the row does not count), q (n, k) = the weight of a slot's class (the slots of a row
  * that name the same class all hold their sum) and count (1) = number of counted rows (written for reductions 1 and 2).
  * ttype: element type of top.  n <= 2^23. */
 ISTNET_PN2_API int istnet_distill_scratch_kib(long long n, int v, int k);

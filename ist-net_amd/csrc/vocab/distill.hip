@@ -12,6 +12,7 @@
 namespace {
 
 constexpr int kMaxSlots = 256;
+constexpr int kShortRow = 2048;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNaN = __builtin_nanf("");
 
@@ -95,6 +96,25 @@ __device__ __forceinline__ Stat scan_row(const T* __restrict__ z, int a, int e, 
   return {m, block_sum<THREADS>(st.s * exp2_raw((st.m - ref) * c), tmp)};
 }
 
+// sum of exponentials of a row beside ONE of its largest logits, m: what 1 + rest rounds away where the largest is almost certain
+template <typename T, int THREADS>
+__device__ __forceinline__ float rest_of_row(const T* __restrict__ z, int v, float m, float c, float* tmp) {
+  constexpr int V = kVec<T>;
+  float rest = 0.f, largest = 0.f;
+  for (int at = threadIdx.x * V; at < v; at += THREADS * V) {
+    float f[V];
+    load_part(z + at, v - at, f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (at + i < v) {
+        if (f[i] == m) largest += 1.f; else rest += exp2_raw((f[i] - m) * c);
+      }
+    }
+  }
+  rest = block_sum<THREADS>(rest, tmp);
+  return rest + (block_sum<THREADS>(largest, tmp) - 1.f);
+}
+
 // the row's loss from its statistics: teacher's softmax, the k picked logits, weights of the slots for the backward
 template <typename T, int THREADS>
 __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k, int ttype, int idx64, const void* __restrict__ top,
@@ -104,9 +124,12 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k
   const int tid = threadIdx.x;
   if (!counts) {
     for (int j = tid; j < k; j += THREADS) q[row * k + j] = 0.f;
-    if (tid == 0) { stats[2 * row] = 0.f; stats[2 * row + 1] = 0.f; row_loss[row] = 0.f; }
+    if (tid == 0) { stats[2 * row] = 0.f; stats[2 * row + 1] = -1.f; row_loss[row] = 0.f; }
     return;
   }
+  // rows short enough for one wave are looked at once more (they are in the caches); in longer ones the rest is no small number
+  const float rest = fabsf(st.m) == INFINITY ? kNaN : THREADS == 64 && v <= kShortRow ? rest_of_row<T, THREADS>(z, v, st.m, kLog2e / temp, tmp)
+                                                                                : st.s - 1.f;
   float tm = -INFINITY, bad = 0.f;
   for (int j = tid; j < k; j += THREADS) {
     const long long id = load_index(idx, row * k + j, idx64);
@@ -125,7 +148,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k
   float ts = 0.f;
   for (int j = tid; j < k; j += THREADS) ts += lidx[j] >= 0 ? expf(lq[j] - tm) : 0.f;
   ts = block_sum<THREADS>(ts, tmp);
-  const float log_ts = logf(ts), log_s = logf(st.s);
+  const float log_ts = logf(ts), log_s = log1pf(rest);
   float loss = 0.f;
   for (int j = tid; j < k; j += THREADS) {
     const float t = lq[j];
@@ -146,7 +169,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k
   }
   if (tid == 0) {
     stats[2 * row] = st.m;
-    stats[2 * row + 1] = bad > 0.f ? kNaN : 1.f / st.s;
+    stats[2 * row + 1] = bad > 0.f ? kNaN : rest;
     row_loss[row] = bad > 0.f ? kNaN : temp * temp * loss;
   }
 }
@@ -200,7 +223,7 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(long long n, int me
   double sum = 0.0, rows = 0.0;
   for (long long i = threadIdx.x; i < n; i += 1024) {
     sum += row_loss[i];
-    rows += stats[2 * i + 1] == 0.f ? 0.0 : 1.0;      // 1 / sum of exponentials: zero only where nothing was counted
+    rows += stats[2 * i + 1] == -1.f ? 0.0 : 1.0;
   }
   sum = wave_sum(sum);
   rows = wave_sum(rows);
@@ -223,9 +246,9 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
   constexpr int V = kVec<T>;
   const long long row = blockIdx.x / splits;
   const int a = (int)(blockIdx.x % splits) * width, e = min(v, a + width);
-  const float m = stats[2 * row], inv_s = stats[2 * row + 1], c = kLog2e / temp;
+  const float m = stats[2 * row], rest = stats[2 * row + 1], inv_s = 1.f / (1.f + rest), c = kLog2e / temp;
   T* out = dz + row * v;
-  if (inv_s == 0.f) {      // a row without a teacher: its logits are not looked at
+  if (rest == -1.f) {      // a row without a teacher: its logits are not looked at
     const float zero[V] = {};
     for (int at = a + threadIdx.x * V; at < e; at += THREADS * V) store_part(out + at, e - at, zero);
     return;
@@ -253,11 +276,15 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
     for (int i = 0; i < V; ++i) f[i] = gp * exp2_raw((f[i] - m) * c);
     store_part(out + at, e - at, f);
   }
-  // the teacher's classes: p - q is formed before it is rounded.  The barrier orders these stores behind the row's.
+  // the teacher's classes: p - q is formed before it is rounded, as (e - q - q rest) / (1 + rest), which keeps its precision where
+  // both are almost one.  The barrier orders these stores behind the row's.
   __syncthreads();
   for (int j = threadIdx.x; j < k; j += THREADS) {
     const long long id = load_index(idx, row * k + j, idx64);
-    if (id >= a && id < e) out[id] = from_f32<T>(g * (inv_s * exp2_raw((to_f32(in[id]) - m) * c) - q[row * k + j]));
+    if (id >= a && id < e) {
+      const float qj = q[row * k + j], ej = exp2_raw((to_f32(in[id]) - m) * c);
+      out[id] = from_f32<T>(gp * __builtin_fmaf(-qj, rest, ej - qj));
+    }
   }
 }
 

@@ -10,12 +10,16 @@
 // so the logits cost a second product (8 N V D operations instead of 6) and the memory is that of one piece.
 //
 // Rows whose target is ignore_index are left out before the products: the rows that count are packed (padded to whole tiles with
-// zeros), so masked rows cost nothing and whatever they hold is not looked at.  bfloat16 and float16 operands go to the matrix cores
-// as they are; a float32 operand is held as two float16 numbers to a common power of two, x = 2^-e (hi + lo), and a product is
-// hi hi + hi lo + lo hi: 22 bits of each factor, the dropped lo lo is 2^-22 of the product at most and 2^-24 mostly; entries smaller
-// than 2^-17 of the largest one keep an absolute error of 2^-39 of that.  Three half-precision products run at three times the rate
-// of one float32 product on this chip.  All sums are float32, p - t is rounded to 16 bits (float32: to hi + lo) after the target was
-// taken off, as the operands are.
+// zeros), so masked rows cost nothing and whatever they hold is not looked at.
+//
+// Numbers.  The logits of bfloat16 and float16 operands are exact products summed in float32.  A float32 operand is held as two
+// float16 numbers to a common power of two, x = 2^-e (hi + lo), and a product is hi hi + hi lo + lo hi: 22 bits of each factor, the
+// dropped lo lo is 2^-22 of the product at most; entries smaller than 2^-17 of the largest one keep an absolute error of 2^-39 of
+// that.  Three half-precision products run at three times the rate of one float32 product on this chip.
+// p - t is rounded once the target is taken off, always to float16 numbers scaled by 2^14, and always to more bits than the gradients
+// have, because an error of p - t of the result's own rounding would add as much again to it: one number (11 bits) for bfloat16
+// operands, which are turned into float16 ones with an exponent in common for this (exact down to 2^-29 of the largest entry), hi + lo
+// (22 bits) for float16 and float32 ones.  All sums are float32.
 #include <algorithm>
 
 #include "vocab_common.h"
@@ -47,15 +51,22 @@ struct Operand {
   int last_row, last_col8;
 };
 
+// What the backward needs of a row: p_v = inv * 2^(z_v - ref) in log2 units; the derivative at the target, p_t - 1, comes from the
+// sum over the OTHER classes, so that it (and the loss) keep their relative precision where the target is almost certain.
+struct __attribute__((aligned(16))) RowStat { float ref, inv, at_target, unused; };
+
 struct Epilogue {
   // logits
   const float* scal;             // device scalars, see Scal
-  const float* bias2;            // log2(e) * bias, -inf behind the last class; or null
+  const float* bias2;            // log2(e) * bias, -inf behind the last class
+  int biased;
   const int* target;             // packed rows: class or < 0
-  const float* lse2;             // log2-sum-exp per packed row
-  float2* part;                  // [class tile][packed row]
-  float* zt2;                    // target's logit * log2(e)
-  uint16_t* dz[2];               // [packed row][piece], hi (and lo)
+  const RowStat* stat;           // per packed row
+  float2* part;                  // [class tile][packed row]: largest of the other classes' logits in log2 units, sum of exponentials
+  float* zt;                     // the target's logit as the product left it (with a bias: finished, in log2 units)
+  uint16_t* dz[2];               // [packed row][piece], float16 hi (and lo)
+  const int* rowmap;             // with weights: packed row -> row
+  const float* weights;          // weights of the rows' losses where they are taken into p - t, or null
   long long ld_dz;
   int v, v0;                     // classes in all, first class of the piece
   int parts_ld;
@@ -66,12 +77,11 @@ struct Epilogue {
   void* out;                     // [row][d] final
   int out_rows, d, reduction;
   const float* gout;
-  float fixed_scale;
-  int scale_slot;                // Scal index of the operand scale that is divided out
 };
 
 // device scalars
-enum Scal { kCount = 0, kLogitScale = 1, kXScale = 2, kWScale = 3, kGMax = 4, kScalars = 8 };
+// (kXScale, kWScale: of the packed operands; kXBack, kWBack: of those that the gradients are formed from)
+enum Scal { kCount = 0, kLogitScale = 1, kXScale = 2, kWScale = 3, kGMax = 4, kXBack = 5, kWBack = 6, kScalars = 8 };
 
 __device__ __forceinline__ int swz_kc(int row) { return ((row >> 1) ^ (row >> 3)) & 3; }
 template <int R> __device__ __forceinline__ int swz_ks(int k) { return R >= 256 ? ((k & 3) | (((k >> 3) & 1) << 2)) : (k & 3); }
@@ -192,13 +202,14 @@ __device__ __forceinline__ void tile_of(int wg, int total, int tm, int tn, int* 
 
 enum { kLse = 0, kDz = 1, kSlab = 2, kOut = 3 };
 
-// C (M x N) = A (M x K) B (N x K)^T, tile MT x NT, four waves of MT / 2 x NT / 2.  M: matrix element type; P: planes (2 = float32 held
-// as two); T: element type of the final output.  The lane of column n holds rows 8 j + 4 (lane / 32) + 0..3 of every 32 x 32 block.
+// C (M x N) = A (M x K) B (N x K)^T, tile MT x NT, four waves of MT / 2 x NT / 2.  M: matrix element type; SEGS: products of planes
+// that make one up, walked one after the other along K, small ones first (1: hi hi; 2: hi lo, hi hi; 3: lo hi, hi lo, hi hi);
+// PD: planes of p - t that are written; T: element type of the final output.  The lane of column n holds rows 8 j + 4 (lane / 32) + 0..3 of every 32 x 32 block.
 // ROWS_N / ROWS_K: the packed rows are the N dimension (tiles behind the last row leave) / the K dimension (it ends there).
-template <typename M, int P, bool AKS, bool BKS, int MT, int NT, int EPI, typename T>
+template <typename M, int SEGS, int PD, bool AKS, bool BKS, int MT, int NT, int EPI, typename T>
 __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, int tm, int tn, int ksteps, int per_split, int rows_n,
                                                          int rows_k, Epilogue e) {
-  constexpr int WAVES = 4, MB = MT / 64, NB = NT / 64, SEG = P == 2 ? 3 : 1;
+  constexpr int WAVES = 4, MB = MT / 64, NB = NT / 64;
   constexpr int ABYTES = MT * 64, BBYTES = NT * 64, STAGE = ABYTES + BBYTES;
   __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
@@ -207,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   const int count = (rows_n || rows_k) ? (int)e.scal[kCount] : 0;
   if (rows_n && nt * NT >= count) return;
   if (rows_k) ksteps = (count + BK - 1) / BK;
-  const int all = ksteps * SEG;
+  const int all = ksteps * SEGS;
   const int t0 = per_split ? min(all, split * per_split) : 0, t1 = per_split ? min(all, t0 + per_split) : all;
   const int m0 = mt * MT, n0 = nt * NT;
 
@@ -230,10 +241,9 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   constexpr int LOADS = Stager<AKS, MT, WAVES>::LOADS + Stager<BKS, NT, WAVES>::LOADS;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds));
 
-  int seg = P == 2 ? t0 / max(ksteps, 1) : 0, k = t0 - seg * ksteps, slot = 0;      // of the next step to load
+  int seg = SEGS > 1 ? t0 / max(ksteps, 1) : 0, k = t0 - seg * ksteps, slot = 0;      // of the next step to load
   auto issue = [&]() {
-    // the products of the halves, small ones first: lo hi, hi lo, hi hi
-    const int pa = P == 2 ? (seg == 0) : 0, pb = P == 2 ? (seg == 1) : 0;
+    const int pa = SEGS == 3 ? (seg == 0) : 0, pb = SEGS == 3 ? (seg == 1) : SEGS == 2 ? (seg == 0) : 0;
     sa.issue(a, pa, m0, k * BK, lds0 + slot * STAGE, wave, lane);
     sb.issue(b, pb, n0, k * BK, lds0 + slot * STAGE + ABYTES, wave, lane);
     slot = slot == kStages - 1 ? 0 : slot + 1;
@@ -267,92 +277,91 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   barrier();      // the tiles' LDS is free
 
   const int half = lane >> 5, col = lane & 31;
+  // logits in log2 units: without a bias they stay as the product left them and are scaled inside the exponential
+  const float c = EPI <= kDz && !e.biased ? e.scal[kLogitScale] : 1.f;
+  const int mw = m0 + wm * (MT / 2);
+  auto finish_logits = [&](int j) {
+    if (e.biased) {
+      const float scale = e.scal[kLogitScale];
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 bb = *reinterpret_cast<const f32x4*>(e.bias2 + e.v0 + mw + i * 32 + g * 8 + half * 4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][g * 4 + r] = __builtin_fmaf(acc[i][j][g * 4 + r], scale, bb[r]);
+        }
+    } else if (e.v0 + m0 + MT > e.v) {
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (e.v0 + mw + i * 32 + (r >> 2) * 8 + half * 4 + (r & 3) >= e.v) acc[i][j][r] = -INFINITY;
+    }
+  };
   if constexpr (EPI == kLse) {
-    const float c = e.scal[kLogitScale];
-    const int mw = m0 + wm * (MT / 2);
-    const bool add = e.bias2 != nullptr && (m0 + MT > e.v || e.accumulate);      // accumulate: a bias is there
     float2* pair = reinterpret_cast<float2*>(lds);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int n = n0 + wn * (NT / 2) + j * 32 + col;
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        if (add) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4 bb = *reinterpret_cast<const f32x4*>(e.bias2 + mw + i * 32 + g * 8 + half * 4);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][g * 4 + r] = __builtin_fmaf(acc[i][j][g * 4 + r], c, bb[r]);
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] *= c;
-        }
-      }
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-      m = fmaxf(m, __shfl_xor(m, 32));
-      const float ref = m == -INFINITY ? 0.f : m;
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s += exp2_raw(acc[i][j][r] - ref);
-      s += __shfl_xor(s, 32);
-      if (half == 0) pair[wm * NT + wn * (NT / 2) + j * 32 + col] = make_float2(m, s);
+      finish_logits(j);
       const int t = e.target[n] - mw;
       if (__any(t >= 0 && t < MT / 2)) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (t == i * 32 + (r >> 2) * 8 + half * 4 + (r & 3)) e.zt2[n] = acc[i][j][r];
+            if (t == i * 32 + (r >> 2) * 8 + half * 4 + (r & 3)) {
+              e.zt[n] = acc[i][j][r];
+              acc[i][j][r] = -INFINITY;
+            }
       }
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+      m = fmaxf(m, __shfl_xor(m, 32)) * c;
+      const float ref = m == -INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += exp2_raw(__builtin_fmaf(acc[i][j][r], c, -ref));
+      s += __shfl_xor(s, 32);
+      if (half == 0) pair[wm * NT + wn * (NT / 2) + j * 32 + col] = make_float2(m, s);
     }
     __syncthreads();
     if (threadIdx.x < NT) {
       e.part[(long long)mt * e.parts_ld + n0 + threadIdx.x] = merge(pair[threadIdx.x], pair[NT + threadIdx.x]);
     }
   } else if constexpr (EPI == kDz) {
-    const float c = e.scal[kLogitScale];
-    const int mw = m0 + wm * (MT / 2);      // within the piece
-    const bool add = e.bias2 != nullptr && (e.v0 + m0 + MT > e.v || e.accumulate);
     // per wave NT / 2 rows of MT / 2 classes, written row by row: pitch MT / 2 + 8 elements keeps the rows' writes apart
     constexpr int PITCH = MT / 2 + 8, ROWS = NT / 2;
     static_assert(4 * ROWS * PITCH * 2 <= kStages * STAGE, "the epilogue's rows fit the tiles' LDS");
     uint16_t* mine = reinterpret_cast<uint16_t*>(lds) + wave * ROWS * PITCH;
 #pragma unroll
-    for (int pl = 0; pl < P; ++pl) {
+    for (int pl = 0; pl < PD; ++pl) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         const int n = n0 + wn * (NT / 2) + j * 32 + col;
         if (pl == 0) {
-          const float l = e.lse2[n];
-          const float one = P == 2 || !__is_same(M, bf16) ? kDzScale : 1.f;
+          finish_logits(j);
+          const RowStat st = e.stat[n];
+          float one = kDzScale;
+          if (e.weights) one *= n < count ? e.weights[e.rowmap[n]] / e.scal[kGMax] : 0.f;
+          const float w = one * st.inv;
 #pragma unroll
-          for (int i = 0; i < MB; ++i) {
-            if (add) {
+          for (int i = 0; i < MB; ++i)
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const f32x4 bb = *reinterpret_cast<const f32x4*>(e.bias2 + e.v0 + mw + i * 32 + g * 8 + half * 4);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  acc[i][j][g * 4 + r] = one * exp2_raw(__builtin_fmaf(acc[i][j][g * 4 + r], c, bb[r]) - l);
-              }
-            } else {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) acc[i][j][r] = one * exp2_raw(acc[i][j][r] * c - l);
-            }
-          }
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = w * exp2_raw(__builtin_fmaf(acc[i][j][r], c, -st.ref));
           const int t = e.target[n] - e.v0 - mw;
           if (__any(t >= 0 && t < MT / 2)) {
+            const float x = one * st.at_target;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) acc[i][j][r] -= t == i * 32 + (r >> 2) * 8 + half * 4 + (r & 3) ? one : 0.f;
+              for (int r = 0; r < 16; ++r) acc[i][j][r] = t == i * 32 + (r >> 2) * 8 + half * 4 + (r & 3) ? x : acc[i][j][r];
           }
         }
 #pragma unroll
@@ -363,13 +372,9 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float x = acc[i][j][g * 4 + r];
-              if constexpr (__is_same(M, bf16)) {
-                h[r] = bf16_bits(x);
-              } else {
-                const f16 y = (f16)x;
-                h[r] = __builtin_bit_cast(uint16_t, y);
-                if (P == 2 && pl == 0) acc[i][j][g * 4 + r] = x - (float)y;
-              }
+              const f16 y = (f16)x;
+              h[r] = __builtin_bit_cast(uint16_t, y);
+              if (PD == 2 && pl == 0) acc[i][j][g * 4 + r] = x - (float)y;
             }
             *reinterpret_cast<uint2*>(mine + (j * 32 + col) * PITCH + i * 32 + g * 8 + half * 4) =
                 make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   } else {
     const float rows = e.scal[kCount];
     const float g = e.reduction == 0 ? e.scal[kGMax] : e.reduction == 1 ? e.gout[0] / rows : e.gout[0];
-    const float f = rows == 0.f ? 0.f : g * e.fixed_scale / e.scal[e.scale_slot];
+    const float f = rows == 0.f ? 0.f : g / kDzScale / e.scal[kXBack];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int n = n0 + wn * (NT / 2) + j * 32 + col;
@@ -445,30 +450,50 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
 
 // ---- before and after the products -------------------------------------------------------------------------------------------
 
-// largest magnitude of float32 rows (NaN and infinities included as they come): one value per workgroup
+// largest magnitude of a row (infinities as they come, NaN passed over), this lane's part
+template <typename T> __device__ __forceinline__ float row_amax(const T* row, int d, float m) {
+  for (int c = (threadIdx.x & 63) * kVec<T>; c < d; c += 64 * kVec<T>) {
+    float f[kVec<T>];
+    load_part(row + c, d - c, f);
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) m = fmaxf(m, fabsf(f[i]));
+  }
+  return m;
+}
+__device__ __forceinline__ void store_amax(float m, float* tmp, float* part) {
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
+}
+// the largest magnitude of the rows of x that count ([0, xwgs)) and of w, one value per workgroup
 __global__ __launch_bounds__(256) void ce_amax_kernel(int n, int v, int d, const float* __restrict__ x, long long ldx,
                                                       const float* __restrict__ w, long long ldw, const void* __restrict__ target,
                                                       int idx64, long long ignore, int xwgs, float* __restrict__ part) {
   __shared__ float tmp[4];
-  const bool is_x = (int)blockIdx.x < xwgs;
-  const int wg = is_x ? blockIdx.x : blockIdx.x - xwgs, wgs = is_x ? xwgs : gridDim.x - xwgs, rows = is_x ? n : v;
-  const float* src = is_x ? x : w;
-  const long long ld = is_x ? ldx : ldw;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6;
   float m = 0.f;
-  for (int r = wg * 4 + wave; r < rows; r += wgs * 4) {
-    if (is_x && load_index(target, r, idx64) == ignore) continue;
-    for (int c = lane * 4; c < d; c += 256) {
-      float f[4];
-      load_part(src + r * ld + c, d - c, f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(f[i]));
-    }
+  if ((int)blockIdx.x < xwgs) {
+    for (int r = blockIdx.x * 4 + wave; r < n; r += xwgs * 4)
+      if (load_index(target, r, idx64) != ignore) m = row_amax(x + r * ldx, d, m);
+  } else {
+    for (int r = (blockIdx.x - xwgs) * 4 + wave; r < v; r += (gridDim.x - xwgs) * 4) m = row_amax(w + r * ldw, d, m);
   }
-  m = wave_max(m);
-  if (lane == 0) tmp[wave] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
+  store_amax(m, tmp, part);
+}
+// the same of packed rows
+__global__ __launch_bounds__(256) void ce_amax_packed_kernel(int kp, const bf16* __restrict__ xp, const float* __restrict__ scal, int v,
+                                                             int d, const bf16* __restrict__ w, long long ldw, int xwgs,
+                                                             float* __restrict__ part) {
+  __shared__ float tmp[4];
+  const int wave = threadIdx.x >> 6, count = (int)scal[kCount];
+  float m = 0.f;
+  if ((int)blockIdx.x < xwgs) {
+    for (int r = blockIdx.x * 4 + wave; r < count; r += xwgs * 4) m = row_amax(xp + (long long)r * kp, kp, m);
+  } else {
+    for (int r = (blockIdx.x - xwgs) * 4 + wave; r < v; r += (gridDim.x - xwgs) * 4) m = row_amax(w + r * ldw, d, m);
+  }
+  store_amax(m, tmp, part);
 }
 
 // counted rows per block of 256
@@ -543,6 +568,23 @@ __global__ __launch_bounds__(1024) void ce_plan_kernel(int n, int counted, const
     scal[kXScale] = sx;
     scal[kWScale] = sw;
     scal[kGMax] = 1.f;
+    scal[kXBack] = sx;
+    scal[kWBack] = sw;
+  }
+}
+
+// scales of bfloat16 operands as float16 ones
+__global__ __launch_bounds__(1024) void ce_scales_kernel(int xwgs, int wgs, const float* __restrict__ amax, float* __restrict__ scal) {
+  __shared__ float tmx[16], tmw[16];
+  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+  const float m = i < wgs ? amax[i] : 0.f, mx = wave_max(i < xwgs ? m : 0.f), mw = wave_max(i < xwgs ? 0.f : m);
+  if (lane == 0) { tmx[wave] = mx; tmw[wave] = mw; }
+  __syncthreads();
+  if (i == 0) {
+    float x = 0.f, w = 0.f;
+    for (int k = 0; k < 16; ++k) { x = fmaxf(x, tmx[k]); w = fmaxf(w, tmw[k]); }
+    scal[kXBack] = scale_for(x);
+    scal[kWBack] = scale_for(w);
   }
 }
 
@@ -647,11 +689,11 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(int n, int v, int d, int k
   }
 }
 
-// log2-sum-exp and loss of 16 packed rows per workgroup, from the tiles' partial sums
-__global__ __launch_bounds__(256) void ce_finish_kernel(int tiles, int parts_ld, const float2* __restrict__ part,
-                                                        const float* __restrict__ zt2, const int* __restrict__ tgt,
+// statistics and loss of 16 packed rows per workgroup, from the tiles' partial sums
+__global__ __launch_bounds__(256) void ce_finish_kernel(int tiles, int parts_ld, int biased, const float2* __restrict__ part,
+                                                        const float* __restrict__ zt, const int* __restrict__ tgt,
                                                         const int* __restrict__ rowmap, const float* __restrict__ scal,
-                                                        float* __restrict__ lse2, float* __restrict__ packed_loss,
+                                                        RowStat* __restrict__ stat, float* __restrict__ packed_loss,
                                                         float* __restrict__ row_loss) {
   __shared__ float2 tmp[16][17];
   const int count = (int)scal[kCount], t = threadIdx.x & 15, j = threadIdx.x >> 4, row = blockIdx.x * 16 + t;
@@ -666,13 +708,30 @@ __global__ __launch_bounds__(256) void ce_finish_kernel(int tiles, int parts_ld,
   if (j == 0) {
     if (row < count) {
       for (int k = 1; k < 16; ++k) ms = merge(ms, tmp[k][t]);
-      const bool good = tgt[row] >= 0;
-      const float l = good ? ms.x + __log2f(ms.y) : kNaN, loss = good ? kLn2 * (l - zt2[row]) : kNaN;
-      lse2[row] = l;
+      // ms: the other classes.  d = target's logit above their largest; loss = log(1 + rest), rest = others over target
+      RowStat r = {kNaN, kNaN, kNaN, 0.f};
+      float loss = kNaN;
+      if (tgt[row] >= 0) {
+        const float c = biased ? 1.f : scal[kLogitScale], z = zt[row];
+        const float d = ms.x == -INFINITY ? INFINITY : __builtin_fmaf(z, c, -ms.x);
+        r.ref = d > 0.f ? z * c : ms.x;
+        const float others = ms.x == -INFINITY ? ms.y : ms.y * exp2_raw(ms.x - r.ref), mine = exp2_raw(__builtin_fmaf(z, c, -r.ref));
+        r.inv = 1.f / (others + mine);
+        if (d < -100.f) {
+          loss = kLn2 * -d + logf(ms.y);
+          r.at_target = -1.f + 0.f * loss;      // NaN stays NaN
+          if (d == -INFINITY) r.at_target = -1.f;
+        } else {
+          const float rest = others / mine;
+          loss = log1pf(rest);
+          r.at_target = -rest / (1.f + rest);
+        }
+      }
+      stat[row] = r;
       packed_loss[row] = loss;
       if (row_loss) row_loss[rowmap[row]] = loss;
     } else {
-      lse2[row] = INFINITY;      // a row of padding: every probability zero
+      stat[row] = {INFINITY, 1.f, 0.f, 0.f};      // a row of padding: every probability zero
     }
   }
 }
@@ -709,21 +768,49 @@ __global__ __launch_bounds__(1024) void ce_gmax_kernel(const float* __restrict__
   }
 }
 
-// packed rows of g_i / max |g| * x_i: what dw is formed from where the rows' losses have weights of their own
+// eight elements as float16 (P == 2: hi and lo) whatever their type
 template <typename T, int P>
-__global__ __launch_bounds__(256) void ce_weigh_kernel(int d, int kp, const T* __restrict__ x, long long ldx,
-                                                       const float* __restrict__ gout, const int* __restrict__ rowmap,
-                                                       const float* __restrict__ scal, uint16_t* __restrict__ xp, long long xplane) {
+__device__ __forceinline__ void pack8_f16(const T* src, int left, float scale, u32x4* hi, u32x4* lo) {
+  if constexpr (__is_same(T, bf16)) {
+    float f[8];
+    load_part(src, left, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= scale;
+    *hi = pack<f16>(f);
+  } else {
+    pack8<T, P>(src, left, scale, hi, lo);
+  }
+}
+
+// Packed float16 rows that dw is formed from: of g_i / max |g| * x_i where the rows' losses have weights of their own, of x_i else.
+template <typename T, int P>
+__global__ __launch_bounds__(256) void ce_back_x_kernel(int d, int kp, const T* __restrict__ x, long long ldx,
+                                                        const float* __restrict__ gout, const int* __restrict__ rowmap,
+                                                        const float* __restrict__ scal, uint16_t* __restrict__ xp, long long xplane) {
   const int count = (int)scal[kCount], end = (count + kPad - 1) / kPad * kPad, lane = threadIdx.x & 63;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= end) return;
   const int i = r < count ? rowmap[r] : -1;
-  const float s = i >= 0 ? gout[i] / scal[kGMax] * scal[kXScale] : 0.f;
+  const float s = i < 0 ? 0.f : gout ? gout[i] / scal[kGMax] * scal[kXBack] : scal[kXBack];
   for (int c = lane * 8; c < kp; c += 512) {
     u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-    if (i >= 0) pack8<T, P>(x + (long long)i * ldx + c, d - c, s, &hi, &lo);
+    if (i >= 0) pack8_f16<T, P>(x + (long long)i * ldx + c, d - c, s, &hi, &lo);
     store16(xp + (long long)r * kp + c, hi);
     if constexpr (P == 2) store16(xp + xplane + (long long)r * kp + c, lo);
+  }
+}
+
+// rows of a piece of bfloat16 w as float16
+__global__ __launch_bounds__(256) void ce_back_w_kernel(int rows, int d, int kp, const bf16* __restrict__ w, long long ldw,
+                                                        const float* __restrict__ scal, uint16_t* __restrict__ wp) {
+  const int lane = threadIdx.x & 63;
+  const float s = scal[kWBack];
+  for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4) {
+    for (int c = lane * 8; c < kp; c += 512) {
+      u32x4 hi, lo;
+      pack8_f16<bf16, 1>(w + r * ldw + c, d - c, s, &hi, &lo);
+      store16(wp + (long long)r * kp + c, hi);
+    }
   }
 }
 
@@ -731,8 +818,7 @@ __global__ __launch_bounds__(256) void ce_weigh_kernel(int d, int kp, const T* _
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, const float* __restrict__ slab, long long slab_stride,
                                                     long long ld, const int* __restrict__ inverse, const float* __restrict__ gout,
-                                                    int reduction, float fixed_scale, const float* __restrict__ scal,
-                                                    T* __restrict__ dx) {
+                                                    int reduction, int folded, const float* __restrict__ scal, T* __restrict__ dx) {
   const int per = (d + 3) / 4;
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, i = id / per;
   if (i >= n) return;
@@ -746,7 +832,8 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, co
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] += y[r];
     }
-    const float g = (reduction == 0 ? gout[i] : reduction == 1 ? gout[0] / scal[kCount] : gout[0]) * fixed_scale / scal[kWScale];
+    const float g = (folded ? scal[kGMax] : reduction == 0 ? gout[i] : reduction == 1 ? gout[0] / scal[kCount] : gout[0]) / kDzScale /
+                    scal[kWBack];
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] *= g;
   }
@@ -758,7 +845,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, co
 // dw where its product was split along the rows
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dw_kernel(int rows, int d, int splits, const float* __restrict__ slab, long long slab_stride,
-                                                    long long ld, const float* __restrict__ gout, int reduction, float fixed_scale,
+                                                    long long ld, const float* __restrict__ gout, int reduction,
                                                     const float* __restrict__ scal, T* __restrict__ dw) {
   const int per = (d + 3) / 4;
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, i = id / per;
@@ -772,30 +859,29 @@ __global__ __launch_bounds__(256) void ce_dw_kernel(int rows, int d, int splits,
     for (int r = 0; r < 4; ++r) x[r] += y[r];
   }
   const float n = scal[kCount];
-  const float g = n == 0.f ? 0.f : (reduction == 0 ? scal[kGMax] : reduction == 1 ? gout[0] / n : gout[0]) * fixed_scale / scal[kXScale];
+  const float g = n == 0.f ? 0.f : (reduction == 0 ? scal[kGMax] : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale / scal[kXBack];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (c + r < d) dw[i * d + c + r] = from_f32<T>(g * x[r]);
 }
 
 // db: column sums of p - t over the packed rows, `chunks` parts of the rows side by side, joined in order
-template <typename M, int P>
+template <int PD>
 __global__ __launch_bounds__(256) void ce_colsum_kernel(int width, const uint16_t* __restrict__ hi, const uint16_t* __restrict__ lo,
                                                         long long ld, const float* __restrict__ gout, const int* __restrict__ rowmap,
-                                                        int reduction, const float* __restrict__ scal, int chunks,
-                                                        float* __restrict__ part) {
+                                                        const float* __restrict__ scal, int chunks, float* __restrict__ part) {
   const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, chunk = blockIdx.y * 4 + (threadIdx.x >> 6);
   const int count = (int)scal[kCount], per = (count + chunks - 1) / chunks, a = chunk * per, b = min(count, a + per);
   if (c >= width) return;
   float s[8] = {};
 #pragma unroll 4
   for (int r = a; r < b; ++r) {
-    const float g = reduction == 0 ? gout[rowmap[r]] : 1.f;
+    const float g = gout ? gout[rowmap[r]] : 1.f;
     float f[8];
-    unpack<M>(*reinterpret_cast<const u32x4*>(hi + r * ld + c), f);
-    if constexpr (P == 2) {
+    unpack<f16>(*reinterpret_cast<const u32x4*>(hi + r * ld + c), f);
+    if constexpr (PD == 2) {
       float l[8];
-      unpack<M>(*reinterpret_cast<const u32x4*>(lo + r * ld + c), l);
+      unpack<f16>(*reinterpret_cast<const u32x4*>(lo + r * ld + c), l);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] += l[i];
     }
@@ -807,7 +893,7 @@ __global__ __launch_bounds__(256) void ce_colsum_kernel(int width, const uint16_
 }
 template <typename T>
 __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chunks, const float* __restrict__ part,
-                                                    const float* __restrict__ gout, int reduction, float fixed_scale,
+                                                    const float* __restrict__ gout, int reduction, int folded,
                                                     const float* __restrict__ scal, T* __restrict__ db) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= rows) return;
@@ -815,7 +901,7 @@ __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chu
 #pragma unroll 4
   for (int k = 0; k < chunks; ++k) s += part[(long long)k * width + c];
   const float n = scal[kCount];
-  const float g = n == 0.f ? 0.f : (reduction == 0 ? 1.f : reduction == 1 ? gout[0] / n : gout[0]) * fixed_scale;
+  const float g = n == 0.f ? 0.f : (folded ? scal[kGMax] : reduction == 0 ? 1.f : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale;
   db[c] = from_f32<T>((float)(g * s));
 }
 
@@ -837,7 +923,7 @@ inline bool direct_w(int d, int dtype, const void* w, long long ldw) {
 
 struct Keep {      // what the backward needs, in the caller's `keep`
   long long np, kp, vp, planes;
-  long long xp, wp, bias2, rowmap, inverse, tgt, lse2, scal, bytes;
+  long long xp, wp, bias2, rowmap, inverse, tgt, stat, scal, bytes;
 };
 inline Keep keep_plan(long long n, int d, int v, int dtype, bool direct) {
   Keep k = {};
@@ -853,19 +939,19 @@ inline Keep keep_plan(long long n, int d, int v, int dtype, bool direct) {
   k.rowmap = take(4 * k.np);
   k.inverse = take(4 * k.np);
   k.tgt = take(4 * k.np);
-  k.lse2 = take(4 * k.np);
+  k.stat = take((long long)sizeof(RowStat) * k.np);
   k.scal = take(4 * kScalars);
   k.bytes = at;
   return k;
 }
-struct Forward { long long part, zt2, loss, blocks, amax, bytes; int tiles; };
+struct Forward { long long part, zt, loss, blocks, amax, bytes; int tiles; };
 inline Forward forward_plan(const Keep& k) {
   Forward f = {};
   f.tiles = (int)(k.vp / kMT);
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
   f.part = take(8ll * f.tiles * k.np);
-  f.zt2 = take(4 * k.np);
+  f.zt = take(4 * k.np);
   f.loss = take(4 * k.np);
   f.blocks = take(4 * (k.np / 256 + 1));
   f.amax = take(4 * 1024);
@@ -874,16 +960,17 @@ inline Forward forward_plan(const Keep& k) {
 }
 struct Backward {
   int pieces, dx_splits, dx_per, dw_splits, dw_per;
-  long long piece, dz, xg, dx_slab, dx_rows, dw_slab, dw_rows, col, ld, bytes;
+  long long piece, dz, xb, wb, amax, dx_slab, dx_rows, dw_slab, dw_rows, col, ld, bytes;
 };
-inline Backward backward_plan(const Keep& k, long long n, int d, int v, int reduction) {
+inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtype, int reduction) {
   Backward b = {};
-  const long long most = std::max<long long>(kMT, kPieceBytes / (2 * k.planes * k.np) / kMT * kMT);
+  const long long planes = dtype == ISTNET_VOCAB_BF16 ? 1 : 2;      // of p - t
+  const long long most = std::max<long long>(kMT, kPieceBytes / (2 * planes * k.np) / kMT * kMT);
   b.pieces = (int)((k.vp + most - 1) / most);
   b.piece = round_up((k.vp + b.pieces - 1) / b.pieces, kMT);
   b.pieces = (int)((k.vp + b.piece - 1) / b.piece);
   b.ld = round_up(d, kMT);
-  const long long dt = b.ld / kMT, seg = k.planes == 2 ? 3 : 1;
+  const long long dt = b.ld / kMT, seg = dtype == ISTNET_VOCAB_F32 ? 3 : planes;
   // two workgroups fit a compute unit: split K while that fills more of the 512 places, eight steps at least
   auto splits = [&](long long tiles, long long steps) {
     return std::max<long long>(1, std::min<long long>(512 / std::max<long long>(1, tiles), steps / 8));
@@ -897,8 +984,10 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int redu
   b.dw_per = (int)((dw_steps + b.dw_splits - 1) / b.dw_splits);
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
-  b.dz = take(2 * k.planes * k.np * b.piece);
-  b.xg = reduction == 0 ? take(2 * k.planes * k.np * k.kp) : 0;
+  b.dz = take(2 * planes * k.np * b.piece);
+  b.xb = dtype == ISTNET_VOCAB_BF16 || (dtype == ISTNET_VOCAB_F32 && reduction == 0) ? take(2 * k.planes * k.np * k.kp) : 0;
+  b.wb = dtype == ISTNET_VOCAB_BF16 ? take(2 * most_rows * k.kp) : 0;
+  b.amax = take(4 * 1024);
   b.dx_slab = take(4 * b.dx_splits * b.dx_rows * b.ld);
   b.dw_slab = b.dw_splits > 1 ? take(4 * b.dw_splits * b.dw_rows * b.ld) : 0;
   b.col = take(4ll * kChunks * b.piece);
@@ -906,9 +995,11 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int redu
   return b;
 }
 
-// element type of the matrix products, planes
-template <typename T> struct Matrix { typedef T M; static constexpr int P = 1; };
-template <> struct Matrix<float> { typedef f16 M; static constexpr int P = 2; };
+// element type of the logits' product, planes of the operands and of p - t, products of planes per product of the logits / gradients
+template <typename T> struct Matrix;
+template <> struct Matrix<float> { typedef f16 M; static constexpr int P = 2, PD = 2, LOGIT = 3, GRAD = 3; };
+template <> struct Matrix<f16> { typedef f16 M; static constexpr int P = 1, PD = 2, LOGIT = 1, GRAD = 2; };
+template <> struct Matrix<bf16> { typedef bf16 M; static constexpr int P = 1, PD = 1, LOGIT = 1, GRAD = 1; };
 
 }  // namespace
 
@@ -919,7 +1010,7 @@ extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, c
 extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward) {
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
   const Keep k = keep_plan(n, d, v, dtype, false);
-  return (int)(((backward ? backward_plan(k, n, d, v, reduction).bytes : forward_plan(k).bytes) + 1023) / 1024);
+  return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k).bytes) + 1023) / 1024);
 }
 
 extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w,
@@ -936,7 +1027,8 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   int* blocks = (int*)(wb + f.blocks);
   float *amax = (float*)(wb + f.amax), *packed_loss = (float*)(wb + f.loss), *row_loss = reduction == 0 ? loss : nullptr;
   uint16_t *xp = (uint16_t*)(kb + k.xp), *wp = (uint16_t*)(kb + k.wp);
-  float *bias2 = (float*)(kb + k.bias2), *lse2 = (float*)(kb + k.lse2), *zt2 = (float*)(wb + f.zt2);
+  float *bias2 = (float*)(kb + k.bias2), *zt = (float*)(wb + f.zt);
+  RowStat* stat = (RowStat*)(kb + k.stat);
   int *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse), *tgt = (int*)(kb + k.tgt);
   const int ax = split ? (int)std::min<long long>(256, (n + 3) / 4) : 0, aw = split ? (int)std::min<long long>(768, (v + 3ll) / 4) : 0;
   if (split)
@@ -960,18 +1052,18 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
     Epilogue e = {};
     e.scal = scal;
     e.bias2 = bias2;
-    e.accumulate = bias != nullptr;
+    e.biased = bias != nullptr;
     e.target = tgt;
     e.part = (float2*)(wb + f.part);
-    e.zt2 = zt2;
+    e.zt = zt;
     e.v = v;
     e.parts_ld = (int)k.np;
     const int tn = (int)((n + kNT - 1) / kNT);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<typename X::M, X::P, false, false, kMT, kNT, kLse, T>), dim3(f.tiles * tn),
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<typename X::M, X::LOGIT, 1, false, false, kMT, kNT, kLse, T>), dim3(f.tiles * tn),
                        dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), 0, 1, 0, e);
   });
   hipLaunchKernelGGL(ce_finish_kernel, dim3((unsigned)(round_up(n, kPad) / 16)), dim3(256), 0, st, f.tiles, (int)k.np,
-                     (const float2*)(wb + f.part), zt2, tgt, rowmap, scal, lse2, packed_loss, row_loss);
+                     bias != nullptr, (const float2*)(wb + f.part), zt, tgt, rowmap, scal, stat, packed_loss, row_loss);
   if (reduction != 0)
     hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, reduction == 1, packed_loss, scal, loss);
   return launch_status();
@@ -985,23 +1077,30 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   const hipStream_t st = (hipStream_t)stream;
   const bool direct = direct_w(d, dtype, w, ldw);
   const Keep k = keep_plan(n, d, v, dtype, direct);
-  const Backward b = backward_plan(k, n, d, v, reduction);
+  const Backward b = backward_plan(k, n, d, v, dtype, reduction);
   char *kb = (char*)keep, *wb = (char*)ws;
   float* scal = (float*)(kb + k.scal);
   uint16_t *xp = (uint16_t*)(kb + k.xp), *wp = (uint16_t*)(kb + k.wp), *dz = (uint16_t*)(wb + b.dz);
   int *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse);
-  const float fixed = dtype == ISTNET_VOCAB_BF16 ? 1.f : 1.f / kDzScale;
   const int tn = (int)((n + kNT - 1) / kNT), dt = (int)(b.ld / kMT);
+  const bool weighted = reduction == 0, folded = weighted && dtype == ISTNET_VOCAB_F16, turned = dtype == ISTNET_VOCAB_BF16;
+  if (weighted) hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, st, gout, rowmap, scal);
+  if (turned) {
+    const int ax = (int)std::min<long long>(256, (n + 3) / 4), aw = (int)std::min<long long>(768, (v + 3ll) / 4);
+    float* amax = (float*)(wb + b.amax);
+    hipLaunchKernelGGL(ce_amax_packed_kernel, dim3(ax + aw), dim3(256), 0, st, (int)k.kp, (const bf16*)xp, scal, v, d,
+                       (const bf16*)w, ldw, ax, amax);
+    hipLaunchKernelGGL(ce_scales_kernel, dim3(1), dim3(1024), 0, st, ax, ax + aw, amax, scal);
+  }
   VOCAB_DISPATCH(dtype, T, {
     typedef Matrix<T> X;
     typedef typename X::M M;
-    constexpr int P = X::P;
-    uint16_t* xg = xp;
-    if (reduction == 0 && dw) {
-      xg = (uint16_t*)(wb + b.xg);
-      hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, st, gout, rowmap, scal);
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_weigh_kernel<T, P>), dim3((unsigned)(round_up(n, kPad) / 4)), dim3(256), 0, st, d, (int)k.kp,
-                         (const T*)x, ldx, gout, rowmap, scal, xg, k.np * k.kp);
+    constexpr int P = X::P, PD = X::PD;
+    uint16_t* xb = xp;      // rows that dw is formed from
+    if (dw && (turned || (weighted && !folded))) {
+      xb = (uint16_t*)(wb + b.xb);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_back_x_kernel<T, P>), dim3((unsigned)(round_up(n, kPad) / 4)), dim3(256), 0, st, d, (int)k.kp,
+                         (const T*)x, ldx, weighted ? gout : nullptr, rowmap, scal, xb, k.np * k.kp);
     }
     const uint16_t* wd = direct ? (const uint16_t*)w : wp;
     const long long ldwd = direct ? ldw : k.kp, wplane = direct ? 0 : v * k.kp, xplane = (P - 1) * k.np * k.kp, dzp = k.np * b.piece;
@@ -1010,20 +1109,22 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
       Epilogue e = {};
       e.scal = scal;
       e.bias2 = (float*)(kb + k.bias2);
-      e.accumulate = has_bias;
+      e.biased = has_bias;
       e.target = (int*)(kb + k.tgt);
-      e.lse2 = (float*)(kb + k.lse2);
+      e.stat = (const RowStat*)(kb + k.stat);
       e.dz[0] = dz;
       e.dz[1] = dz + dzp;
       e.ld_dz = b.piece;
+      e.rowmap = rowmap;
+      e.weights = folded ? gout : nullptr;
       e.v = v;
       e.v0 = v0;
       const uint16_t* w0 = wd + v0 * ldwd;
       const Operand A = {{w0, w0 + (P - 1) * wplane}, ldwd, rows - 1, 0};
       const Operand B = {{xp, xp + xplane}, k.kp, (int)k.np - 1, 0};
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<M, P, false, false, kMT, kNT, kDz, T>), dim3(width / kMT * tn), dim3(256), 0, st,
-                         A, B, width / kMT, tn, (int)(k.kp / BK), 0, 1, 0, e);
-      const Operand D = {{dz, dz + (P - 1) * dzp}, b.piece, (int)k.np - 1, (int)b.piece / 8 - 1};
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<M, X::LOGIT, PD, false, false, kMT, kNT, kDz, T>), dim3(width / kMT * tn),
+                         dim3(256), 0, st, A, B, width / kMT, tn, (int)(k.kp / BK), 0, 1, 0, e);
+      const Operand D = {{dz, dz + (PD - 1) * dzp}, b.piece, (int)k.np - 1, (int)b.piece / 8 - 1};
       if (dx) {
         Epilogue s = {};
         s.scal = scal;
@@ -1031,10 +1132,15 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
         s.slab_stride = b.dx_rows * b.ld;
         s.ld_slab = b.ld;
         s.accumulate = piece > 0;
-        const Operand Wt = {{w0, w0 + (P - 1) * wplane}, ldwd, rows - 1, (int)(direct ? d : k.kp) / 8 - 1};
-        const int steps = (rows + BK - 1) / BK;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<M, P, true, false, kMT, kNT, kSlab, T>), dim3(dt * tn * b.dx_splits), dim3(256),
-                           0, st, Wt, D, dt, tn, steps, b.dx_per, 1, 0, s);
+        Operand Wt = {{w0, w0 + (P - 1) * wplane}, ldwd, rows - 1, (int)(direct ? d : k.kp) / 8 - 1};
+        if (turned) {
+          uint16_t* wf = (uint16_t*)(wb + b.wb);
+          hipLaunchKernelGGL(ce_back_w_kernel, dim3(std::min((rows + 3) / 4, 2048)), dim3(256), 0, st, rows, d, (int)k.kp,
+                             (const bf16*)w + v0 * ldw, ldw, scal, wf);
+          Wt = {{wf, wf}, k.kp, rows - 1, (int)k.kp / 8 - 1};
+        }
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, false, kMT, kNT, kSlab, T>), dim3(dt * tn * b.dx_splits),
+                           dim3(256), 0, st, Wt, D, dt, tn, (rows + BK - 1) / BK, b.dx_per, 1, 0, s);
       }
       if (dw) {
         Epilogue s = {};
@@ -1048,31 +1154,30 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
         s.d = d;
         s.reduction = reduction;
         s.gout = gout;
-        s.fixed_scale = fixed;
-        s.scale_slot = kXScale;
-        const Operand Xt = {{xg, xg + xplane}, k.kp, (int)k.np - 1, (int)k.kp / 8 - 1};
+        const Operand Xt = {{xb, xb + xplane}, k.kp, (int)k.np - 1, (int)k.kp / 8 - 1};
         const int vt = (rows + kNT - 1) / kNT;
         if (b.dw_splits == 1) {
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<M, P, true, true, kMT, kNT, kOut, T>), dim3(dt * vt), dim3(256), 0, st, Xt, D,
-                             dt, vt, 0, 0, 0, 1, s);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kOut, T>), dim3(dt * vt), dim3(256), 0,
+                             st, Xt, D, dt, vt, 0, 0, 0, 1, s);
         } else {
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<M, P, true, true, kMT, kNT, kSlab, T>), dim3(dt * vt * b.dw_splits), dim3(256),
-                             0, st, Xt, D, dt, vt, 0, b.dw_per, 0, 1, s);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kSlab, T>), dim3(dt * vt * b.dw_splits),
+                             dim3(256), 0, st, Xt, D, dt, vt, 0, b.dw_per, 0, 1, s);
           hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dw_kernel<T>), dim3((unsigned)(((long long)rows * ((d + 3) / 4) + 255) / 256)), dim3(256),
-                             0, st, rows, d, b.dw_splits, s.slab, s.slab_stride, b.ld, gout, reduction, fixed, scal, dw0);
+                             0, st, rows, d, b.dw_splits, s.slab, s.slab_stride, b.ld, gout, reduction, scal, dw0);
         }
       }
       if (db) {
         float* col = (float*)(wb + b.col);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_colsum_kernel<M, P>), dim3((width + 511) / 512, kChunks / 4), dim3(256), 0, st, width, dz,
-                           dz + (P - 1) * dzp, b.piece, gout, rowmap, reduction, scal, kChunks, col);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_colsum_kernel<PD>), dim3((width + 511) / 512, kChunks / 4), dim3(256), 0, st, width, dz,
+                           dz + (PD - 1) * dzp, b.piece, weighted && !folded ? gout : nullptr, rowmap, scal, kChunks, col);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_db_kernel<T>), dim3((rows + 255) / 256), dim3(256), 0, st, rows, width, kChunks, col, gout,
-                           reduction, fixed, scal, (T*)db + v0);
+                           reduction, folded, scal, (T*)db + v0);
       }
     }
     if (dx)
       hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dx_kernel<T>), dim3((unsigned)((n * ((d + 3) / 4) + 255) / 256)), dim3(256), 0, st, (int)n, d,
-                         b.dx_splits, (const float*)(wb + b.dx_slab), b.dx_rows * b.ld, b.ld, inverse, gout, reduction, fixed, scal, (T*)dx);
+                         b.dx_splits, (const float*)(wb + b.dx_slab), b.dx_rows * b.ld, b.ld, inverse, gout, reduction, folded, scal,
+                         (T*)dx);
   });
   return launch_status();
 }

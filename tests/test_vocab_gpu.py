@@ -333,8 +333,8 @@ def _ce_reference(x, w, b, t, reduction, gout):
     matrix instruction does inside).  float32 operands are hi + lo of float16, each off by 2^-22 of itself, the product lo lo of
     2^-22 is left out: 12 U |x w| more, and entries below 2^-17 of the largest have an absolute error of 2^-39 of it.
     p = 2^(z2 - lse2): both logs of size L are off by a few roundings, the sum of exponentials goes through 64 additions per lane and
-    tile and about tiles / 16 + 20 merges of some eight roundings.  p - [v = t] is rounded once more, to the operands' type (float32:
-    2^-22), with float16 scaled by 2^14: absolute 2^-39."""
+    tile and about tiles / 16 + 20 merges of some eight roundings.  p - [v = t] is rounded once more, to one float16 number for bfloat16
+    operands, to two (2^-22) for others, scaled by 2^14: absolute 2^-39."""
     t64 = t.long()
     keep = t64 != IGNORE
     kind, d, v = x.dtype, x.shape[1], w.shape[0]
@@ -364,21 +364,21 @@ def _ce_reference(x, w, b, t, reduction, gout):
     p = torch.exp(z - lse.unsqueeze(1))
     y = p.scatter_add(1, pick, -torch.ones_like(pick, dtype=torch.float64))
     y = y.masked_fill(~keep.unsqueeze(1), 0.0).masked_fill(wrong.unsqueeze(1), NAN)
-    unit = 4 * U if kind == F32 else _round(kind)
-    dy = (rel.unsqueeze(1) * p + unit * y.abs() + (0.0 if kind == BF16 else 2.0 ** -39) + 2.0 ** -120) * keep.unsqueeze(1)
+    unit = _round(F16) if kind == BF16 else 4 * U
     f = torch.where(keep, factor, 0.0).unsqueeze(1)
+    # (float16 operands: the weights of the rows are taken into p - t, whose absolute error is then one of the largest weight's)
+    folded = float(f.abs().max()) / f.abs().clamp(min=1e-30) if kind == F16 and reduction == "none" else 1.0
+    dy = (rel.unsqueeze(1) * p + unit * y.abs() + folded * 2.0 ** -39) * keep.unsqueeze(1)
     extra = 12 * U if kind == F32 else 0.0
     gx, gw, gb = f * (y @ W), (f * y).t() @ X, (f * y).sum(0)
     bx = f.abs() * (dy @ W.abs() + ((2 * v + 2) * U + extra) * (y.abs() @ W.abs()))
     # weights of the rows are taken into the rows of x, which are rounded again
-    again = unit if reduction == "none" else 0.0
+    again = unit if reduction == "none" and kind != F16 else 0.0
     bw = (f.abs() * dy).t() @ X.abs() + ((2 * x.shape[0] + 2) * U + extra + again) * ((f * y).abs().t() @ X.abs())
     bb = (f.abs() * dy).sum(0) + (x.shape[0] + 4) * U * (f * y).abs().sum(0)
-    if kind == F32:
+    if kind != F16:      # operands to a common power of two: the smallest entries
         bx = bx + f.abs() * 2.0 ** -39 * float(W.abs().max()) * y.abs().sum(1, keepdim=True)
-        bw = bw + 2.0 ** -39 * float(X.abs().max()) * (f * y).abs().sum(0).unsqueeze(1)
-    if kind == F16 and reduction == "none":      # weighted rows of x below the normal range of float16
-        bw = bw + 2.0 ** -25 * float(f.abs().max()) * (y.abs().sum(0)).unsqueeze(1)
+        bw = bw + 2.0 ** -39 * float(X.abs().max()) * float(f.abs().max()) * y.abs().sum(0).unsqueeze(1)
     end = lambda bound, ref: (bound + (_round(kind) + 8 * U) * ref.abs() + _tiny(kind)).nan_to_num(INF)
     # For the error as a whole: the d roundings of a logit's partial sums, each at most U times a partial sum of at most sum |x w|, have
     # random signs and the partial sums grow with the square root of their length, so that they add up to a few U sum |x w|.  What is
@@ -402,12 +402,12 @@ def _check_ce(x, w, b, t, reduction, ignore=IGNORE, norms=True):
     _within(loss, want, bound, "loss")
     # the bounds are for the worst case; roundings of many terms rarely agree in sign, so that the error as a whole stays within a few
     # units of the roundings of p - t and of the result, beside that of p
-    unit = (4 * U if x.dtype == F32 else _round(x.dtype)) * 2
+    unit = 4 * (_round(F16) if x.dtype == BF16 else 4 * U) + 2 * _round(x.dtype) + 64 * U
     for name, got, (ref, gb, of_p) in zip(("dx", "dw", "db"), grads, pairs):
         _within(got, ref, gb, name)
         if norms and ref.isfinite().all() and float(ref.norm()) > 0:
             off = float((got.double() - ref).norm())
-            assert off <= (4 * unit + 64 * U) * float(ref.norm()) + of_p + ref.numel() ** 0.5 * _tiny(x.dtype), (name, off, float(ref.norm()))
+            assert off <= unit * float(ref.norm()) + of_p + ref.numel() ** 0.5 * _tiny(x.dtype), (name, off, float(ref.norm()))
     return loss, grads
 
 
