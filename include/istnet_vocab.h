@@ -55,17 +55,17 @@ ISTNET_PN2_API int istnet_distill_backward(long long n, int v, int k, int dtype,
  *   z = x w^T + bias,  row = log sum_v exp z_v - z_target,  loss = per row (reduction 0), sum (2) or mean over the counted rows (1).
  * Rows whose target is `ignore` do not count (loss 0; they are not looked at); any other target outside [0, v) makes the row NaN.
  * The logits are formed piece by piece and never kept.  keep (istnet_linear_ce_keep_kib, for the same w and ldw) carries the packed
- * operands and row statistics from the forward to the backward of the same call, ws (istnet_linear_ce_scratch_kib) is scratch.
- * n <= 2^22, d <= 2^20, v <= 2^28. */
-ISTNET_PN2_API int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, const void *w, long long ldw);
+ * operands and row statistics from the forward to the backward of the same call; train == 0: there will be none.  ws
+ * (istnet_linear_ce_scratch_kib) is scratch.  n <= 2^22, d <= 2^20, v <= 2^28, n v <= 2^38. */
+ISTNET_PN2_API int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, int train, const void *w, long long ldw);
 ISTNET_PN2_API int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward);
-ISTNET_PN2_API int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, const void *x, long long ldx,
-                                            const void *w, long long ldw, const void *bias, const void *target, long long ignore,
+ISTNET_PN2_API int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, int train, const void *x,
+                                            long long ldx, const void *w, long long ldw, const void *bias, const void *target, long long ignore,
                                             int reduction, float *loss, void *keep, void *ws, void *stream);
 /* dx (n, d), dw (v, d), db (v), contiguous, each may be NULL; gout as for istnet_distill_backward. */
-ISTNET_PN2_API int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void *x, long long ldx, const void *w,
-                                             long long ldw, int has_bias, int reduction, const float *gout, void *keep, void *ws,
-                                             void *dx, void *dw, void *db, void *stream);
+ISTNET_PN2_API int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void *x, long long ldx, int has_bias,
+                                             int reduction, const float *gout, void *keep, void *ws, void *dx, void *dw, void *db,
+                                             void *stream);
 
 #ifdef __cplusplus
 }

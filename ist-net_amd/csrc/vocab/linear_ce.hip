@@ -12,15 +12,20 @@
 // Rows whose target is ignore_index are left out before the products: the rows that count are packed (padded to whole tiles with
 // zeros), so masked rows cost nothing and whatever they hold is not looked at.
 //
-// Numbers.  The logits of bfloat16 and float16 operands are exact products summed in float32.  A float32 operand is held as two
-// float16 numbers to a common power of two, x = 2^-e (hi + lo), and a product is hi hi + hi lo + lo hi: 22 bits of each factor, the
-// dropped lo lo is 2^-22 of the product at most; entries smaller than 2^-17 of the largest one keep an absolute error of 2^-39 of
-// that.  Three half-precision products run at three times the rate of one float32 product on this chip.
-// p - t is rounded once the target is taken off, always to float16 numbers scaled by 2^14, and always to more bits than the gradients
-// have, because an error of p - t of the result's own rounding would add as much again to it: one number (11 bits) for bfloat16
-// operands, which are turned into float16 ones with an exponent in common for this (exact down to 2^-29 of the largest entry), hi + lo
-// (22 bits) for float16 and float32 ones.  All sums are float32.
+// Numbers.  The matrix cores are fed float16.  bfloat16 operands are turned into float16 ones with an exponent in common (exact down to
+// 2^-29 of the largest entry, an absolute error of 2^-40 of it below).  A float32 operand is held as two float16 numbers with an
+// exponent in common, x = 2^-e (hi + lo), and a product is hi hi + hi lo + lo hi: 22 bits of each factor, the dropped lo lo is 2^-22 of
+// the product at most; entries smaller than 2^-17 of the largest one keep an absolute error of 2^-39 of that.  Three half-precision
+// products run at three times the rate of one float32 product on this chip.  p - t is rounded once the target is taken off, scaled
+// by 2^14, and to more bits than the gradients have, because an error of p - t of the result's own rounding would add as much again to
+// it: one float16 number (11 bits) for bfloat16 operands, hi + lo (22 bits) for float16 and float32 ones.  All sums are float32.
+//
+// Layout.  Packed operands and p - t lie in panels of 32 columns: element (r, c) at ((c / 32) rows + r) 32 + c % 32.  A step of 32 along
+// a row of a tile is then R consecutive rows of 64 bytes, and a step of 32 along a column is R / 32 runs of 2 KB, so that every load of
+// a tile is a run of whole cache lines: from rows as they usually lie a step takes half a line of each row, and the L2 delivers half
+// its rate (8192 x 65536 x 1024 bf16, loads alone: 828 us from rows, 580 us from panels; the whole product 1140 and 986 us).
 #include <algorithm>
+#include <type_traits>
 
 #include "vocab_common.h"
 
@@ -42,13 +47,14 @@ constexpr float kDzScale = 16384.f;      // p - t in float16: 1 -> 2^14, so that
 
 // ---- the product ----------------------------------------------------------------------------------------------------------
 
-// An operand: `ld` elements between its rows.  Along-K rows ("KC"): row r of the tile is a row of memory, K is contiguous.
-// Across-K rows ("KS"): K runs over the rows of memory and the tile's index is contiguous.  Rows beyond `last_row` and (KS) blocks
-// of eight columns beyond `last_col8` are replaced by the last one: what they give is multiplied by zero or not stored.
+// An operand's memory: 16-bit element (r, c) at r * row_stride + (c / 32) * unit_stride + (c % 32) * 2 bytes -- panels (row_stride 64,
+// unit_stride 64 rows), or rows as they lie (row_stride 2 ld, unit_stride 64).  As a KC operand its rows are the tile's index and its
+// columns K; as a KS operand its rows are K and its columns the tile's index.  Rows beyond `last_row` and (KS) units of 32 columns
+// beyond `last_unit` are replaced by the last one: what they give is multiplied by zero or not stored.
 struct Operand {
-  const uint16_t* plane[2];      // float32: hi, lo; else both the same
-  long long ld;
-  int last_row, last_col8;
+  const char* plane[2];      // hi, lo where there are two
+  long long row_stride, unit_stride;
+  int last_row, last_unit;
 };
 
 // What the backward needs of a row: p_v = inv * 2^(z_v - ref) in log2 units; the derivative at the target, p_t - 1, comes from the
@@ -64,10 +70,10 @@ struct Epilogue {
   const RowStat* stat;           // per packed row
   float2* part;                  // [class tile][packed row]: largest of the other classes' logits in log2 units, sum of exponentials
   float* zt;                     // the target's logit as the product left it (with a bias: finished, in log2 units)
-  uint16_t* dz[2];               // [packed row][piece], float16 hi (and lo)
+  uint16_t* dz[2];               // panels of [packed row][32], float16 hi (and lo)
   const int* rowmap;             // with weights: packed row -> row
   const float* weights;          // weights of the rows' losses where they are taken into p - t, or null
-  long long ld_dz;
+  long long dz_unit;             // bytes of a panel
   int v, v0;                     // classes in all, first class of the piece
   int parts_ld;
   // gradients
@@ -80,11 +86,12 @@ struct Epilogue {
 };
 
 // device scalars
-// (kXScale, kWScale: of the packed operands; kXBack, kWBack: of those that the gradients are formed from)
-enum Scal { kCount = 0, kLogitScale = 1, kXScale = 2, kWScale = 3, kGMax = 4, kXBack = 5, kWBack = 6, kScalars = 8 };
+enum Scal { kCount = 0, kLogitScale = 1, kXScale = 2, kWScale = 3, kGMax = 4, kScalars = 8 };
 
-__device__ __forceinline__ int swz_kc(int row) { return ((row >> 1) ^ (row >> 3)) & 3; }
-template <int R> __device__ __forceinline__ int swz_ks(int k) { return R >= 256 ? ((k & 3) | (((k >> 3) & 1) << 2)) : (k & 3); }
+// A KC tile in LDS: rows of 64 bytes, their 16-byte chunks exchanged so that the sixteen lanes that read together (rows of four groups
+// of four, of which no two fall on the same chunk) cover all 64 banks.  A KS tile: units of 32 x 64 bytes, read by the transposing loads
+// 256 consecutive bytes at a time.
+__device__ __forceinline__ int swz_kc(int row) { return (row >> 2) & 3; }
 
 // sixteen bytes per lane from memory to LDS at `lds` + 16 * lane, past the registers.  Inline: the compiler would wait for every such
 // load before the next LDS read; the waits are placed by hand.  Nothing else in these kernels uses m0, and it takes one wait state
@@ -105,37 +112,28 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 
 template <bool KS, int R, int WAVES> struct Stager {
   static constexpr int LOADS = R * 4 / (64 * WAVES);      // sixteen-byte chunks per lane and step
-  static constexpr int CPR = KS ? R / 8 : 4;              // chunks per row of the tile in LDS
-  uint32_t off[LOADS];
+  uint32_t off[KS ? 1 : LOADS];
   __device__ __forceinline__ void init(const Operand& o, int first, int wave, int lane) {
+    if constexpr (!KS) {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int p = (j * WAVES + wave) * 64 + lane, row = p / CPR, pos = p % CPR;
-      if constexpr (KS) {
-        const int c8 = min(first / 8 + ((((pos >> 2) ^ swz_ks<R>(row)) << 2) | (pos & 3)), o.last_col8);
-        off[j] = (uint32_t)(row * o.ld * 2 + (long long)(c8 - first / 8) * 16);      // first / 8 <= last_col8: not negative beyond the tile
-      } else {
-        const int r = min(first + row, o.last_row) - first;
-        off[j] = (uint32_t)(r * o.ld * 2 + ((pos ^ swz_kc(row)) << 4));
+      for (int j = 0; j < LOADS; ++j) {
+        const int row = ((j * WAVES + wave) * 64 + lane) >> 2, r = min(first + row, o.last_row) - first;
+        off[j] = (uint32_t)(r * o.row_stride) + (((lane & 3) ^ swz_kc(row)) << 4);
       }
     }
   }
-  // step `k0` (first K) of the operand's plane
-  __device__ __forceinline__ void issue(const Operand& o, int plane, int first, int k0, uint32_t lds, int wave, int lane) {
+  // step k (of 32) of the operand's plane
+  __device__ __forceinline__ void issue(const Operand& o, int plane, int first, int k, uint32_t lds, int wave, int lane) {
     if constexpr (KS) {
-      const uint16_t* base = o.plane[plane] + (long long)k0 * o.ld + first;
-      if (k0 + BK - 1 <= o.last_row) {
+      const char* base = o.plane[plane] + (long long)k * 32 * o.row_stride;
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) load_lds16(base, off[j], lds + (j * WAVES + wave) * 1024);
-      } else {
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          const int row = ((j * WAVES + wave) * 64 + lane) / CPR, over = max(0, k0 + row - o.last_row);
-          load_lds16(base, off[j] - (uint32_t)(over * o.ld * 2), lds + (j * WAVES + wave) * 1024);
-        }
+      for (int j = 0; j < LOADS; ++j) {
+        const int q = j * WAVES + wave, unit = min((first >> 5) + (q >> 1), o.last_unit);      // a wave's load is half a unit
+        const int row = min((q & 1) * 16 + (lane >> 2), o.last_row - k * 32);
+        load_lds16(base + unit * o.unit_stride, (uint32_t)(row * o.row_stride) + ((lane & 3) << 4), lds + q * 1024);
       }
     } else {
-      const uint16_t* base = o.plane[plane] + (long long)first * o.ld + k0;
+      const char* base = o.plane[plane] + (long long)first * o.row_stride + k * o.unit_stride;
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) load_lds16(base, off[j], lds + (j * WAVES + wave) * 1024);
     }
@@ -143,32 +141,28 @@ template <bool KS, int R, int WAVES> struct Stager {
 };
 
 // lane addresses of an operand's fragments in its LDS tile
-template <bool KS, int R, int BLOCKS> struct Reader {
-  static constexpr int N = KS ? BLOCKS : 2;
-  uint32_t at[N];
+template <bool KS> struct Reader {
+  uint32_t at[KS ? 1 : 2];
   __device__ __forceinline__ void init(int first, int lane) {
     if constexpr (KS) {
-      const int k = ((lane >> 5) << 3) + ((lane & 15) >> 2);
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-        at[b] = k * R * 2 + (((first / 32 + b) ^ swz_ks<R>(k)) << 6) + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3);
+      at[0] = (first >> 5) * 2048 + (((lane >> 5) << 3) + ((lane & 15) >> 2)) * 64 + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3);
     } else {
       const int row = first + (lane & 31);
 #pragma unroll
       for (int s = 0; s < 2; ++s) at[s] = row * 64 + (((2 * s + (lane >> 5)) ^ swz_kc(row)) << 4);
     }
   }
-  // the 32 x 16 fragment of block b, half s of the step
+  // the 32 x 16 fragment of block b, half s of the step: lane l holds row l % 32, K 8 (l / 32) .. + 7
   __device__ __forceinline__ s16x8 get(const char* tile, int b, int s) const {
     typedef __attribute__((address_space(3))) s16x4 lds4;
     typedef __attribute__((address_space(3))) s16x8 lds8;
     const auto t = (const __attribute__((address_space(3))) char*)tile;
-    if constexpr (KS) {
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(t + at[b] + s * 16 * R * 2));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(t + at[b] + s * 16 * R * 2 + 4 * R * 2));
+    if constexpr (KS) {      // each of sixteen lanes names 8 bytes of four rows of K, and gets one column of the four
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(t + at[0] + b * 2048 + s * 1024));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(t + at[0] + b * 2048 + s * 1024 + 256));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      return *(const lds8*)(t + at[s] + b * 32 * 64);
+      return *(const lds8*)(t + at[s] + b * 2048);
     }
   }
 };
@@ -234,8 +228,8 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   Stager<BKS, NT, WAVES> sb;
   sa.init(a, m0, wave, lane);
   sb.init(b, n0, wave, lane);
-  Reader<AKS, MT, MB> ra;
-  Reader<BKS, NT, NB> rb;
+  Reader<AKS> ra;
+  Reader<BKS> rb;
   ra.init(wm * MT / 2, lane);
   rb.init(wn * NT / 2, lane);
   constexpr int LOADS = Stager<AKS, MT, WAVES>::LOADS + Stager<BKS, NT, WAVES>::LOADS;
@@ -244,34 +238,53 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   int seg = SEGS > 1 ? t0 / max(ksteps, 1) : 0, k = t0 - seg * ksteps, slot = 0;      // of the next step to load
   auto issue = [&]() {
     const int pa = SEGS == 3 ? (seg == 0) : 0, pb = SEGS == 3 ? (seg == 1) : SEGS == 2 ? (seg == 0) : 0;
-    sa.issue(a, pa, m0, k * BK, lds0 + slot * STAGE, wave, lane);
-    sb.issue(b, pb, n0, k * BK, lds0 + slot * STAGE + ABYTES, wave, lane);
+    sa.issue(a, pa, m0, k, lds0 + slot * STAGE, wave, lane);
+    sb.issue(b, pb, n0, k, lds0 + slot * STAGE + ABYTES, wave, lane);
     slot = slot == kStages - 1 ? 0 : slot + 1;
     if (++k == ksteps) { k = 0; ++seg; }
   };
-  if (t0 < t1) issue();
-  if (t0 + 1 < t1) issue();
+  // A step is two halves of K.  The fragments of a half are read from LDS while the products of the half before run; the barrier, behind
+  // which the next step's first half can be read, stands between the two.
+  s16x8 fa[2][MB], fb[2][NB];
+  auto read = [&](int slot_, int s) {
+    const char* at = lds + slot_ * STAGE;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) fa[s][i] = ra.get(at, i, s);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) fb[s][j] = rb.get(at + ABYTES, j, s);
+  };
+  auto multiply = [&](int s) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = mfma<M>(fa[s][i], fb[s][j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (t0 < t1) {
+    issue();
+    if (t0 + 1 < t1) {
+      issue();
+      wait_loads<LOADS>();
+    } else {
+      wait_loads<0>();
+    }
+    barrier();
+    read(0, 0);
+  }
   int from = 0;
   for (int t = t0; t < t1; ++t) {
-    // this step's loads have landed (those of the next may still be under way), for every wave; and every wave is done with the slot
-    // of the step before, which is the one the next loads go to
-    if (t + 1 < t1) wait_loads<LOADS>(); else wait_loads<0>();
-    barrier();
+    read(from, 1);
+    // into the slot of the step before: its last reads were in registers before the last barrier
     if (t + 2 < t1) issue();
-    const char* at = lds + from * STAGE;
+    multiply(0);
     from = from == kStages - 1 ? 0 : from + 1;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      s16x8 fa[MB], fb[NB];
-#pragma unroll
-      for (int i = 0; i < MB; ++i) fa[i] = ra.get(at, i, s);
-#pragma unroll
-      for (int j = 0; j < NB; ++j) fb[j] = rb.get(at + ABYTES, j, s);
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = mfma<M>(fa[i], fb[j], acc[i][j]);
+    if (t + 1 < t1) {
+      if (t + 2 < t1) wait_loads<LOADS>(); else wait_loads<0>();
+      barrier();
+      read(from, 0);
     }
+    multiply(1);
   }
   wait_loads<0>();
   barrier();      // the tiles' LDS is free
@@ -381,14 +394,16 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
           }
       }
       // a wave reads what it wrote itself: LDS keeps its order
-      constexpr int CH = MT / 16;      // sixteen-byte chunks of a row
-      uint16_t* out = e.dz[pl] + (long long)(n0 + wn * ROWS) * e.ld_dz + mw;
+      char* out = reinterpret_cast<char*>(e.dz[pl]) + (mw >> 5) * e.dz_unit + (long long)(n0 + wn * ROWS) * 64;
       asm volatile("" ::: "memory");
 #pragma unroll
-      for (int q = 0; q < ROWS * CH / 64; ++q) {
-        const int p = q * 64 + lane, row = p / CH, ch = p % CH;
-        *reinterpret_cast<u32x4*>(out + row * e.ld_dz + ch * 8) = *reinterpret_cast<const u32x4*>(mine + row * PITCH + ch * 8);
-      }
+      for (int u = 0; u < MT / 64; ++u)
+#pragma unroll
+        for (int q = 0; q < ROWS / 16; ++q) {
+          const int row = q * 16 + (lane >> 2);
+          *reinterpret_cast<u32x4*>(out + u * e.dz_unit + row * 64 + ((lane & 3) << 4)) =
+              *reinterpret_cast<const u32x4*>(mine + row * PITCH + u * 32 + (lane & 3) * 8);
+        }
       asm volatile("" ::: "memory");
     }
   } else if constexpr (EPI == kSlab) {
@@ -414,7 +429,7 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   } else {
     const float rows = e.scal[kCount];
     const float g = e.reduction == 0 ? e.scal[kGMax] : e.reduction == 1 ? e.gout[0] / rows : e.gout[0];
-    const float f = rows == 0.f ? 0.f : g / kDzScale / e.scal[kXBack];
+    const float f = rows == 0.f ? 0.f : g / kDzScale / e.scal[kXScale];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int n = n0 + wn * (NT / 2) + j * 32 + col;
@@ -467,8 +482,9 @@ __device__ __forceinline__ void store_amax(float m, float* tmp, float* part) {
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
 }
 // the largest magnitude of the rows of x that count ([0, xwgs)) and of w, one value per workgroup
-__global__ __launch_bounds__(256) void ce_amax_kernel(int n, int v, int d, const float* __restrict__ x, long long ldx,
-                                                      const float* __restrict__ w, long long ldw, const void* __restrict__ target,
+template <typename T>
+__global__ __launch_bounds__(256) void ce_amax_kernel(int n, int v, int d, const T* __restrict__ x, long long ldx,
+                                                      const T* __restrict__ w, long long ldw, const void* __restrict__ target,
                                                       int idx64, long long ignore, int xwgs, float* __restrict__ part) {
   __shared__ float tmp[4];
   const int wave = threadIdx.x >> 6;
@@ -481,21 +497,6 @@ __global__ __launch_bounds__(256) void ce_amax_kernel(int n, int v, int d, const
   }
   store_amax(m, tmp, part);
 }
-// the same of packed rows
-__global__ __launch_bounds__(256) void ce_amax_packed_kernel(int kp, const bf16* __restrict__ xp, const float* __restrict__ scal, int v,
-                                                             int d, const bf16* __restrict__ w, long long ldw, int xwgs,
-                                                             float* __restrict__ part) {
-  __shared__ float tmp[4];
-  const int wave = threadIdx.x >> 6, count = (int)scal[kCount];
-  float m = 0.f;
-  if ((int)blockIdx.x < xwgs) {
-    for (int r = blockIdx.x * 4 + wave; r < count; r += xwgs * 4) m = row_amax(xp + (long long)r * kp, kp, m);
-  } else {
-    for (int r = (blockIdx.x - xwgs) * 4 + wave; r < v; r += (gridDim.x - xwgs) * 4) m = row_amax(w + r * ldw, d, m);
-  }
-  store_amax(m, tmp, part);
-}
-
 // counted rows per block of 256
 __global__ __launch_bounds__(256) void ce_count_kernel(int n, const void* __restrict__ target, int idx64, long long ignore,
                                                        int* __restrict__ blocks) {
@@ -568,62 +569,59 @@ __global__ __launch_bounds__(1024) void ce_plan_kernel(int n, int counted, const
     scal[kXScale] = sx;
     scal[kWScale] = sw;
     scal[kGMax] = 1.f;
-    scal[kXBack] = sx;
-    scal[kWBack] = sw;
   }
 }
 
-// scales of bfloat16 operands as float16 ones
-__global__ __launch_bounds__(1024) void ce_scales_kernel(int xwgs, int wgs, const float* __restrict__ amax, float* __restrict__ scal) {
-  __shared__ float tmx[16], tmw[16];
-  const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
-  const float m = i < wgs ? amax[i] : 0.f, mx = wave_max(i < xwgs ? m : 0.f), mw = wave_max(i < xwgs ? 0.f : m);
-  if (lane == 0) { tmx[wave] = mx; tmw[wave] = mw; }
-  __syncthreads();
-  if (i == 0) {
-    float x = 0.f, w = 0.f;
-    for (int k = 0; k < 16; ++k) { x = fmaxf(x, tmx[k]); w = fmaxf(w, tmw[k]); }
-    scal[kXBack] = scale_for(x);
-    scal[kWBack] = scale_for(w);
-  }
-}
-
-// eight elements of a row, scaled and rounded (P == 2: split), as they lie in the packed operand
-template <typename T, int P>
+// Eight elements of a row as they lie in a packed operand: float16, scaled (P == 2: split); RAW: as they are.
+template <typename T, int P, bool RAW>
 __device__ __forceinline__ void pack8(const T* src, int left, float scale, u32x4* hi, u32x4* lo) {
-  float f[8];
   if constexpr (sizeof(T) == 2) {
+    float f[8];
     load_part(src, left, f);
-    if (scale != 1.f) {
+    if constexpr (RAW) {
+      *hi = pack<T>(f);
+    } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] *= scale;
+      *hi = pack<f16>(f);
     }
-    *hi = pack<T>(f);
   } else {
-    float g[4], h[4];
+    float f[8], g[4], h[4], r[8];
     load_part(src, left, g);
     load_part(src + 4, left - 4, h);
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[i] = g[i] * scale; f[4 + i] = h[i] * scale; }
-    float r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = f[i] - (float)(f16)f[i];
     *hi = pack<f16>(f);
     *lo = pack<f16>(r);
   }
 }
+// sixteen rows into panels: a lane has one row (`src`, null: zeros; `to` < 0: none) and one chunk of a panel, a wave every fourth panel
+template <typename T, int P, bool RAW>
+__device__ __forceinline__ void pack_rows(const T* src, int to, int d, int kp, long long rows, float scale, char* out, long long plane) {
+  if (to < 0) return;
+  for (int u = threadIdx.x >> 6; u < kp / 32; u += 4) {
+    const int c = u * 32 + (threadIdx.x & 3) * 8;
+    u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+    if (src) pack8<T, P, RAW>(src + c, d - c, scale, &hi, &lo);
+    char* p = out + u * rows * 64 + (long long)to * 64 + ((threadIdx.x & 3) << 4);
+    *reinterpret_cast<u32x4*>(p) = hi;
+    if constexpr (P == 2) *reinterpret_cast<u32x4*>(p + plane) = lo;
+  }
+}
 
-// Packed rows of x (and of w where its own rows cannot be read as they are), the bias in log2 units.  Workgroups [0, xwgs): 16 rows of
-// x each; the next 16: the zeros behind the last packed row; the rest: 4 rows of w each step, and the bias.
+// Packed rows of x (and of w unless it is read as it lies), the bias in log2 units.  Workgroups [0, xwgs): 16 rows of x each; the next
+// 16: the zeros behind the last packed row; the rest: 16 rows of w a step, and the bias.
 constexpr int kPackRows = 16;
-template <typename T, int P>
+template <typename T, int P, bool RAW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(int n, int v, int d, int kp, int vp, const T* __restrict__ x, long long ldx,
                                                       const T* __restrict__ w, long long ldw, const T* __restrict__ bias,
                                                       const void* __restrict__ target, int idx64, long long ignore, int xwgs,
-                                                      int pack_w, const int* __restrict__ blocks, const float* __restrict__ scal,
-                                                      uint16_t* __restrict__ xp, long long xplane, uint16_t* __restrict__ wp,
-                                                      long long wplane, float* __restrict__ bias2, int* __restrict__ rowmap,
-                                                      int* __restrict__ inverse, int* __restrict__ tgt, float* __restrict__ row_loss) {
+                                                      const int* __restrict__ blocks, const float* __restrict__ scal,
+                                                      char* __restrict__ xp, long long np, char* __restrict__ wp,
+                                                      float* __restrict__ bias2, int* __restrict__ rowmap, int* __restrict__ inverse,
+                                                      int* __restrict__ tgt, float* __restrict__ row_loss) {
   __shared__ int flag[4];
   __shared__ int where[256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wg = blockIdx.x;
@@ -648,45 +646,33 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(int n, int v, int d, int k
       }
     }
     __syncthreads();
-    const float s = scal[kXScale];
-    for (int r = r0 + wave; r < r0 + kPackRows; r += 4) {
-      const int to = where[r];
-      if (to < 0) continue;
-      const T* src = x + (long long)(block * 256 + r) * ldx;
-      for (int c = lane * 8; c < kp; c += 512) {
-        u32x4 hi, lo;
-        pack8<T, P>(src + c, d - c, s, &hi, &lo);
-        store16(xp + (long long)to * kp + c, hi);
-        if constexpr (P == 2) store16(xp + xplane + (long long)to * kp + c, lo);
-      }
-    }
+    const int r = r0 + (lane >> 2), to = where[r];
+    pack_rows<T, P, RAW>(to < 0 ? nullptr : x + (long long)(block * 256 + r) * ldx, to, d, kp, np, scal[kXScale], xp, np * kp * 2);
   } else if (wg < xwgs + kPad / kPackRows) {
-    const int count = (int)scal[kCount], end = (count + kPad - 1) / kPad * kPad, r0 = count + (wg - xwgs) * kPackRows;
-    const u32x4 zero = {0, 0, 0, 0};
-    for (int r = r0 + wave; r < min(end, r0 + kPackRows); r += 4) {
-      for (int c = lane * 8; c < kp; c += 512) {
-        store16(xp + (long long)r * kp + c, zero);
-        if constexpr (P == 2) store16(xp + xplane + (long long)r * kp + c, zero);
-      }
-      if (lane == 0) tgt[r] = -2;
-    }
+    const int count = (int)scal[kCount], end = (count + kPad - 1) / kPad * kPad, r = count + (wg - xwgs) * kPackRows + (lane >> 2);
+    pack_rows<T, P, RAW>(nullptr, r < end ? r : -1, d, kp, np, 1.f, xp, np * kp * 2);
+    if (r < end && wave == 0 && (lane & 3) == 0) tgt[r] = -2;
   } else {
     const int first = wg - xwgs - kPad / kPackRows, wgs = gridDim.x - xwgs - kPad / kPackRows;
-    for (int c = first * 256 + threadIdx.x; c < vp; c += wgs * 256)
-      bias2[c] = c >= v ? -INFINITY : bias ? kLog2e * to_f32(bias[c]) : 0.f;
-    if (pack_w) {
-      const float s = scal[kWScale];
-      for (int r = first * 4 + wave; r < v; r += wgs * 4) {
-        const T* src = w + r * ldw;
-        for (int c = lane * 8; c < kp; c += 512) {
-          u32x4 hi, lo;
-          pack8<T, P>(src + c, d - c, s, &hi, &lo);
-          store16(wp + (long long)r * kp + c, hi);
-          if constexpr (P == 2) store16(wp + wplane + (long long)r * kp + c, lo);
-        }
+    if (bias)
+      for (int c = first * 256 + threadIdx.x; c < vp; c += wgs * 256) bias2[c] = c < v ? kLog2e * to_f32(bias[c]) : -INFINITY;
+    if (wp)
+      for (int r0 = first * kPackRows; r0 < v; r0 += wgs * kPackRows) {
+        const int r = r0 + (lane >> 2);
+        pack_rows<T, P, RAW>(w + (long long)(r < v ? r : 0) * ldw, r < v ? r : -1, d, kp, v, scal[kWScale], wp, (long long)v * kp * 2);
       }
-    }
   }
+}
+
+// Packed rows of g_i / max |g| * x_i: what dw is formed from where the rows' losses have weights of their own.
+template <typename T, int P>
+__global__ __launch_bounds__(256) void ce_weigh_kernel(int d, int kp, const T* __restrict__ x, long long ldx,
+                                                       const float* __restrict__ gout, const int* __restrict__ rowmap,
+                                                       const float* __restrict__ scal, char* __restrict__ xp, long long np) {
+  const int count = (int)scal[kCount], end = (count + kPad - 1) / kPad * kPad, r = blockIdx.x * kPackRows + ((threadIdx.x & 63) >> 2);
+  const int i = r < count ? rowmap[r] : -1;
+  pack_rows<T, P, false>(i < 0 ? nullptr : x + (long long)i * ldx, r < end ? r : -1, d, kp, np,
+                         i < 0 ? 0.f : gout[i] / scal[kGMax] * scal[kXScale], xp, np * kp * 2);
 }
 
 // statistics and loss of 16 packed rows per workgroup, from the tiles' partial sums
@@ -768,52 +754,6 @@ __global__ __launch_bounds__(1024) void ce_gmax_kernel(const float* __restrict__
   }
 }
 
-// eight elements as float16 (P == 2: hi and lo) whatever their type
-template <typename T, int P>
-__device__ __forceinline__ void pack8_f16(const T* src, int left, float scale, u32x4* hi, u32x4* lo) {
-  if constexpr (__is_same(T, bf16)) {
-    float f[8];
-    load_part(src, left, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= scale;
-    *hi = pack<f16>(f);
-  } else {
-    pack8<T, P>(src, left, scale, hi, lo);
-  }
-}
-
-// Packed float16 rows that dw is formed from: of g_i / max |g| * x_i where the rows' losses have weights of their own, of x_i else.
-template <typename T, int P>
-__global__ __launch_bounds__(256) void ce_back_x_kernel(int d, int kp, const T* __restrict__ x, long long ldx,
-                                                        const float* __restrict__ gout, const int* __restrict__ rowmap,
-                                                        const float* __restrict__ scal, uint16_t* __restrict__ xp, long long xplane) {
-  const int count = (int)scal[kCount], end = (count + kPad - 1) / kPad * kPad, lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= end) return;
-  const int i = r < count ? rowmap[r] : -1;
-  const float s = i < 0 ? 0.f : gout ? gout[i] / scal[kGMax] * scal[kXBack] : scal[kXBack];
-  for (int c = lane * 8; c < kp; c += 512) {
-    u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-    if (i >= 0) pack8_f16<T, P>(x + (long long)i * ldx + c, d - c, s, &hi, &lo);
-    store16(xp + (long long)r * kp + c, hi);
-    if constexpr (P == 2) store16(xp + xplane + (long long)r * kp + c, lo);
-  }
-}
-
-// rows of a piece of bfloat16 w as float16
-__global__ __launch_bounds__(256) void ce_back_w_kernel(int rows, int d, int kp, const bf16* __restrict__ w, long long ldw,
-                                                        const float* __restrict__ scal, uint16_t* __restrict__ wp) {
-  const int lane = threadIdx.x & 63;
-  const float s = scal[kWBack];
-  for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4) {
-    for (int c = lane * 8; c < kp; c += 512) {
-      u32x4 hi, lo;
-      pack8_f16<bf16, 1>(w + r * ldw + c, d - c, s, &hi, &lo);
-      store16(wp + (long long)r * kp + c, hi);
-    }
-  }
-}
-
 // dx: slabs added in order, scaled, back to the rows they belong to; rows that do not count get zeros
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, const float* __restrict__ slab, long long slab_stride,
@@ -833,7 +773,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, co
       for (int r = 0; r < 4; ++r) x[r] += y[r];
     }
     const float g = (folded ? scal[kGMax] : reduction == 0 ? gout[i] : reduction == 1 ? gout[0] / scal[kCount] : gout[0]) / kDzScale /
-                    scal[kWBack];
+                    scal[kWScale];
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] *= g;
   }
@@ -842,46 +782,57 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, co
     if (c + r < d) dx[i * d + c + r] = from_f32<T>(x[r]);
 }
 
-// dw where its product was split along the rows
+// dw where its product was split along the rows: four parts of the slabs side by side, each in order, joined in order
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dw_kernel(int rows, int d, int splits, const float* __restrict__ slab, long long slab_stride,
                                                     long long ld, const float* __restrict__ gout, int reduction,
                                                     const float* __restrict__ scal, T* __restrict__ dw) {
-  const int per = (d + 3) / 4;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, i = id / per;
-  if (i >= rows) return;
+  __shared__ f32x4 tmp[256];
+  const int per = (d + 3) / 4, part = threadIdx.x >> 6, each = (splits + 3) / 4;
+  const long long id = (long long)blockIdx.x * 64 + (threadIdx.x & 63), i = id / per;
   const int c = (int)(id % per) * 4;
-  const float* p = slab + i * ld + c;
-  f32x4 x = *reinterpret_cast<const f32x4*>(p);
-  for (int s = 1; s < splits; ++s) {
-    const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * slab_stride);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (i < rows) {
+    const float* p = slab + i * ld + c;
+#pragma unroll 8
+    for (int s = part * each; s < min(splits, (part + 1) * each); ++s) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * slab_stride);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] += y[r];
+      for (int r = 0; r < 4; ++r) x[r] += y[r];
+    }
   }
+  tmp[threadIdx.x] = x;
+  __syncthreads();
+  if (part || i >= rows) return;
+  for (int s = 1; s < 4; ++s)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] += tmp[s * 64 + threadIdx.x][r];
   const float n = scal[kCount];
-  const float g = n == 0.f ? 0.f : (reduction == 0 ? scal[kGMax] : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale / scal[kXBack];
+  const float g = n == 0.f ? 0.f : (reduction == 0 ? scal[kGMax] : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale / scal[kXScale];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (c + r < d) dw[i * d + c + r] = from_f32<T>(g * x[r]);
 }
 
-// db: column sums of p - t over the packed rows, `chunks` parts of the rows side by side, joined in order
+// db: column sums of p - t over the packed rows.  A workgroup has one panel and `chunk` rows: sixteen rows times four chunks of eight
+// columns per wave, the lanes of a column added up in a fixed order.
 template <int PD>
-__global__ __launch_bounds__(256) void ce_colsum_kernel(int width, const uint16_t* __restrict__ hi, const uint16_t* __restrict__ lo,
-                                                        long long ld, const float* __restrict__ gout, const int* __restrict__ rowmap,
-                                                        const float* __restrict__ scal, int chunks, float* __restrict__ part) {
-  const int c = (blockIdx.x * 64 + (threadIdx.x & 63)) * 8, chunk = blockIdx.y * 4 + (threadIdx.x >> 6);
-  const int count = (int)scal[kCount], per = (count + chunks - 1) / chunks, a = chunk * per, b = min(count, a + per);
-  if (c >= width) return;
+__global__ __launch_bounds__(256) void ce_colsum_kernel(const char* __restrict__ hi, const char* __restrict__ lo, long long unit_stride,
+                                                        int width, const float* __restrict__ gout, const int* __restrict__ rowmap,
+                                                        const float* __restrict__ scal, int chunk, float* __restrict__ part) {
+  __shared__ float tmp[4][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = (int)scal[kCount];
+  const int a = blockIdx.y * chunk, b = min(count, a + chunk);
+  const long long at = blockIdx.x * unit_stride + ((lane & 3) << 4);
   float s[8] = {};
 #pragma unroll 4
-  for (int r = a; r < b; ++r) {
+  for (int r = a + wave * 16 + (lane >> 2); r < b; r += 64) {
     const float g = gout ? gout[rowmap[r]] : 1.f;
     float f[8];
-    unpack<f16>(*reinterpret_cast<const u32x4*>(hi + r * ld + c), f);
+    unpack<f16>(*reinterpret_cast<const u32x4*>(hi + at + r * 64ll), f);
     if constexpr (PD == 2) {
       float l[8];
-      unpack<f16>(*reinterpret_cast<const u32x4*>(lo + r * ld + c), l);
+      unpack<f16>(*reinterpret_cast<const u32x4*>(lo + at + r * 64ll), l);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] += l[i];
     }
@@ -889,7 +840,15 @@ __global__ __launch_bounds__(256) void ce_colsum_kernel(int width, const uint16_
     for (int i = 0; i < 8; ++i) s[i] += g * f[i];
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[(long long)chunk * width + c + i] = s[i];
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) s[i] += __shfl_xor(s[i], o);
+    if (lane < 4) tmp[wave][lane * 8 + i] = s[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 32)
+    part[(long long)blockIdx.y * width + blockIdx.x * 32 + threadIdx.x] =
+        tmp[0][threadIdx.x] + tmp[1][threadIdx.x] + tmp[2][threadIdx.x] + tmp[3][threadIdx.x];
 }
 template <typename T>
 __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chunks, const float* __restrict__ part,
@@ -898,7 +857,7 @@ __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chu
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= rows) return;
   double s = 0.0;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < chunks; ++k) s += part[(long long)k * width + c];
   const float n = scal[kCount];
   const float g = n == 0.f ? 0.f : (folded ? scal[kGMax] : reduction == 0 ? 1.f : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale;
@@ -908,17 +867,18 @@ __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chu
 // ---- sizes and launches ------------------------------------------------------------------------------------------------------
 
 constexpr int kMT = 256, kNT = 128;
-constexpr int kChunks = 64;                              // parts of the rows of a bias gradient
 constexpr long long kPieceBytes = 512ll << 20;           // memory of one piece of p - t
+constexpr int kMostSplits = 128;
 
 inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
 inline bool ce_ok(long long n, int d, int v, int dtype) {
   return n >= 1 && n <= (1ll << 22) && d >= 1 && d <= (1 << 20) && v >= 1 && v <= (1 << 28) && dtype >= 0 && dtype <= 2 &&
          ((n + 127) / 128) * ((v + 255ll) / 256) <= (1ll << 23);      // a launch holds fewer than 2^32 threads
 }
-// rows of w that the matrix cores can be fed from as they lie: whole steps of K, sixteen-byte chunks
-inline bool direct_w(int d, int dtype, const void* w, long long ldw) {
-  return dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
+// Without a backward and for few rows, 16-bit rows of w are read as they lie: packing them costs three passes over w (81 us of
+// 65536 x 1024), which the products of panels win back from about 4000 rows on.
+inline bool direct_w(long long n, int d, int dtype, int train, const void* w, long long ldw) {
+  return !train && n <= 4096 && dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
 }
 
 struct Keep {      // what the backward needs, in the caller's `keep`
@@ -959,8 +919,8 @@ inline Forward forward_plan(const Keep& k) {
   return f;
 }
 struct Backward {
-  int pieces, dx_splits, dx_per, dw_splits, dw_per;
-  long long piece, dz, xb, wb, amax, dx_slab, dx_rows, dw_slab, dw_rows, col, ld, bytes;
+  int pieces, dx_splits, dx_per, dw_splits, dw_per, chunk, chunks;
+  long long piece, dz, xg, dx_slab, dx_rows, dw_slab, dw_rows, col, ld, bytes;
 };
 inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtype, int reduction) {
   Backward b = {};
@@ -973,7 +933,7 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtyp
   const long long dt = b.ld / kMT, seg = dtype == ISTNET_VOCAB_F32 ? 3 : planes;
   // two workgroups fit a compute unit: split K while that fills more of the 512 places, eight steps at least
   auto splits = [&](long long tiles, long long steps) {
-    return std::max<long long>(1, std::min<long long>(512 / std::max<long long>(1, tiles), steps / 8));
+    return std::max<long long>(1, std::min<long long>({512 / std::max<long long>(1, tiles), steps / 8, kMostSplits}));
   };
   const long long most_rows = std::min<long long>(v, b.piece), dx_steps = (most_rows + BK - 1) / BK * seg, dw_steps = (n + BK - 1) / BK * seg;
   b.dx_rows = round_up(n, kNT);
@@ -982,30 +942,35 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtyp
   b.dx_per = (int)((dx_steps + b.dx_splits - 1) / b.dx_splits);
   b.dw_splits = (int)splits(dt * (b.dw_rows / kNT), dw_steps);
   b.dw_per = (int)((dw_steps + b.dw_splits - 1) / b.dw_splits);
+  b.chunk = (int)std::max<long long>(256, round_up((n + 127) / 128, 64));      // rows of one part of a bias gradient: 128 parts at most
+  b.chunks = (int)((n + b.chunk - 1) / b.chunk);
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
   b.dz = take(2 * planes * k.np * b.piece);
-  b.xb = dtype == ISTNET_VOCAB_BF16 || (dtype == ISTNET_VOCAB_F32 && reduction == 0) ? take(2 * k.planes * k.np * k.kp) : 0;
-  b.wb = dtype == ISTNET_VOCAB_BF16 ? take(2 * most_rows * k.kp) : 0;
-  b.amax = take(4 * 1024);
+  b.xg = reduction == 0 && dtype != ISTNET_VOCAB_F16 ? take(2 * k.planes * k.np * k.kp) : 0;
   b.dx_slab = take(4 * b.dx_splits * b.dx_rows * b.ld);
   b.dw_slab = b.dw_splits > 1 ? take(4 * b.dw_splits * b.dw_rows * b.ld) : 0;
-  b.col = take(4ll * kChunks * b.piece);
+  b.col = take(4ll * b.chunks * b.piece);
   b.bytes = at;
   return b;
 }
 
-// element type of the logits' product, planes of the operands and of p - t, products of planes per product of the logits / gradients
+// planes of the operands and of p - t, products of planes per product of the logits / gradients, packed as they are
 template <typename T> struct Matrix;
-template <> struct Matrix<float> { typedef f16 M; static constexpr int P = 2, PD = 2, LOGIT = 3, GRAD = 3; };
-template <> struct Matrix<f16> { typedef f16 M; static constexpr int P = 1, PD = 2, LOGIT = 1, GRAD = 2; };
-template <> struct Matrix<bf16> { typedef bf16 M; static constexpr int P = 1, PD = 1, LOGIT = 1, GRAD = 1; };
+template <> struct Matrix<float> { static constexpr int P = 2, PD = 2, LOGIT = 3, GRAD = 3; static constexpr bool RAW = false; };
+template <> struct Matrix<f16> { static constexpr int P = 1, PD = 2, LOGIT = 1, GRAD = 2; static constexpr bool RAW = true; };
+template <> struct Matrix<bf16> { static constexpr int P = 1, PD = 1, LOGIT = 1, GRAD = 1; static constexpr bool RAW = false; };
+
+template <typename T, bool RAW, typename... A>
+inline void launch_pack(int wgs, hipStream_t st, A... args) {
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_pack_kernel<T, Matrix<T>::P, RAW>), dim3(wgs), dim3(256), 0, st, args...);
+}
 
 }  // namespace
 
-extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, const void* w, long long ldw) {
+extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, int train, const void* w, long long ldw) {
   if (!ce_ok(n, d, v, dtype)) return -1;
-  return (int)((keep_plan(n, d, v, dtype, direct_w(d, dtype, w, ldw)).bytes + 1023) / 1024);
+  return (int)((keep_plan(n, d, v, dtype, direct_w(n, d, dtype, train, w, ldw)).bytes + 1023) / 1024);
 }
 extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward) {
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
@@ -1013,54 +978,71 @@ extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype
   return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k).bytes) + 1023) / 1024);
 }
 
-extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w,
-                                        long long ldw, const void* bias, const void* target, long long ignore, int reduction,
-                                        float* loss, void* keep, void* ws, void* stream) {
+extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, int train, const void* x, long long ldx,
+                                        const void* w, long long ldw, const void* bias, const void* target, long long ignore,
+                                        int reduction, float* loss, void* keep, void* ws, void* stream) {
   if (!ce_ok(n, d, v, dtype) || !x || !w || !target || !loss || !keep || !ws || ldx < d || ldw < d || reduction < 0 || reduction > 2)
     return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
-  const bool direct = direct_w(d, dtype, w, ldw), split = dtype == ISTNET_VOCAB_F32;
+  const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
   const Forward f = forward_plan(k);
-  char *kb = (char*)keep, *wb = (char*)ws;
-  float* scal = (float*)(kb + k.scal);
-  int* blocks = (int*)(wb + f.blocks);
+  char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = direct ? nullptr : kb + k.wp;
+  float *scal = (float*)(kb + k.scal), *bias2 = (float*)(kb + k.bias2), *zt = (float*)(wb + f.zt);
   float *amax = (float*)(wb + f.amax), *packed_loss = (float*)(wb + f.loss), *row_loss = reduction == 0 ? loss : nullptr;
-  uint16_t *xp = (uint16_t*)(kb + k.xp), *wp = (uint16_t*)(kb + k.wp);
-  float *bias2 = (float*)(kb + k.bias2), *zt = (float*)(wb + f.zt);
   RowStat* stat = (RowStat*)(kb + k.stat);
-  int *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse), *tgt = (int*)(kb + k.tgt);
-  const int ax = split ? (int)std::min<long long>(256, (n + 3) / 4) : 0, aw = split ? (int)std::min<long long>(768, (v + 3ll) / 4) : 0;
-  if (split)
-    hipLaunchKernelGGL(ce_amax_kernel, dim3(ax + aw), dim3(256), 0, st, (int)n, v, d, (const float*)x, ldx, (const float*)w, ldw, target,
-                       idx64, ignore, ax, amax);
+  int *blocks = (int*)(wb + f.blocks), *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse), *tgt = (int*)(kb + k.tgt);
+  const int ax = (int)std::min<long long>(256, (n + 3) / 4), aw = (int)std::min<long long>(768, (v + 3ll) / 4);
+  if (scaled) {
+    if (dtype == ISTNET_VOCAB_F32)
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_amax_kernel<float>), dim3(ax + aw), dim3(256), 0, st, (int)n, v, d, (const float*)x, ldx,
+                         (const float*)w, ldw, target, idx64, ignore, ax, amax);
+    else
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_amax_kernel<bf16>), dim3(ax + aw), dim3(256), 0, st, (int)n, v, d, (const bf16*)x, ldx,
+                         (const bf16*)w, ldw, target, idx64, ignore, ax, amax);
+  }
   const int counted = n > 16384;      // up to here one workgroup counts the rows while it is at it
   if (counted)
     hipLaunchKernelGGL(ce_count_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (int)n, target, idx64, ignore, blocks);
-  hipLaunchKernelGGL(ce_plan_kernel, dim3(1), dim3(1024), 0, st, (int)n, counted, target, idx64, ignore, (int)split, ax, ax + aw, amax,
+  hipLaunchKernelGGL(ce_plan_kernel, dim3(1), dim3(1024), 0, st, (int)n, counted, target, idx64, ignore, (int)scaled, ax, ax + aw, amax,
                      blocks, scal);
   const int xwgs = (int)((n + 255) / 256 * (256 / kPackRows));
-  const int wwgs = direct ? (int)std::min<long long>(256, (k.vp + 255) / 256) : (int)std::min<long long>(2048, (v + 3ll) / 4);
+  const int wwgs = direct ? (bias ? (int)std::min<long long>(256, (k.vp + 255) / 256) : 0)
+                          : (int)std::min<long long>(4096, (v + kPackRows - 1ll) / kPackRows);
+  const int tn = (int)((n + kNT - 1) / kNT);
+  Operand A = {{wp, wp}, 64, v * 64ll, v - 1, 0}, B = {{xp, xp}, 64, k.np * 64, (int)k.np - 1, 0};
+  if (direct) A = {{(const char*)w, (const char*)w}, ldw * 2, 64, v - 1, 0};
+  if (k.planes == 2) {
+    A.plane[1] += 2ll * v * k.kp;
+    B.plane[1] += 2 * k.np * k.kp;
+  }
+  Epilogue e = {};
+  e.scal = scal;
+  e.bias2 = bias2;
+  e.biased = bias != nullptr;
+  e.target = tgt;
+  e.part = (float2*)(wb + f.part);
+  e.zt = zt;
+  e.v = v;
+  e.parts_ld = (int)k.np;
   VOCAB_DISPATCH(dtype, T, {
     typedef Matrix<T> X;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_pack_kernel<T, X::P>), dim3(xwgs + kPad / kPackRows + wwgs), dim3(256), 0, st, (int)n, v, d,
-                       (int)k.kp, (int)k.vp, (const T*)x, ldx, (const T*)w, ldw, (const T*)bias, target, idx64, ignore, xwgs, !direct,
-                       blocks, scal, xp, k.np * k.kp, wp, v * k.kp, bias2, rowmap, inverse, tgt, row_loss);
-    const uint16_t* wd = direct ? (const uint16_t*)w : wp;
-    const Operand A = {{wd, direct ? wd : wp + v * k.kp}, direct ? ldw : k.kp, v - 1, 0};
-    const Operand B = {{xp, xp + (X::P - 1) * k.np * k.kp}, k.kp, (int)k.np - 1, 0};
-    Epilogue e = {};
-    e.scal = scal;
-    e.bias2 = bias2;
-    e.biased = bias != nullptr;
-    e.target = tgt;
-    e.part = (float2*)(wb + f.part);
-    e.zt = zt;
-    e.v = v;
-    e.parts_ld = (int)k.np;
-    const int tn = (int)((n + kNT - 1) / kNT);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<typename X::M, X::LOGIT, 1, false, false, kMT, kNT, kLse, T>), dim3(f.tiles * tn),
-                       dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), 0, 1, 0, e);
+    const auto pack = [&](auto raw) {
+      launch_pack<T, decltype(raw)::value>(xwgs + kPad / kPackRows + wwgs, st, (int)n, v, d, (int)k.kp, (int)k.vp, (const T*)x, ldx,
+                                           (const T*)w, ldw, (const T*)bias, target, idx64, ignore, xwgs, (const int*)blocks,
+                                           (const float*)scal, xp, k.np, wp, bias2, rowmap, inverse, tgt, row_loss);
+    };
+    const auto product = [&](auto m) {
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<decltype(m), X::LOGIT, 1, false, false, kMT, kNT, kLse, f16>),
+                         dim3(f.tiles * tn), dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), 0, 1, 0, e);
+    };
+    if (__is_same(T, bf16) && direct) {
+      pack(std::true_type{});
+      product(bf16{});
+    } else {
+      pack(std::integral_constant<bool, X::RAW>{});
+      product(f16{});
+    }
   });
   hipLaunchKernelGGL(ce_finish_kernel, dim3((unsigned)(round_up(n, kPad) / 16)), dim3(256), 0, st, f.tiles, (int)k.np,
                      bias != nullptr, (const float2*)(wb + f.part), zt, tgt, rowmap, scal, stat, packed_loss, row_loss);
@@ -1069,62 +1051,51 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   return launch_status();
 }
 
-extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw,
-                                         int has_bias, int reduction, const float* gout, void* keep, void* ws, void* dx, void* dw,
-                                         void* db, void* stream) {
-  if (!ce_ok(n, d, v, dtype) || !x || !w || !gout || !keep || !ws || ldx < d || ldw < d || reduction < 0 || reduction > 2)
-    return ISTNET_PN2_EINVAL;
+extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void* x, long long ldx, int has_bias, int reduction,
+                                         const float* gout, void* keep, void* ws, void* dx, void* dw, void* db, void* stream) {
+  if (!ce_ok(n, d, v, dtype) || !x || !gout || !keep || !ws || ldx < d || reduction < 0 || reduction > 2) return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
-  const bool direct = direct_w(d, dtype, w, ldw);
-  const Keep k = keep_plan(n, d, v, dtype, direct);
+  const Keep k = keep_plan(n, d, v, dtype, false);
   const Backward b = backward_plan(k, n, d, v, dtype, reduction);
-  char *kb = (char*)keep, *wb = (char*)ws;
+  char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = kb + k.wp, *dz = wb + b.dz, *xb = xp;
   float* scal = (float*)(kb + k.scal);
-  uint16_t *xp = (uint16_t*)(kb + k.xp), *wp = (uint16_t*)(kb + k.wp), *dz = (uint16_t*)(wb + b.dz);
   int *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse);
   const int tn = (int)((n + kNT - 1) / kNT), dt = (int)(b.ld / kMT);
-  const bool weighted = reduction == 0, folded = weighted && dtype == ISTNET_VOCAB_F16, turned = dtype == ISTNET_VOCAB_BF16;
+  // weights of the rows' losses: taken into the rows of x that dw is formed from, which rounds them once more to 22 bits (float32) or
+  // 11 (bfloat16); for float16 that would be the result's own precision, there they are taken into p - t
+  const bool weighted = reduction == 0, folded = weighted && dtype == ISTNET_VOCAB_F16;
   if (weighted) hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, st, gout, rowmap, scal);
-  if (turned) {
-    const int ax = (int)std::min<long long>(256, (n + 3) / 4), aw = (int)std::min<long long>(768, (v + 3ll) / 4);
-    float* amax = (float*)(wb + b.amax);
-    hipLaunchKernelGGL(ce_amax_packed_kernel, dim3(ax + aw), dim3(256), 0, st, (int)k.kp, (const bf16*)xp, scal, v, d,
-                       (const bf16*)w, ldw, ax, amax);
-    hipLaunchKernelGGL(ce_scales_kernel, dim3(1), dim3(1024), 0, st, ax, ax + aw, amax, scal);
-  }
   VOCAB_DISPATCH(dtype, T, {
     typedef Matrix<T> X;
-    typedef typename X::M M;
     constexpr int P = X::P, PD = X::PD;
-    uint16_t* xb = xp;      // rows that dw is formed from
-    if (dw && (turned || (weighted && !folded))) {
-      xb = (uint16_t*)(wb + b.xb);
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_back_x_kernel<T, P>), dim3((unsigned)(round_up(n, kPad) / 4)), dim3(256), 0, st, d, (int)k.kp,
-                         (const T*)x, ldx, weighted ? gout : nullptr, rowmap, scal, xb, k.np * k.kp);
+    if (dw && weighted && !folded) {
+      xb = wb + b.xg;
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_weigh_kernel<T, P>), dim3((unsigned)(round_up(n, kPad) / kPackRows)), dim3(256), 0, st, d,
+                         (int)k.kp, (const T*)x, ldx, gout, rowmap, scal, xb, k.np);
     }
-    const uint16_t* wd = direct ? (const uint16_t*)w : wp;
-    const long long ldwd = direct ? ldw : k.kp, wplane = direct ? 0 : v * k.kp, xplane = (P - 1) * k.np * k.kp, dzp = k.np * b.piece;
+    const long long wplane = (P - 1) * 2ll * v * k.kp, xplane = (P - 1) * 2 * k.np * k.kp, dzplane = (PD - 1) * 2 * k.np * b.piece;
     for (int piece = 0; piece < b.pieces; ++piece) {
       const int v0 = (int)(piece * b.piece), width = (int)std::min(b.piece, k.vp - v0), rows = std::min(width, v - v0);
+      const char* w0 = wp + v0 * 64ll;
+      const Operand W = {{w0, w0 + wplane}, 64, v * 64ll, rows - 1, (int)k.kp / 32 - 1};
+      const Operand Xl = {{xp, xp + xplane}, 64, k.np * 64, (int)k.np - 1, (int)k.kp / 32 - 1};
+      const Operand Xw = {{xb, xb + xplane}, 64, k.np * 64, (int)k.np - 1, (int)k.kp / 32 - 1};
+      const Operand D = {{dz, dz + dzplane}, 64, k.np * 64, (int)k.np - 1, (int)b.piece / 32 - 1};
       Epilogue e = {};
       e.scal = scal;
       e.bias2 = (float*)(kb + k.bias2);
       e.biased = has_bias;
       e.target = (int*)(kb + k.tgt);
       e.stat = (const RowStat*)(kb + k.stat);
-      e.dz[0] = dz;
-      e.dz[1] = dz + dzp;
-      e.ld_dz = b.piece;
+      e.dz[0] = (uint16_t*)dz;
+      e.dz[1] = (uint16_t*)(dz + dzplane);
+      e.dz_unit = k.np * 64;
       e.rowmap = rowmap;
       e.weights = folded ? gout : nullptr;
       e.v = v;
       e.v0 = v0;
-      const uint16_t* w0 = wd + v0 * ldwd;
-      const Operand A = {{w0, w0 + (P - 1) * wplane}, ldwd, rows - 1, 0};
-      const Operand B = {{xp, xp + xplane}, k.kp, (int)k.np - 1, 0};
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<M, X::LOGIT, PD, false, false, kMT, kNT, kDz, T>), dim3(width / kMT * tn),
-                         dim3(256), 0, st, A, B, width / kMT, tn, (int)(k.kp / BK), 0, 1, 0, e);
-      const Operand D = {{dz, dz + (PD - 1) * dzp}, b.piece, (int)k.np - 1, (int)b.piece / 8 - 1};
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::LOGIT, PD, false, false, kMT, kNT, kDz, f16>), dim3(width / kMT * tn),
+                         dim3(256), 0, st, W, Xl, width / kMT, tn, (int)(k.kp / BK), 0, 1, 0, e);
       if (dx) {
         Epilogue s = {};
         s.scal = scal;
@@ -1132,15 +1103,8 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
         s.slab_stride = b.dx_rows * b.ld;
         s.ld_slab = b.ld;
         s.accumulate = piece > 0;
-        Operand Wt = {{w0, w0 + (P - 1) * wplane}, ldwd, rows - 1, (int)(direct ? d : k.kp) / 8 - 1};
-        if (turned) {
-          uint16_t* wf = (uint16_t*)(wb + b.wb);
-          hipLaunchKernelGGL(ce_back_w_kernel, dim3(std::min((rows + 3) / 4, 2048)), dim3(256), 0, st, rows, d, (int)k.kp,
-                             (const bf16*)w + v0 * ldw, ldw, scal, wf);
-          Wt = {{wf, wf}, k.kp, rows - 1, (int)k.kp / 8 - 1};
-        }
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, false, kMT, kNT, kSlab, T>), dim3(dt * tn * b.dx_splits),
-                           dim3(256), 0, st, Wt, D, dt, tn, (rows + BK - 1) / BK, b.dx_per, 1, 0, s);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, false, kMT, kNT, kSlab, f16>),
+                           dim3(dt * tn * b.dx_splits), dim3(256), 0, st, W, D, dt, tn, (rows + BK - 1) / BK, b.dx_per, 1, 0, s);
       }
       if (dw) {
         Epilogue s = {};
@@ -1154,23 +1118,22 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
         s.d = d;
         s.reduction = reduction;
         s.gout = gout;
-        const Operand Xt = {{xb, xb + xplane}, k.kp, (int)k.np - 1, (int)k.kp / 8 - 1};
         const int vt = (rows + kNT - 1) / kNT;
         if (b.dw_splits == 1) {
           hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kOut, T>), dim3(dt * vt), dim3(256), 0,
-                             st, Xt, D, dt, vt, 0, 0, 0, 1, s);
+                             st, Xw, D, dt, vt, 0, 0, 0, 1, s);
         } else {
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kSlab, T>), dim3(dt * vt * b.dw_splits),
-                             dim3(256), 0, st, Xt, D, dt, vt, 0, b.dw_per, 0, 1, s);
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dw_kernel<T>), dim3((unsigned)(((long long)rows * ((d + 3) / 4) + 255) / 256)), dim3(256),
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kSlab, f16>),
+                             dim3(dt * vt * b.dw_splits), dim3(256), 0, st, Xw, D, dt, vt, 0, b.dw_per, 0, 1, s);
+          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dw_kernel<T>), dim3((unsigned)(((long long)rows * ((d + 3) / 4) + 63) / 64)), dim3(256),
                              0, st, rows, d, b.dw_splits, s.slab, s.slab_stride, b.ld, gout, reduction, scal, dw0);
         }
       }
       if (db) {
         float* col = (float*)(wb + b.col);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_colsum_kernel<PD>), dim3((width + 511) / 512, kChunks / 4), dim3(256), 0, st, width, dz,
-                           dz + (PD - 1) * dzp, b.piece, weighted && !folded ? gout : nullptr, rowmap, scal, kChunks, col);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_db_kernel<T>), dim3((rows + 255) / 256), dim3(256), 0, st, rows, width, kChunks, col, gout,
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_colsum_kernel<PD>), dim3(width / 32, b.chunks), dim3(256), 0, st, dz, dz + dzplane,
+                           k.np * 64, width, weighted && !folded ? gout : nullptr, rowmap, scal, b.chunk, col);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_db_kernel<T>), dim3((rows + 255) / 256), dim3(256), 0, st, rows, width, b.chunks, col, gout,
                            reduction, folded, scal, (T*)db + v0);
       }
     }

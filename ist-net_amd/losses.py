@@ -120,7 +120,8 @@ def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, r
         vn.require_float(features, "features")
         vn.require(n <= 1 << 22 and d <= 1 << 20 and v <= 1 << 28 and -(-n // 128) * -(-v // 256) <= 1 << 23,
                    f"{n} rows of {d} features and {v} classes are too many for one call", ValueError)
-        loss = vn.LinearCEFunction.apply(x, weight, bias, t, ignore_index, vn.REDUCTIONS[reduction])
+        train = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+        loss = vn.LinearCEFunction.apply(x, weight, bias, t, ignore_index, vn.REDUCTIONS[reduction], train)
     else:                                            # host: the definition as it is written
         kind = torch.float64 if features.dtype == torch.float64 else torch.float32
         counted = t != ignore_index

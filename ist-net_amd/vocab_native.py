@@ -130,41 +130,42 @@ class DistillFunction(Function):
 
 
 class LinearCEFunction(Function):
-    """x (N, D), weight (V, D), bias (V) or None, target (N) -> loss (N,) or scalar, float32; gradients for x, weight, bias."""
+    """x (N, D), weight (V, D), bias (V) or None, target (N) -> loss (N,) or scalar, float32; gradients for x, weight, bias.
+    ``train``: a backward may follow."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore, reduction):
+    def forward(ctx, x, weight, bias, target, ignore, reduction, train):
         dev, (n, d), v, dtype = x.device, x.shape, weight.shape[0], DTYPES[x.dtype]
         lib = _native.lib()
         xr, ldx = _rows(x)
         w, ldw = _rows(weight)
         b, t = (None if bias is None else bias.contiguous()), target.contiguous()
         loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        keep = _scratch(lib.istnet_linear_ce_keep_kib(n, d, v, dtype, w.data_ptr(), ldw), dev)
+        keep = _scratch(lib.istnet_linear_ce_keep_kib(n, d, v, dtype, train, w.data_ptr(), ldw), dev)
         ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 0), dev)
-        _launch(dev, "linear_ce_forward", lib.istnet_linear_ce_forward, n, d, v, dtype, t.dtype == torch.int64, xr.data_ptr(), ldx,
-                w.data_ptr(), ldw, None if b is None else b.data_ptr(), t.data_ptr(), ignore, reduction, loss.data_ptr(),
+        _launch(dev, "linear_ce_forward", lib.istnet_linear_ce_forward, n, d, v, dtype, t.dtype == torch.int64, train, xr.data_ptr(),
+                ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(), t.data_ptr(), ignore, reduction, loss.data_ptr(),
                 keep.data_ptr(), ws.data_ptr())
-        ctx.save_for_backward(x, weight, keep)
-        ctx.args = (reduction, None if bias is None else bias.dtype)
+        if train:
+            ctx.save_for_backward(x, weight, keep)
+            ctx.args = (reduction, None if bias is None else bias.dtype)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        x, weight, keep = ctx.saved_tensors
+        x, weight, keep = ctx.saved_tensors      # (weight: so that a change of it in between is noticed)
         reduction, bias_type = ctx.args
         dev, (n, d), v, dtype = x.device, x.shape, weight.shape[0], DTYPES[x.dtype]
         lib = _native.lib()
         xr, ldx = _rows(x)
-        w, ldw = _rows(weight)
         gout = gout.contiguous()
         need = ctx.needs_input_grad
         dx = torch.empty((n, d), dtype=x.dtype, device=dev) if need[0] else None
         dw = torch.empty((v, d), dtype=x.dtype, device=dev) if need[1] else None
         db = torch.empty((v,), dtype=bias_type, device=dev) if need[2] else None
         ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 1), dev)
-        _launch(dev, "linear_ce_backward", lib.istnet_linear_ce_backward, n, d, v, dtype, xr.data_ptr(), ldx, w.data_ptr(), ldw,
-                bias_type is not None, reduction, gout.data_ptr(), keep.data_ptr(), ws.data_ptr(),
+        _launch(dev, "linear_ce_backward", lib.istnet_linear_ce_backward, n, d, v, dtype, xr.data_ptr(), ldx, bias_type is not None,
+                reduction, gout.data_ptr(), keep.data_ptr(), ws.data_ptr(),
                 *(None if t is None else t.data_ptr() for t in (dx, dw, db)))
-        return dx, dw, db, None, None, None
+        return dx, dw, db, None, None, None, None
