@@ -925,12 +925,21 @@ struct Backward {
 inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtype, int reduction) {
   Backward b = {};
   const long long planes = dtype == ISTNET_VOCAB_BF16 ? 1 : 2;      // of p - t
-  const long long most = std::max<long long>(kMT, kPieceBytes / (2 * planes * k.np) / kMT * kMT);
-  b.pieces = (int)((k.vp + most - 1) / most);
-  b.piece = round_up((k.vp + b.pieces - 1) / b.pieces, kMT);
-  b.pieces = (int)((k.vp + b.piece - 1) / b.piece);
   b.ld = round_up(d, kMT);
   const long long dt = b.ld / kMT, seg = dtype == ISTNET_VOCAB_F32 ? 3 : planes;
+  // As few rounds of 512 workgroups for dw over all pieces as pieces of that memory allow, and as few pieces as that takes: 65536 classes
+  // of 1024 features are four pieces of one full round each, not three of a round and a third.
+  const long long most = std::max<long long>(kMT, kPieceBytes / (2 * planes * k.np) / kMT * kMT), least = (k.vp + most - 1) / most;
+  long long best = -1;
+  for (long long p = least; p <= least + 3; ++p) {
+    const long long piece = round_up((k.vp + p - 1) / p, kMT), full = v / piece, rest = v - full * piece;
+    const long long rounds = full * ((dt * (piece / kNT) + 511) / 512) + (dt * ((rest + kNT - 1) / kNT) + 511) / 512;
+    if (best < 0 || rounds < best) {
+      best = rounds;
+      b.piece = piece;
+    }
+  }
+  b.pieces = (int)((k.vp + b.piece - 1) / b.piece);
   // two workgroups fit a compute unit: split K while that fills more of the 512 places, eight steps at least
   auto splits = [&](long long tiles, long long steps) {
     return std::max<long long>(1, std::min<long long>({512 / std::max<long long>(1, tiles), steps / 8, kMostSplits}));
