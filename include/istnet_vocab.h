@@ -63,9 +63,9 @@ ISTNET_PN2_API int istnet_linear_ce_forward(long long n, int d, int v, int dtype
                                             long long ldx, const void *w, long long ldw, const void *bias, const void *target, long long ignore,
                                             int reduction, float *loss, void *keep, void *ws, void *stream);
 /* dx (n, d), dw (v, d), db (v), contiguous, each may be NULL; gout as for istnet_distill_backward. */
-ISTNET_PN2_API int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void *x, long long ldx, int has_bias,
-                                             int reduction, const float *gout, void *keep, void *ws, void *dx, void *dw, void *db,
-                                             void *stream);
+ISTNET_PN2_API int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void *x, long long ldx, const void *w,
+                                             long long ldw, int has_bias, int reduction, const float *gout, void *keep, void *ws,
+                                             void *dx, void *dw, void *db, void *stream);
 
 #ifdef __cplusplus
 }

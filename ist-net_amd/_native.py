@@ -157,7 +157,7 @@ SIGNATURES = {
     "istnet_linear_ce_keep_kib": [_l, _i, _i, _i, _i, _p, _l],
     "istnet_linear_ce_scratch_kib": [_l, _i, _i, _i, _i, _i],
     "istnet_linear_ce_forward": [_l, _i, _i, _i, _i, _i, _p, _l, _p, _l, _p, _p, _l, _i] + [_p] * 4,
-    "istnet_linear_ce_backward": [_l, _i, _i, _i, _p, _l, _i, _i] + [_p] * 7,
+    "istnet_linear_ce_backward": [_l, _i, _i, _i, _p, _l, _p, _l, _i, _i] + [_p] * 7,
     # compact-column form of a set-abstraction scale (csrc/sa_compact.hip)
     "istnet_sa_compact": [_i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p],
     "istnet_sa_compact_pair": [_i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _i, _p],

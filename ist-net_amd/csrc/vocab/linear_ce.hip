@@ -869,6 +869,7 @@ __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chu
 constexpr int kMT = 256, kNT = 128;
 constexpr long long kPieceBytes = 512ll << 20;           // memory of one piece of p - t
 constexpr int kMostSplits = 128;
+constexpr double kSmallProducts = 1 << 26;
 
 inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
 inline bool ce_ok(long long n, int d, int v, int dtype) {
@@ -879,6 +880,11 @@ inline bool ce_ok(long long n, int d, int v, int dtype) {
 // 65536 x 1024), which the products of panels win back from about 4000 rows on.
 inline bool direct_w(long long n, int d, int dtype, int train, const void* w, long long ldw) {
   return !train && n <= 4096 && dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
+}
+
+// Problems that the four launches of linear_ce_small.hip serve: see there.
+inline bool small_ce(long long n, int d, int v) {
+  return n <= 4096 && v <= 4096 && n * v <= (1ll << 21) && (double)n * v * d <= kSmallProducts;
 }
 
 struct Keep {      // what the backward needs, in the caller's `keep`
@@ -979,10 +985,12 @@ inline void launch_pack(int wgs, hipStream_t st, A... args) {
 
 extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, int train, const void* w, long long ldw) {
   if (!ce_ok(n, d, v, dtype)) return -1;
+  if (small_ce(n, d, v)) return (int)((vocab_small_ce_keep(n, v) + 1023) / 1024);
   return (int)((keep_plan(n, d, v, dtype, direct_w(n, d, dtype, train, w, ldw)).bytes + 1023) / 1024);
 }
 extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward) {
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
+  if (small_ce(n, d, v)) return backward ? 1 : (int)((4 * n + 1023) / 1024);
   const Keep k = keep_plan(n, d, v, dtype, false);
   return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k).bytes) + 1023) / 1024);
 }
@@ -993,6 +1001,8 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   if (!ce_ok(n, d, v, dtype) || !x || !w || !target || !loss || !keep || !ws || ldx < d || ldw < d || reduction < 0 || reduction > 2)
     return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
+  if (small_ce(n, d, v))
+    return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, ws, st);
   const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
   const Forward f = forward_plan(k);
@@ -1060,10 +1070,13 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   return launch_status();
 }
 
-extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void* x, long long ldx, int has_bias, int reduction,
-                                         const float* gout, void* keep, void* ws, void* dx, void* dw, void* db, void* stream) {
-  if (!ce_ok(n, d, v, dtype) || !x || !gout || !keep || !ws || ldx < d || reduction < 0 || reduction > 2) return ISTNET_PN2_EINVAL;
+extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw,
+                                         int has_bias, int reduction, const float* gout, void* keep, void* ws, void* dx, void* dw,
+                                         void* db, void* stream) {
+  if (!ce_ok(n, d, v, dtype) || !x || !w || !gout || !keep || !ws || ldx < d || ldw < d || reduction < 0 || reduction > 2)
+    return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
+  if (small_ce(n, d, v)) return vocab_small_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, dx, dw, db, st);
   const Keep k = keep_plan(n, d, v, dtype, false);
   const Backward b = backward_plan(k, n, d, v, dtype, reduction);
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = kb + k.wp, *dz = wb + b.dz, *xb = xp;

@@ -1,0 +1,317 @@
+// Cross entropy of a linear head for small problems (the operator of linear_ce.hip, whose packing, splitting and joining are a dozen
+// launches: below some 10^8 multiplications those launches, not the products, are what a call costs).  gfx950, wave64.
+//
+// Four launches: the logits (kept: a few megabytes here), row statistics and p - t in their place, the loss, and ONE launch for dx, dw
+// and db.  Products on the float32 matrix instructions (v_mfma_f32_32x32x2_f32), operands straight from memory into registers whatever
+// their type, stride or alignment; eight waves split K and join through LDS in a fixed order.  Everything is float32, rounded once.
+#include <algorithm>
+
+#include "vocab_common.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+struct __attribute__((packed, aligned(2))) Raw8 { u32x2 v; };
+
+constexpr float kNaN = __builtin_nanf("");
+constexpr int kWaves = 8, kTM = 64, kTN = 32;      // tile of a workgroup: every wave has all of it for its part of K
+constexpr int kPitch = kTM + 4;
+
+// four elements from p, those at or behind `left` as zeros
+template <typename T> __device__ __forceinline__ f32x4 load4(const T* p, int left) {
+  f32x4 f;
+  if constexpr (sizeof(T) == 4) {
+    if (left >= 4) {
+      const u32x4 r = load16(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(r[i]);
+      return f;
+    }
+  } else {
+    if (left >= 4) {
+      const u32x2 r = reinterpret_cast<const Raw8*>(p)->v;
+      f[0] = to_f32(__builtin_bit_cast(T, (uint16_t)(r.x & 0xffffu)));
+      f[1] = to_f32(__builtin_bit_cast(T, (uint16_t)(r.x >> 16)));
+      f[2] = to_f32(__builtin_bit_cast(T, (uint16_t)(r.y & 0xffffu)));
+      f[3] = to_f32(__builtin_bit_cast(T, (uint16_t)(r.y >> 16)));
+      return f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = i < left ? to_f32(p[i]) : 0.f;
+  return f;
+}
+
+struct Tile { f32x16 c[2]; };
+__device__ __forceinline__ void multiply(Tile& t, const f32x4 (&a)[2], const f32x4& b) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) t.c[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][k], b[k], t.c[i], 0, 0, 0);
+}
+// the wave's part of K, two steps of loads in flight; `load(k0, a, b)`: the operands of K k0 .. k0 + 7, zeros behind the end
+template <typename F> __device__ __forceinline__ void walk(Tile& t, int wave, int steps, F&& load) {
+  constexpr int S = kWaves * 8;
+  f32x4 a0[2] = {}, a1[2] = {}, b0 = {}, b1 = {};
+  int k0 = wave * 8;
+  if (k0 < steps) load(k0, a0, b0);
+  while (k0 < steps) {
+    if (k0 + S < steps) load(k0 + S, a1, b1);
+    multiply(t, a0, b0);
+    k0 += S;
+    if (k0 >= steps) break;
+    if (k0 + S < steps) load(k0 + S, a0, b0);
+    multiply(t, a1, b1);
+    k0 += S;
+  }
+}
+// the waves' tiles added up in wave order: thread t gets rows 4 (t % 16) .. + 3 of column t / 16
+__device__ __forceinline__ f32x4 join(const Tile& t, float* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float* mine = lds + wave * kTN * kPitch + (lane & 31) * kPitch;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = t.c[i][g * 4 + r];
+      *reinterpret_cast<f32x4*>(mine + i * 32 + g * 8 + (lane >> 5) * 4) = x;
+    }
+  __syncthreads();
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  const float* at = lds + (threadIdx.x >> 4) * kPitch + (threadIdx.x & 15) * 4;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(at + w * kTN * kPitch);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] += x[r];
+  }
+  return s;
+}
+
+__device__ __forceinline__ bool counts(const void* target, long long i, int idx64, long long ignore) {
+  return load_index(target, i, idx64) != ignore;
+}
+
+// z (n, vp) = x w^T + bias; a lane's K of one step of 8: 4 (lane / 32) .. + 3
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves) void ce_small_logits_kernel(int n, int d, int v, int vp, const T* __restrict__ x, long long ldx,
+                                                                      const T* __restrict__ w, long long ldw, const T* __restrict__ bias,
+                                                                      const void* __restrict__ target, int idx64, long long ignore,
+                                                                      float* __restrict__ z) {
+  __shared__ __attribute__((aligned(16))) float lds[kWaves * kTN * kPitch];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tv = (v + kTM - 1) / kTM;
+  const int v0 = (int)(blockIdx.x % tv) * kTM, n0 = (int)(blockIdx.x / tv) * kTN;
+  const int row = n0 + (lane & 31);
+  const bool on = row < n && counts(target, row, idx64, ignore);      // rows that do not count are not looked at
+  const T* xr = x + (long long)(on ? row : 0) * ldx;
+  const T* wr[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) wr[i] = w + (long long)min(v0 + i * 32 + (lane & 31), v - 1) * ldw;
+  Tile t = {};
+  walk(t, wave, d, [&](int k0, f32x4(&a)[2], f32x4& b) {
+    const int k = k0 + (lane >> 5) * 4;
+    a[0] = load4(wr[0] + k, d - k);
+    a[1] = load4(wr[1] + k, d - k);
+    b = load4(xr + k, on ? d - k : 0);
+  });
+  const f32x4 s = join(t, lds);
+  const int r = n0 + (threadIdx.x >> 4), c = v0 + (threadIdx.x & 15) * 4;
+  if (r < n && c < vp) {
+    f32x4 y = s;
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] += c + i < v ? to_f32(bias[c + i]) : 0.f;
+    }
+    *reinterpret_cast<f32x4*>(z + (long long)r * vp + c) = y;
+  }
+}
+
+// one wave per row: loss, and p - t in the logits' place (zeros behind the last class and in rows that do not count)
+__global__ __launch_bounds__(256) void ce_small_rows_kernel(int n, int v, int vp, const void* __restrict__ target, int idx64,
+                                                            long long ignore, float* __restrict__ z, float* __restrict__ row_loss,
+                                                            int* __restrict__ on) {
+  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= n) return;
+  const long long t = load_index(target, i, idx64);
+  float* row = z + (long long)i * vp;
+  if (t == ignore || t < 0 || t >= v) {
+    const float fill = t == ignore ? 0.f : kNaN;
+    for (int c = lane; c < vp; c += 64) row[c] = c < v ? fill : 0.f;
+    if (lane == 0) { row_loss[i] = fill; on[i] = t != ignore; }
+    return;
+  }
+  // the other classes: largest logit and sum of exponentials, so that the loss and the target's derivative keep their relative
+  // precision where the target is almost certain
+  float m = -INFINITY;
+  for (int c = lane; c < v; c += 64) m = c == t ? m : fmaxf(m, row[c]);
+  m = wave_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int c = lane; c < v; c += 64) s += c == t ? 0.f : expf(row[c] - ref);
+  s = wave_sum(s);
+  const float zt = row[t], d = zt - m;
+  float loss, at_target, top;
+  if (m == -INFINITY) {
+    loss = s + 0.f * zt;      // zero, or NaN
+    at_target = -loss;
+    top = zt;
+  } else if (d < -60.f) {
+    loss = logf(s) - d;
+    at_target = d == -INFINITY ? -1.f : -1.f + 0.f * loss;
+    top = m;
+  } else {
+    const float rest = d > 0.f ? s * expf(-d) : s / expf(d);
+    loss = log1pf(rest);
+    at_target = -rest / (1.f + rest);
+    top = fmaxf(m, zt);
+  }
+  const float inv = 1.f / ((m == -INFINITY ? s : s * expf(m - top)) + expf(zt - top));
+  for (int c = lane; c < vp; c += 64) row[c] = c >= v ? 0.f : c == t ? at_target : inv * expf(row[c] - top);
+  if (lane == 0) { row_loss[i] = loss; on[i] = 1; }
+}
+
+__global__ __launch_bounds__(1024) void ce_small_total_kernel(int n, int reduction, const float* __restrict__ row_loss,
+                                                              const int* __restrict__ on, float* __restrict__ loss,
+                                                              float* __restrict__ count) {
+  __shared__ double tmp[2][16];
+  double sum = 0.0, rows = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    sum += row_loss[i];
+    rows += on[i];
+  }
+  sum = wave_sum(sum);
+  rows = wave_sum(rows);
+  if ((threadIdx.x & 63) == 0) { tmp[0][threadIdx.x >> 6] = sum; tmp[1][threadIdx.x >> 6] = rows; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = rows = 0.0;
+    for (int w = 0; w < 16; ++w) { sum += tmp[0][w]; rows += tmp[1][w]; }
+    if (reduction) *loss = (float)(reduction == 1 ? sum / rows : sum);
+    *count = (float)rows;
+  }
+}
+
+// Workgroups [0, dxs): tiles of dx = g dz w (K: classes); [dxs, dxs + dws): tiles of dw = (g dz)^T x (K: rows); the rest: 64 classes of
+// db each.  The tile's 64 is d, so that a thread has four consecutive elements of a row to write.
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves) void ce_small_grads_kernel(int n, int d, int v, int vp, const T* __restrict__ x, long long ldx,
+                                                                     const T* __restrict__ w, long long ldw, const float* __restrict__ dz,
+                                                                     const int* __restrict__ on, const float* __restrict__ count,
+                                                                     int reduction, const float* __restrict__ gout, int dxs, int dws,
+                                                                     T* __restrict__ dx, T* __restrict__ dw, T* __restrict__ db) {
+  __shared__ __attribute__((aligned(16))) float lds[kWaves * kTN * kPitch];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), td = (d + kTM - 1) / kTM;
+  int wg = blockIdx.x;
+  const float whole = reduction == 0 ? 1.f : reduction == 1 ? (*count == 0.f ? 0.f : gout[0] / *count) : gout[0];
+  if (wg < dxs + dws) {
+    const bool is_dx = wg < dxs;
+    wg -= is_dx ? 0 : dxs;
+    const int d0 = wg % td * kTM, c0 = wg / td * kTN;      // c0: row (dx) or class (dw)
+    const int col = c0 + (lane & 31), steps = is_dx ? v : n;
+    const T* src = is_dx ? w : x;
+    const long long ld = is_dx ? ldw : ldx;
+    int a_col[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) a_col[i] = min(d0 + i * 32 + (lane & 31), d - 1);
+    Tile t = {};
+    if (is_dx) {
+      const float* row = dz + (long long)min(col, n - 1) * vp;
+      walk(t, wave, steps, [&](int k0, f32x4(&a)[2], f32x4& b) {
+        const int k = k0 + (lane >> 5) * 4;
+        b = load4(row + k, steps - k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const T* r = src + (long long)min(k + j, steps - 1) * ld;      // behind the last class: times zero
+#pragma unroll
+          for (int i = 0; i < 2; ++i) a[i][j] = to_f32(r[a_col[i]]);
+        }
+      });
+    } else {
+      const int bc = min(col, vp - 1);
+      walk(t, wave, steps, [&](int k0, f32x4(&a)[2], f32x4& b) {
+        const int k = k0 + (lane >> 5) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i0 = min(k + j, steps - 1);
+          const bool use = k + j < steps && on[i0];      // what rows that do not count hold is not used
+          const float g = reduction == 0 ? gout[i0] : 1.f, y = dz[(long long)i0 * vp + bc];
+          const T *r = src + (long long)i0 * ld, x0 = r[a_col[0]], x1 = r[a_col[1]];
+          b[j] = use ? g * y : 0.f;
+          a[0][j] = use ? to_f32(x0) : 0.f;
+          a[1][j] = use ? to_f32(x1) : 0.f;
+        }
+      });
+    }
+    const f32x4 s = join(t, lds);
+    const int r = c0 + (threadIdx.x >> 4), c = d0 + (threadIdx.x & 15) * 4;
+    if (r < (is_dx ? n : v)) {
+      const float g = is_dx ? (reduction == 0 ? (on[r] ? gout[r] : 0.f) : on[r] ? whole : 0.f) : whole;
+      T* out = (is_dx ? dx : dw) + (long long)r * d;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < d) out[c + i] = from_f32<T>(is_dx && !on[r] ? 0.f : g * s[i]);
+    }
+  } else {
+    const int c = (wg - dxs - dws) * 64 + lane;
+    float s = 0.f;
+    if (c < v)
+#pragma unroll 4
+      for (int i = wave; i < n; i += kWaves) s += (reduction == 0 && on[i] ? gout[i] : 1.f) * dz[(long long)i * vp + c];
+    lds[threadIdx.x] = s;
+    __syncthreads();
+    if (wave == 0 && c < v) {
+      for (int k = 1; k < kWaves; ++k) s += lds[k * 64 + lane];
+      db[c] = from_f32<T>(whole * s);
+    }
+  }
+}
+
+struct SmallKeep { long long vp, z, on, count, bytes; };
+inline SmallKeep small_keep(long long n, int v) {
+  SmallKeep k;
+  k.vp = (v + 3ll) / 4 * 4;
+  k.z = 0;
+  k.on = (4 * n * k.vp + 255) / 256 * 256;
+  k.count = k.on + (4 * n + 255) / 256 * 256;
+  k.bytes = k.count + 256;
+  return k;
+}
+
+}  // namespace
+
+long long vocab_small_ce_keep(long long n, int v) { return small_keep(n, v).bytes; }
+
+int vocab_small_ce_forward(int n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w, long long ldw,
+                           const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, void* ws,
+                           hipStream_t st) {
+  const SmallKeep k = small_keep(n, v);
+  float *z = (float*)((char*)keep + k.z), *row_loss = reduction == 0 ? loss : (float*)ws;
+  int* on = (int*)((char*)keep + k.on);
+  VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_small_logits_kernel<T>),
+                                              dim3(((v + kTM - 1) / kTM) * ((n + kTN - 1) / kTN)), dim3(64 * kWaves), 0, st, n, d, v,
+                                              (int)k.vp, (const T*)x, ldx, (const T*)w, ldw, (const T*)bias, target, idx64, ignore, z));
+  hipLaunchKernelGGL(ce_small_rows_kernel, dim3((n + 3) / 4), dim3(256), 0, st, n, v, (int)k.vp, target, idx64, ignore, z, row_loss, on);
+  if (reduction != 0)
+    hipLaunchKernelGGL(ce_small_total_kernel, dim3(1), dim3(1024), 0, st, n, reduction, row_loss, on, loss,
+                       (float*)((char*)keep + k.count));
+  return launch_status();
+}
+
+int vocab_small_ce_backward(int n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw, int reduction,
+                            const float* gout, const void* keep, void* dx, void* dw, void* db, hipStream_t st) {
+  const SmallKeep k = small_keep(n, v);
+  const float* z = (const float*)((const char*)keep + k.z);
+  const int* on = (const int*)((const char*)keep + k.on);
+  const int td = (d + kTM - 1) / kTM, dxs = dx ? td * ((n + kTN - 1) / kTN) : 0, dws = dw ? td * ((v + kTN - 1) / kTN) : 0;
+  const int dbs = db ? (v + 63) / 64 : 0;
+  if (dxs + dws + dbs == 0) return 0;
+  VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_small_grads_kernel<T>), dim3(dxs + dws + dbs), dim3(64 * kWaves), 0, st,
+                                              n, d, v, (int)k.vp, (const T*)x, ldx, (const T*)w, ldw, z, on,
+                                              (const float*)((const char*)keep + k.count), reduction, gout, dxs, dws, (T*)dx, (T*)dw,
+                                              (T*)db));
+  return launch_status();
+}

@@ -154,18 +154,19 @@ class LinearCEFunction(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        x, weight, keep = ctx.saved_tensors      # (weight: so that a change of it in between is noticed)
+        x, weight, keep = ctx.saved_tensors
         reduction, bias_type = ctx.args
         dev, (n, d), v, dtype = x.device, x.shape, weight.shape[0], DTYPES[x.dtype]
         lib = _native.lib()
         xr, ldx = _rows(x)
+        w, ldw = _rows(weight)
         gout = gout.contiguous()
         need = ctx.needs_input_grad
         dx = torch.empty((n, d), dtype=x.dtype, device=dev) if need[0] else None
         dw = torch.empty((v, d), dtype=x.dtype, device=dev) if need[1] else None
         db = torch.empty((v,), dtype=bias_type, device=dev) if need[2] else None
         ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 1), dev)
-        _launch(dev, "linear_ce_backward", lib.istnet_linear_ce_backward, n, d, v, dtype, xr.data_ptr(), ldx, bias_type is not None,
-                reduction, gout.data_ptr(), keep.data_ptr(), ws.data_ptr(),
+        _launch(dev, "linear_ce_backward", lib.istnet_linear_ce_backward, n, d, v, dtype, xr.data_ptr(), ldx, w.data_ptr(), ldw,
+                bias_type is not None, reduction, gout.data_ptr(), keep.data_ptr(), ws.data_ptr(),
                 *(None if t is None else t.data_ptr() for t in (dx, dw, db)))
         return dx, dw, db, None, None, None, None

@@ -188,5 +188,5 @@ def test_linear_ce_entry_points_reject_invalid_arguments():
         n, d, v, dt, 1, 1, x, ldx, one, ldw, None, one, -100, red, one, one, one, None)
     assert forward(n=0) == forward(d=0) == forward(v=0) == forward(dt=3) == forward(x=None) == forward(ldx=7) == forward(ldw=7) == bad
     assert forward(red=3) == forward(n=(1 << 22) + 1) == forward(n=1 << 22, v=1 << 28) == bad
-    assert lib.istnet_linear_ce_backward(4, 8, 5, 0, one, 8, 0, 1, None, one, one, one, one, None, None) == bad
+    assert lib.istnet_linear_ce_backward(4, 8, 5, 0, one, 8, one, 8, 0, 1, None, one, one, one, one, None, None) == bad
     assert lib.istnet_linear_ce_keep_kib(0, 8, 5, 0, 1, one, 8) == -1 and lib.istnet_linear_ce_scratch_kib(4, 8, 5, 0, 3, 1) == -1
