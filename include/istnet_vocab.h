@@ -5,8 +5,8 @@
  * Element types: ISTNET_VOCAB_F32 / _BF16 / _F16 (`dtype`, all floating tensors of a call that are not said to be float).
  * Indices are int32 (idx64 == 0) or int64 (idx64 != 0).  Rows are contiguous (last stride 1); a leading dimension `ld*` is the
  * distance of two rows in elements.  Every function enqueues on `stream` and returns 0, a hipError_t or ISTNET_PN2_EINVAL; the
- * *_scratch_kib functions return the size of the caller's scratch memory `ws` in KiB (-1 for invalid sizes), which nothing has to
- * clear and which may be reused as soon as the call's work on `stream` is done.  Sums are float or double, in an order that the
+ * *_scratch_kib functions return the size of the caller's scratch memory `ws` in KiB (-1 for invalid sizes; 0: ws may be NULL), which nothing
+ * has to clear and which may be reused as soon as the call's work on `stream` is done.  Sums are float or double, in an order that the
  * sizes alone decide: the same inputs give the same bits.
  */
 #ifndef ISTNET_VOCAB_H_

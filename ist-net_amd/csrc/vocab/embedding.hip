@@ -368,10 +368,9 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(int n, int v, int d, 
       if (col < d) sum_run(grad, ldg, perm, a, b, col, d - col, acc);
       join_teams<T>(acc, lds, lanes_log, teams);
       if (team == 0 && col < d) {
-        float* o = part + ((long long)blockIdx.x * 2 + slot) * d + col;
+        float* o = part + ((long long)blockIdx.x * 2 + slot) * ((d + 7) / 8 * 8) + col;
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i)
-          if (col + i < d) o[i] = acc[i];
+        for (int i = 0; i < kVec<T>; ++i) o[i] = acc[i];
       }
     }
   }
@@ -397,9 +396,9 @@ __global__ __launch_bounds__(256) void embed_join_kernel(int n, int v, int d, in
     if (col < d) {
 #pragma unroll 8
       for (int q = a; q < b; ++q) {
-        const float* o = part + ((long long)q * 2 + (s > q * longest ? 1 : 0)) * d + col;
+        const float* o = part + ((long long)q * 2 + (s > q * longest ? 1 : 0)) * ((d + 7) / 8 * 8) + col;
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) acc[i] += col + i < d ? o[i] : 0.f;
+        for (int i = 0; i < kVec<T>; ++i) acc[i] += o[i];
       }
     }
     join_teams<T>(acc, lds, lanes_log, teams);
@@ -407,6 +406,87 @@ __global__ __launch_bounds__(256) void embed_join_kernel(int n, int v, int d, in
 #pragma unroll
       for (int i = 0; i < kVec<T>; ++i) acc[i] *= scale;
       store_part(dw + (long long)k * d + col, d - col, acc);
+    }
+  }
+}
+
+// Few tokens: one launch.  A workgroup owns `rows` (<= 64) consecutive table rows, picks their tokens out of all n in order, sorts them
+// by row in LDS and adds them up; a run longer than kShortRun is shared by its teams.  (77 x 99 into 1000 rows: 5 launches of 2 to 5 us
+// each became one of 6 us, and what they cost the host is gone.)
+constexpr int kFewTokens = 2048, kFewRows = 64, kShortRun = 32;
+template <typename T>
+__global__ __launch_bounds__(256) void embed_few_kernel(int n, int v, int d, int rows, int lanes_log, const T* __restrict__ grad,
+                                                        long long ldg, const void* __restrict__ ids, int idx64, long long padding,
+                                                        float scale, T* __restrict__ dw) {
+  __shared__ float lds[256 * kVec<T>];
+  __shared__ uint32_t list[kFewTokens], sorted[kFewTokens];
+  __shared__ int start[kFewRows + 1], cnt[kFewRows], waves[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long long row0 = (long long)blockIdx.x * rows;
+  int m = 0;
+  for (int base = 0; base < n; base += 256) {
+    const int i = base + tid;
+    const uint32_t key = i < n ? key_of(ids, i, idx64, v, padding) : (uint32_t)v;
+    const bool mine = key < (uint32_t)v && key >= (uint32_t)row0 && key < (uint32_t)(row0 + rows);
+    const uint64_t has = __ballot(mine);
+    if (lane == 0) waves[wave] = __popcll(has);
+    __syncthreads();
+    int at = m + lanes_below(has);
+    for (int w = 0; w < 4; ++w) {
+      at += w < wave ? waves[w] : 0;
+      m += waves[w];
+    }
+    if (mine) list[at] = (uint32_t)(key - (uint32_t)row0) << 16 | (uint32_t)i;
+    __syncthreads();
+  }
+  if (tid < kFewRows) cnt[tid] = 0;
+  __syncthreads();
+  for (int j = tid; j < m; j += 256) atomicAdd(&cnt[list[j] >> 16], 1);
+  __syncthreads();
+  if (wave == 0) {
+    int s = cnt[lane];
+    const int own = s;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(s, o);
+      if (lane >= o) s += y;
+    }
+    start[lane] = s - own;
+    if (lane == 63) start[64] = s;
+    cnt[lane] = s - own;      // from here on: where the row's next token goes
+    for (int j = 0; j < m; j += 64) {
+      const bool active = j + lane < m;
+      const uint32_t e = active ? list[j + lane] : 0u;
+      const int to = rank_and_count(e >> 16, 6, active, cnt, lane);
+      if (active) sorted[to] = e & 0xffffu;
+    }
+  }
+  __syncthreads();
+  const int lanes = 1 << lanes_log, teams = 256 >> lanes_log, at = tid & (lanes - 1), team = tid >> lanes_log;
+  const int last = (int)(v - row0 < rows ? v - row0 : rows);
+  for (int c0 = 0; c0 < d; c0 += lanes * kVec<T>) {
+    const int col = c0 + at * kVec<T>;
+    for (int r = 0; r < last; ++r) {      // long runs: every team a part
+      const int a0 = start[r], a1 = start[r + 1];
+      if (a1 - a0 <= kShortRun) continue;
+      const int per = (a1 - a0 + teams - 1) / teams, a = min(a1, a0 + team * per), b = min(a1, a + per);
+      float acc[kVec<T>] = {};
+      if (col < d) sum_run(grad, ldg, sorted, a, b, col, d - col, acc);
+      join_teams<T>(acc, lds, lanes_log, teams);
+      if (team == 0 && col < d) {
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) acc[i] *= scale;
+        store_part(dw + (row0 + r) * d + col, d - col, acc);
+      }
+    }
+    for (int r = team; r < last && col < d; r += teams) {
+      const int a0 = start[r], a1 = start[r + 1];
+      if (a1 - a0 > kShortRun) continue;
+      float acc[kVec<T>] = {};
+      sum_run(grad, ldg, sorted, a0, a1, col, d - col, acc);
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) acc[i] *= scale;
+      store_part(dw + (row0 + r) * d + col, d - col, acc);
     }
   }
 }
@@ -482,7 +562,7 @@ inline EmbedPlan embed_plan(long long n, int v, int d) {
   for (int i = 0; i < (small ? 1 : 2); ++i) { p.keys[i] = take(4 * n); p.perm[i] = take(4 * n); }
   p.hist = small ? 0 : take(4ll * p.nb << p.bits);
   p.start = take(4ll * (v + 1ll));
-  p.part = p.pieces ? take(8ll * p.pieces * d) : 0;
+  p.part = p.pieces ? take(8ll * p.pieces * ((d + 7) / 8 * 8)) : 0;
   p.bytes = at;
   return p;
 }
@@ -501,13 +581,22 @@ extern "C" int istnet_embed_forward(long long n, int v, int d, int dtype, int id
 
 extern "C" int istnet_embed_scratch_kib(long long n, int v, int d) {
   if (!embed_ok(n, v, d, 0)) return -1;
+  if (n <= kFewTokens) return 0;
   return (int)((embed_plan(n, v, d).bytes + 1023) / 1024);
 }
 
 extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int idx64, const void* grad, long long ldg,
                                      const void* ids, long long padding, float scale, void* ws, void* dw, void* stream) {
-  if (!embed_ok(n, v, d, dtype) || !grad || !ids || !ws || !dw || ldg < d) return ISTNET_PN2_EINVAL;
+  if (!embed_ok(n, v, d, dtype) || !grad || !ids || (!ws && n > kFewTokens) || !dw || ldg < d) return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
+  const int ll = lanes_log_of(d, dtype);
+  if (n <= kFewTokens) {
+    // rows per workgroup: enough workgroups for the chip, few enough that reading all indices in each of them stays cheap
+    const int rows = v <= 4096 ? 16 : kFewRows;
+    VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_few_kernel<T>), dim3((unsigned)((v + rows - 1ll) / rows)), dim3(256),
+                                                0, st, (int)n, v, d, rows, ll, (const T*)grad, ldg, ids, idx64, padding, scale, (T*)dw));
+    return launch_status();
+  }
   const EmbedPlan p = embed_plan(n, v, d);
   char* base = (char*)ws;
   uint32_t *keys[2], *perm[2];
@@ -534,7 +623,6 @@ extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int i
     }
   }
   hipLaunchKernelGGL(embed_starts_kernel, dim3((unsigned)(v / 256 + 1)), dim3(256), 0, st, (int)n, v, keys[last], start);
-  const int ll = lanes_log_of(d, dtype);
   const long long rows = (256 >> ll) * (long long)kTeamRows, grid = std::min((v + rows - 1) / rows, kMaxGrid);
   VOCAB_DISPATCH(dtype, T, {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, v, d, ll, p.longest,

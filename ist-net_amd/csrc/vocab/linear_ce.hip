@@ -990,7 +990,7 @@ extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, i
 }
 extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward) {
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
-  if (small_ce(n, d, v)) return backward ? 1 : (int)((4 * n + 1023) / 1024);
+  if (small_ce(n, d, v)) return 0;
   const Keep k = keep_plan(n, d, v, dtype, false);
   return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k).bytes) + 1023) / 1024);
 }
@@ -998,11 +998,11 @@ extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype
 extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, int train, const void* x, long long ldx,
                                         const void* w, long long ldw, const void* bias, const void* target, long long ignore,
                                         int reduction, float* loss, void* keep, void* ws, void* stream) {
-  if (!ce_ok(n, d, v, dtype) || !x || !w || !target || !loss || !keep || !ws || ldx < d || ldw < d || reduction < 0 || reduction > 2)
+  if (!ce_ok(n, d, v, dtype) || !x || !w || !target || !loss || !keep || (!ws && !small_ce(n, d, v)) || ldx < d || ldw < d || reduction < 0 || reduction > 2)
     return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
   if (small_ce(n, d, v))
-    return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, ws, st);
+    return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, st);
   const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
   const Forward f = forward_plan(k);
@@ -1073,7 +1073,7 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
 extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw,
                                          int has_bias, int reduction, const float* gout, void* keep, void* ws, void* dx, void* dw,
                                          void* db, void* stream) {
-  if (!ce_ok(n, d, v, dtype) || !x || !w || !gout || !keep || !ws || ldx < d || ldw < d || reduction < 0 || reduction > 2)
+  if (!ce_ok(n, d, v, dtype) || !x || !w || !gout || !keep || (!ws && !small_ce(n, d, v)) || ldx < d || ldw < d || reduction < 0 || reduction > 2)
     return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
   if (small_ce(n, d, v)) return vocab_small_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, dx, dw, db, st);

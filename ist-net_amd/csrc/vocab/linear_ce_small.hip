@@ -270,13 +270,14 @@ __global__ __launch_bounds__(64 * kWaves) void ce_small_grads_kernel(int n, int 
   }
 }
 
-struct SmallKeep { long long vp, z, on, count, bytes; };
+struct SmallKeep { long long vp, z, on, loss, count, bytes; };
 inline SmallKeep small_keep(long long n, int v) {
   SmallKeep k;
   k.vp = (v + 3ll) / 4 * 4;
   k.z = 0;
   k.on = (4 * n * k.vp + 255) / 256 * 256;
-  k.count = k.on + (4 * n + 255) / 256 * 256;
+  k.loss = k.on + (4 * n + 255) / 256 * 256;
+  k.count = k.loss + (4 * n + 255) / 256 * 256;
   k.bytes = k.count + 256;
   return k;
 }
@@ -286,10 +287,9 @@ inline SmallKeep small_keep(long long n, int v) {
 long long vocab_small_ce_keep(long long n, int v) { return small_keep(n, v).bytes; }
 
 int vocab_small_ce_forward(int n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w, long long ldw,
-                           const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, void* ws,
-                           hipStream_t st) {
+                           const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, hipStream_t st) {
   const SmallKeep k = small_keep(n, v);
-  float *z = (float*)((char*)keep + k.z), *row_loss = reduction == 0 ? loss : (float*)ws;
+  float *z = (float*)((char*)keep + k.z), *row_loss = reduction == 0 ? loss : (float*)((char*)keep + k.loss);
   int* on = (int*)((char*)keep + k.on);
   VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_small_logits_kernel<T>),
                                               dim3(((v + kTM - 1) / kTM) * ((n + kTN - 1) / kTN)), dim3(64 * kWaves), 0, st, n, d, v,

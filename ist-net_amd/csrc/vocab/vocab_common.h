@@ -11,8 +11,7 @@
 // The cross entropy of small problems (linear_ce_small.hip), called by the entry points of linear_ce.hip.
 long long vocab_small_ce_keep(long long n, int v);
 int vocab_small_ce_forward(int n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w, long long ldw,
-                           const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, void* ws,
-                           hipStream_t st);
+                           const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, hipStream_t st);
 int vocab_small_ce_backward(int n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw, int reduction,
                             const float* gout, const void* keep, void* dx, void* dw, void* db, hipStream_t st);
 

@@ -53,25 +53,30 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
     logits is NaN, loss and gradient.  Differentiable w.r.t. ``logits`` (once).  ``logits`` may be a slice with a row stride, of
     float32, bfloat16 or float16; the gradient has its type, everything between is float32."""
     from . import vocab_native as vn
-    vn.require(reduction in vn.REDUCTIONS, f"reduction must be one of {sorted(vn.REDUCTIONS)}, got {reduction!r}", ValueError)
+    vn.check_reduction(reduction)
     temperature = float(temperature)
-    vn.require(0.0 < temperature < float("inf"), f"temperature must be positive and finite, got {temperature}", ValueError)
-    vn.require(logits.dim() >= 1 and top_index.dim() >= 1 and logits.shape[:-1] == top_index.shape[:-1]
-               and top_logits.shape == top_index.shape,
-               f"shapes do not agree: logits {tuple(logits.shape)}, top_logits {tuple(top_logits.shape)}, "
-               f"top_index {tuple(top_index.shape)}", ValueError)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if (logits.dim() < 1 or top_index.dim() < 1 or logits.shape[:-1] != top_index.shape[:-1]
+            or top_logits.shape != top_index.shape):
+        raise ValueError(f"shapes do not agree: logits {tuple(logits.shape)}, top_logits {tuple(top_logits.shape)}, "
+                         f"top_index {tuple(top_index.shape)}")
     v, k = logits.shape[-1], top_index.shape[-1]
-    vn.require(v >= 1 and 1 <= k <= 256, f"needs at least one class and 1 to 256 kept logits, got {v} and {k}", ValueError)
-    vn.require_index(top_index, "top_index")
-    vn.require(not top_logits.requires_grad, "top_logits must not require a gradient: the teacher is fixed", ValueError)
-    vn.require_device(logits, "logits", top_logits=top_logits, top_index=top_index)
+    if v < 1 or not 1 <= k <= 256:
+        raise ValueError(f"needs at least one class and 1 to 256 kept logits, got {v} and {k}")
+    vn.check_index(top_index, "top_index")
+    if top_logits.requires_grad:
+        raise ValueError("top_logits must not require a gradient: the teacher is fixed")
+    vn.check_device(logits, "logits", top_logits, "top_logits")
+    vn.check_device(logits, "logits", top_index, "top_index")
     lead = logits.shape[:-1]
     z, top, idx = logits.reshape(-1, v), top_logits.reshape(-1, k), top_index.reshape(-1, k)
     n = z.shape[0]
     if logits.is_cuda and n:
-        vn.require_float(logits, "logits")
-        vn.require_float(top_logits, "top_logits")
-        vn.require(n <= 1 << 23 and v < 2 ** 31 - 65536, "more than 2^23 rows or too many classes", ValueError)
+        vn.check_float(logits, "logits")
+        vn.check_float(top_logits, "top_logits")
+        if n > 1 << 23 or v >= 2 ** 31 - 65536:
+            raise ValueError(f"{n} rows of {v} classes are too many for one call")
         loss = vn.DistillFunction.apply(z, top, idx, temperature, vn.REDUCTIONS[reduction])
     else:                                            # host: the definition as it is written
         z = z if z.dtype == torch.float64 else z.float()
@@ -102,24 +107,28 @@ def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, r
     operands: both are held as two float16 numbers to a common power of two, 22 bits, with an absolute error of 2^-39 of the
     largest entry below that).  The backward forms the logits a second time instead of keeping them."""
     from . import vocab_native as vn
-    vn.require(reduction in vn.REDUCTIONS, f"reduction must be one of {sorted(vn.REDUCTIONS)}, got {reduction!r}", ValueError)
-    vn.require(features.dim() >= 1 and weight.dim() == 2 and features.shape[-1] == weight.shape[1]
-               and target.shape == features.shape[:-1] and (bias is None or bias.shape == weight.shape[:1]),
-               f"shapes do not agree: features {tuple(features.shape)}, weight {tuple(weight.shape)}, target {tuple(target.shape)}"
-               + ("" if bias is None else f", bias {tuple(bias.shape)}"), ValueError)
+    vn.check_reduction(reduction)
+    if (features.dim() < 1 or weight.dim() != 2 or features.shape[-1] != weight.shape[1] or target.shape != features.shape[:-1]
+            or (bias is not None and bias.shape != weight.shape[:1])):
+        raise ValueError(f"shapes do not agree: features {tuple(features.shape)}, weight {tuple(weight.shape)}, target "
+                         f"{tuple(target.shape)}, bias {None if bias is None else tuple(bias.shape)}")
     v, d = weight.shape
-    vn.require(v >= 1 and d >= 1, f"weight must not be empty, got {(v, d)}", ValueError)
-    vn.require_index(target, "target")
-    vn.require(weight.dtype == features.dtype and (bias is None or bias.dtype == features.dtype),
-               f"features ({features.dtype}), weight ({weight.dtype}) and bias must have one type", TypeError)
-    vn.require_device(features, "features", weight=weight, target=target, **({} if bias is None else {"bias": bias}))
+    if v < 1 or d < 1:
+        raise ValueError(f"weight must not be empty, got {(v, d)}")
+    vn.check_index(target, "target")
+    if weight.dtype != features.dtype or (bias is not None and bias.dtype != features.dtype):
+        raise TypeError(f"features ({features.dtype}), weight ({weight.dtype}) and bias must have one type")
+    vn.check_device(features, "features", weight, "weight")
+    vn.check_device(features, "features", target, "target")
+    if bias is not None:
+        vn.check_device(features, "features", bias, "bias")
     ignore_index = int(ignore_index)
     x, t = features.reshape(-1, d), target.reshape(-1)
     n = x.shape[0]
     if features.is_cuda and n:
-        vn.require_float(features, "features")
-        vn.require(n <= 1 << 22 and d <= 1 << 20 and v <= 1 << 28 and -(-n // 128) * -(-v // 256) <= 1 << 23,
-                   f"{n} rows of {d} features and {v} classes are too many for one call", ValueError)
+        vn.check_float(features, "features")
+        if n > 1 << 22 or d > 1 << 20 or v > 1 << 28 or -(-n // 128) * -(-v // 256) > 1 << 23:
+            raise ValueError(f"{n} rows of {d} features and {v} classes are too many for one call")
         train = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
         loss = vn.LinearCEFunction.apply(x, weight, bias, t, ignore_index, vn.REDUCTIONS[reduction], train)
     else:                                            # host: the definition as it is written

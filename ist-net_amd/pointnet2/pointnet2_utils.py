@@ -142,16 +142,17 @@ def embedding_operation(weight, idx, scale=1.0, padding_idx=None):
     ``idx`` may repeat, be empty and have any shape; ``weight`` may be a slice with a row stride.  CUDA only."""
     if not weight.is_cuda:
         raise RuntimeError("CPU not supported")
-    vocab_native.require(weight.dim() == 2 and weight.shape[0] >= 1 and weight.shape[1] >= 1,
-                         f"weight must be a non-empty (V, D) tensor, got {tuple(weight.shape)}", ValueError)
-    vocab_native.require_float(weight, "weight")
-    vocab_native.require_index(idx, "idx")
-    vocab_native.require(idx.is_cuda, "idx must be a CUDA tensor")
-    vocab_native.require_device(weight, "weight", idx=idx)
-    vocab_native.require(idx.numel() <= 1 << 30, "idx holds more than 2^30 indices", ValueError)
-    vocab_native.require(weight.shape[0] < 2 ** 31 - 257 and weight.shape[1] < 2 ** 31 - 2048, "weight is too large", ValueError)
-    if padding_idx is not None:
-        vocab_native.require(0 <= padding_idx < weight.shape[0], f"padding_idx must be a row of weight, got {padding_idx}", ValueError)
+    if weight.dim() != 2 or not 1 <= weight.shape[0] < 2 ** 31 - 257 or not 1 <= weight.shape[1] < 2 ** 31 - 2048:
+        raise ValueError(f"weight must be a non-empty (V, D) tensor, got {tuple(weight.shape)}")
+    vocab_native.check_float(weight, "weight")
+    vocab_native.check_index(idx, "idx")
+    if not idx.is_cuda:
+        raise RuntimeError("idx must be a CUDA tensor")
+    vocab_native.check_device(weight, "weight", idx, "idx")
+    if idx.numel() > 1 << 30:
+        raise ValueError("idx holds more than 2^30 indices")
+    if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx must be a row of weight, got {padding_idx}")
     return vocab_native.EmbeddingFunction.apply(weight, idx, float(scale), padding_idx)
 
 

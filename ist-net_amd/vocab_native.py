@@ -14,50 +14,70 @@ from torch.autograd.function import once_differentiable
 from . import _native
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+INDEX = {torch.int32: 0, torch.int64: 1}
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
-
-def require(cond, msg, kind=RuntimeError):
-    if not cond:
-        raise kind(msg)
+# The host's work is what a small call costs, so that checks build their messages only when they fail, tensors are taken from the
+# allocator at once, and the device and stream are asked for without the wrappers of torch.cuda.
 
 
-def require_float(t, name):
-    require(t.dtype in DTYPES, f"{name} must be a float32, bfloat16 or float16 tensor, got {t.dtype}", TypeError)
+def _once(fn):
+    """once_differentiable at no cost where no graph of the backward is asked for."""
+    graph = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return graph(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return staticmethod(backward)
 
 
-def require_index(t, name):
-    require(t.dtype in (torch.int32, torch.int64), f"{name} must be an int32 or int64 tensor, got {t.dtype}", TypeError)
+def check_float(t, name):
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name} must be a float32, bfloat16 or float16 tensor, got {t.dtype}")
 
 
-def require_device(lead, name, **others):
-    for other, t in others.items():
-        require(t.device == lead.device, f"{other} must be on the same device as {name}")
+def check_index(t, name):
+    if t.dtype not in INDEX:
+        raise TypeError(f"{name} must be an int32 or int64 tensor, got {t.dtype}")
+
+
+def check_device(lead, name, t, other):
+    if t.device != lead.device:
+        raise RuntimeError(f"{other} must be on the same device as {name}")
+
+
+def check_reduction(reduction):
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
 
 
 def _launch(dev, what, fn, *args):
     """fn(*args, current stream of dev) with dev as the current device, which it nearly always is already."""
-    if torch.cuda.current_device() == dev.index:
-        _native.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+    if torch._C._cuda_getDevice() == dev.index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
     else:
         with torch.cuda.device(dev):
-            _native.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if status:
+        _native.check(status, what)
 
 
 def _rows(t):
     """(tensor, leading dimension) of a 2-D operand with contiguous rows that do not overlap; anything else is copied."""
-    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
-        return t, t.stride(0)
-    if t.shape[1] == 1 and t.stride(0) >= 1:
-        return t, t.stride(0)
-    if t.shape[0] == 1 and t.stride(1) == 1:
+    if t.is_contiguous():
         return t, t.shape[1]
-    t = t.contiguous()
-    return t, t.shape[1]
+    n, d = t.shape
+    ld, step = t.stride()
+    if (step == 1 and ld >= d) or (d == 1 and ld >= 1):
+        return t, ld
+    return t.contiguous(), d
 
 
 def _scratch(kib, dev):
-    return torch.empty(max(kib, 1) * 1024, dtype=torch.uint8, device=dev)
+    """The tensor (to be kept until the call that uses it was made) and its address."""
+    if kib == 0:
+        return None, None
+    t = torch.empty(kib * 1024, dtype=torch.uint8, device=dev)
+    return t, t.data_ptr()
 
 
 class EmbeddingFunction(Function):
@@ -66,30 +86,29 @@ class EmbeddingFunction(Function):
     @staticmethod
     def forward(ctx, weight, idx, scale, padding):
         dev, (v, d), n = weight.device, weight.shape, idx.numel()
-        out = torch.empty((*idx.shape, d), dtype=weight.dtype, device=dev)
-        ids = idx.contiguous()
+        out = weight.new_empty((*idx.shape, d))
+        ids = idx if idx.is_contiguous() else idx.contiguous()
         if n:
             w, ldw = _rows(weight)
             _launch(dev, "embed_forward", _native.lib().istnet_embed_forward, n, v, d, DTYPES[weight.dtype],
-                    ids.dtype == torch.int64, w.data_ptr(), ldw, ids.data_ptr(), scale, out.data_ptr())
+                    INDEX[ids.dtype], w.data_ptr(), ldw, ids.data_ptr(), scale, out.data_ptr())
         ctx.save_for_backward(ids)
         ctx.args = (v, d, scale, padding, weight.dtype)
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out):
         (ids,) = ctx.saved_tensors
         v, d, scale, padding, dtype = ctx.args
         dev, n = ids.device, ids.numel()
         if n == 0:
             return torch.zeros((v, d), dtype=dtype, device=dev), None, None, None
-        g, ldg = _rows(grad_out.reshape(n, d))
-        dw = torch.empty((v, d), dtype=dtype, device=dev)
+        g, ldg = _rows(grad_out if grad_out.dim() == 2 else grad_out.reshape(n, d))
+        dw = g.new_empty((v, d))
         lib = _native.lib()
-        ws = _scratch(lib.istnet_embed_scratch_kib(n, v, d), dev)
-        _launch(dev, "embed_backward", lib.istnet_embed_backward, n, v, d, DTYPES[dtype], ids.dtype == torch.int64, g.data_ptr(),
-                ldg, ids.data_ptr(), -1 if padding is None else padding, scale, ws.data_ptr(), dw.data_ptr())
+        ws, at = _scratch(lib.istnet_embed_scratch_kib(n, v, d), dev)
+        _launch(dev, "embed_backward", lib.istnet_embed_backward, n, v, d, DTYPES[dtype], INDEX[ids.dtype], g.data_ptr(),
+                ldg, ids.data_ptr(), -1 if padding is None else padding, scale, at, dw.data_ptr())
         return dw, None, None, None
 
 
@@ -104,17 +123,16 @@ class DistillFunction(Function):
         top, ids = top.contiguous(), idx.contiguous()
         loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=dev)
         keep = torch.empty(n * (2 + k) + 1, dtype=torch.float32, device=dev)      # stats (n, 2), q (n, k), count
-        ws = _scratch(lib.istnet_distill_scratch_kib(n, v, k), dev)
+        ws, at_ws = _scratch(lib.istnet_distill_scratch_kib(n, v, k), dev)
         at = keep.data_ptr()
         _launch(dev, "distill_forward", lib.istnet_distill_forward, n, v, k, DTYPES[z.dtype], DTYPES[top.dtype],
-                ids.dtype == torch.int64, z.data_ptr(), ldz, top.data_ptr(), ids.data_ptr(), temperature, reduction,
-                loss.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), ws.data_ptr())
+                INDEX[ids.dtype], z.data_ptr(), ldz, top.data_ptr(), ids.data_ptr(), temperature, reduction,
+                loss.data_ptr(), at, at + 8 * n, at + 4 * n * (2 + k), at_ws)
         ctx.save_for_backward(logits, ids, keep)
         ctx.args = (temperature, reduction)
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gout):
         logits, ids, keep = ctx.saved_tensors
         temperature, reduction = ctx.args
@@ -124,7 +142,7 @@ class DistillFunction(Function):
         dz = torch.empty((n, v), dtype=logits.dtype, device=dev)
         at = keep.data_ptr()
         _launch(dev, "distill_backward", _native.lib().istnet_distill_backward, n, v, k, DTYPES[z.dtype],
-                ids.dtype == torch.int64, z.data_ptr(), ldz, ids.data_ptr(), temperature, reduction, gout.data_ptr(), at,
+                INDEX[ids.dtype], z.data_ptr(), ldz, ids.data_ptr(), temperature, reduction, gout.data_ptr(), at,
                 at + 8 * n, at + 4 * n * (2 + k), dz.data_ptr())
         return dz, None, None, None, None
 
@@ -139,34 +157,33 @@ class LinearCEFunction(Function):
         lib = _native.lib()
         xr, ldx = _rows(x)
         w, ldw = _rows(weight)
-        b, t = (None if bias is None else bias.contiguous()), target.contiguous()
+        b, t = (None if bias is None else bias.contiguous()), target if target.is_contiguous() else target.contiguous()
         loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        keep = _scratch(lib.istnet_linear_ce_keep_kib(n, d, v, dtype, train, w.data_ptr(), ldw), dev)
-        ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 0), dev)
-        _launch(dev, "linear_ce_forward", lib.istnet_linear_ce_forward, n, d, v, dtype, t.dtype == torch.int64, train, xr.data_ptr(),
+        keep, at = _scratch(lib.istnet_linear_ce_keep_kib(n, d, v, dtype, train, w.data_ptr(), ldw), dev)
+        ws, at_ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 0), dev)
+        _launch(dev, "linear_ce_forward", lib.istnet_linear_ce_forward, n, d, v, dtype, INDEX[t.dtype], train, xr.data_ptr(),
                 ldx, w.data_ptr(), ldw, None if b is None else b.data_ptr(), t.data_ptr(), ignore, reduction, loss.data_ptr(),
-                keep.data_ptr(), ws.data_ptr())
+                at, at_ws)
         if train:
             ctx.save_for_backward(x, weight, keep)
-            ctx.args = (reduction, None if bias is None else bias.dtype)
+            ctx.args = (reduction, bias is not None)
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gout):
         x, weight, keep = ctx.saved_tensors
-        reduction, bias_type = ctx.args
+        reduction, biased = ctx.args
         dev, (n, d), v, dtype = x.device, x.shape, weight.shape[0], DTYPES[x.dtype]
         lib = _native.lib()
         xr, ldx = _rows(x)
         w, ldw = _rows(weight)
-        gout = gout.contiguous()
+        gout = gout if gout.is_contiguous() else gout.contiguous()
         need = ctx.needs_input_grad
-        dx = torch.empty((n, d), dtype=x.dtype, device=dev) if need[0] else None
-        dw = torch.empty((v, d), dtype=x.dtype, device=dev) if need[1] else None
-        db = torch.empty((v,), dtype=bias_type, device=dev) if need[2] else None
-        ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 1), dev)
+        dx = x.new_empty((n, d)) if need[0] else None
+        dw = x.new_empty((v, d)) if need[1] else None
+        db = x.new_empty((v,)) if need[2] else None
+        ws, at_ws = _scratch(lib.istnet_linear_ce_scratch_kib(n, d, v, dtype, reduction, 1), dev)
         _launch(dev, "linear_ce_backward", lib.istnet_linear_ce_backward, n, d, v, dtype, xr.data_ptr(), ldx, w.data_ptr(), ldw,
-                bias_type is not None, reduction, gout.data_ptr(), keep.data_ptr(), ws.data_ptr(),
-                *(None if t is None else t.data_ptr() for t in (dx, dw, db)))
+                biased, reduction, gout.data_ptr(), keep.data_ptr(), at_ws, None if dx is None else dx.data_ptr(),
+                None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr())
         return dx, dw, db, None, None, None, None

@@ -109,9 +109,9 @@ def test_entry_points_reject_invalid_arguments():
     assert lib.istnet_embed_forward(4, 4, 4, 3, 0, one, 4, one, 1.0, one, None) == bad
     assert lib.istnet_embed_forward(4, 4, 4, 0, 0, one, 3, one, 1.0, one, None) == bad
     assert lib.istnet_embed_forward(4, 4, 4, 0, 0, None, 4, one, 1.0, one, None) == bad
-    assert lib.istnet_embed_backward(4, 4, 4, 0, 0, one, 4, one, -1, 1.0, None, one, None) == bad
+    assert lib.istnet_embed_backward(40000, 4, 4, 0, 0, one, 4, one, -1, 1.0, None, one, None) == bad
     assert lib.istnet_embed_backward((1 << 30) + 1, 4, 4, 0, 0, one, 4, one, -1, 1.0, one, one, None) == bad
-    assert lib.istnet_embed_scratch_kib(0, 4, 4) == -1 and lib.istnet_embed_scratch_kib(1, 1, 1) >= 1
+    assert lib.istnet_embed_scratch_kib(0, 4, 4) == -1 and lib.istnet_embed_scratch_kib(40000, 1, 1) >= 1
     forward = lambda n, v, k, t, red, z=one: lib.istnet_distill_forward(n, v, k, 0, 0, 0, z, v, one, one, t, red, one, one, one, one,
                                                                         one, None)
     assert forward(0, 4, 2, 1.0, 1) == forward(4, 0, 2, 1.0, 1) == forward(4, 4, 0, 1.0, 1) == forward(4, 4, 257, 1.0, 1) == bad
