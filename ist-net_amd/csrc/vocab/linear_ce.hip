@@ -465,44 +465,53 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
 
 // ---- before and after the products -------------------------------------------------------------------------------------------
 
-// largest magnitude of a row (infinities as they come, NaN passed over), this lane's part
-template <typename T> __device__ __forceinline__ float row_amax(const T* row, int d, float m) {
-  for (int c = (threadIdx.x & 63) * kVec<T>; c < d; c += 64 * kVec<T>) {
-    float f[kVec<T>];
-    load_part(row + c, d - c, f);
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) m = fmaxf(m, fabsf(f[i]));
-  }
-  return m;
+__device__ __forceinline__ bool row_counts(const void* target, long long i, int idx64, long long ignore) {
+  return load_index(target, i, idx64) != ignore;
 }
-__device__ __forceinline__ void store_amax(float m, float* tmp, float* part) {
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
-}
-// the largest magnitude of the rows of x that count ([0, xwgs)) and of w, one value per workgroup
+
+// Workgroups [0, xwgs): the largest magnitude of the rows of x that count; [xwgs, xwgs + wwgs): of w (infinities as they come, NaN
+// passed over), one value per workgroup; the rest: counted rows per block of 256.  A wave has four rows' loads in flight.
 template <typename T>
-__global__ __launch_bounds__(256) void ce_amax_kernel(int n, int v, int d, const T* __restrict__ x, long long ldx,
+__global__ __launch_bounds__(256) void ce_scan_kernel(int n, int v, int d, const T* __restrict__ x, long long ldx,
                                                       const T* __restrict__ w, long long ldw, const void* __restrict__ target,
-                                                      int idx64, long long ignore, int xwgs, float* __restrict__ part) {
+                                                      int idx64, long long ignore, int xwgs, int wwgs, float* __restrict__ part,
+                                                      int* __restrict__ blocks) {
   __shared__ float tmp[4];
-  const int wave = threadIdx.x >> 6;
-  float m = 0.f;
-  if ((int)blockIdx.x < xwgs) {
-    for (int r = blockIdx.x * 4 + wave; r < n; r += xwgs * 4)
-      if (load_index(target, r, idx64) != ignore) m = row_amax(x + r * ldx, d, m);
-  } else {
-    for (int r = (blockIdx.x - xwgs) * 4 + wave; r < v; r += (gridDim.x - xwgs) * 4) m = row_amax(w + r * ldw, d, m);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wg = blockIdx.x;
+  if (wg >= xwgs + wwgs) {
+    const int b = wg - xwgs - wwgs, i = b * 256 + threadIdx.x;
+    const int c = __syncthreads_count(i < n && row_counts(target, i, idx64, ignore));
+    if (threadIdx.x == 0) blocks[b] = c;
+    return;
   }
-  store_amax(m, tmp, part);
-}
-// counted rows per block of 256
-__global__ __launch_bounds__(256) void ce_count_kernel(int n, const void* __restrict__ target, int idx64, long long ignore,
-                                                       int* __restrict__ blocks) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const int c = __syncthreads_count(i < n && load_index(target, i, idx64) != ignore);
-  if (threadIdx.x == 0) blocks[blockIdx.x] = c;
+  const bool is_x = wg < xwgs;
+  const T* src = is_x ? x : w;
+  const long long ld = is_x ? ldx : ldw;
+  const int rows = is_x ? n : v, step = (is_x ? xwgs : wwgs) * 4;
+  float m = 0.f;
+  for (int r0 = (is_x ? wg : wg - xwgs) * 4 + wave; r0 < rows; r0 += 4 * step) {
+    const T* p[4];
+    bool on[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long r = r0 + (long long)j * step;
+      on[j] = r < rows && (!is_x || row_counts(target, r, idx64, ignore));
+      p[j] = src + (r < rows ? r : r0) * ld;
+    }
+    for (int c = lane * kVec<T>; c < d; c += 64 * kVec<T>) {
+      float f[4][kVec<T>];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load_part(p[j] + c, d - c, f[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) m = on[j] ? fmaxf(m, fabsf(f[j][i])) : m;
+    }
+  }
+  m = wave_max(m);
+  if (lane == 0) tmp[wave] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) part[wg] = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
 }
 
 __device__ __forceinline__ float scale_for(float amax) {      // power of two that takes amax to [2^14, 2^15)
@@ -512,25 +521,20 @@ __device__ __forceinline__ float scale_for(float amax) {      // power of two th
   return ldexpf(1.f, max(-126, min(126, 15 - ex)));
 }
 
-// rows counted before each block of 256 (in place where ce_count_kernel left the counts), number of rows, scales
-__global__ __launch_bounds__(1024) void ce_plan_kernel(int n, int counted, const void* __restrict__ target, int idx64, long long ignore,
-                                                       int split, int xwgs, int wgs, const float* __restrict__ amax,
+__device__ __forceinline__ void store_scalars(float* scal, int count, float sx, float sw) {
+  scal[kCount] = (float)count;
+  scal[kLogitScale] = kLog2e / sx / sw;
+  scal[kXScale] = sx;
+  scal[kWScale] = sw;
+  scal[kGMax] = 1.f;
+}
+
+// many rows: rows counted before each block of 256 (in place of the counts), number of rows, scales
+__global__ __launch_bounds__(1024) void ce_plan_kernel(int n, int xwgs, int wgs, const float* __restrict__ amax,
                                                        int* __restrict__ blocks, float* __restrict__ scal) {
   __shared__ int tmp[16];
   __shared__ float tmx[16], tmw[16];
   const int nb = (n + 255) / 256, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (!counted) {
-    for (int b = wave; b < nb; b += 16) {
-      int c = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = b * 256 + j * 64 + lane;
-        c += __popcll(__ballot(i < n && load_index(target, i < n ? i : 0, idx64) != ignore));
-      }
-      if (lane == 0) blocks[b] = c;
-    }
-    __syncthreads();
-  }
   int carry = 0;
   for (int base = 0; base < nb; base += 1024) {
     const int b = base + threadIdx.x, x = b < nb ? blocks[b] : 0;
@@ -552,24 +556,15 @@ __global__ __launch_bounds__(1024) void ce_plan_kernel(int n, int counted, const
     carry += all;
   }
   float mx = 0.f, mw = 0.f;
-  if (split) {
-    for (int i = threadIdx.x; i < wgs; i += 1024) {
-      if (i < xwgs) mx = fmaxf(mx, amax[i]); else mw = fmaxf(mw, amax[i]);
-    }
-    mx = wave_max(mx);
-    mw = wave_max(mw);
-    if (lane == 0) { tmx[wave] = mx; tmw[wave] = mw; }
-    __syncthreads();
-    for (int w = 0; w < 16; ++w) { mx = fmaxf(mx, tmx[w]); mw = fmaxf(mw, tmw[w]); }
+  for (int i = threadIdx.x; i < wgs; i += 1024) {
+    if (i < xwgs) mx = fmaxf(mx, amax[i]); else mw = fmaxf(mw, amax[i]);
   }
-  if (threadIdx.x == 0) {
-    const float sx = split ? scale_for(mx) : 1.f, sw = split ? scale_for(mw) : 1.f;
-    scal[kCount] = (float)carry;
-    scal[kLogitScale] = kLog2e / sx / sw;
-    scal[kXScale] = sx;
-    scal[kWScale] = sw;
-    scal[kGMax] = 1.f;
-  }
+  mx = wave_max(mx);
+  mw = wave_max(mw);
+  if (lane == 0) { tmx[wave] = mx; tmw[wave] = mw; }
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) { mx = fmaxf(mx, tmx[w]); mw = fmaxf(mw, tmw[w]); }
+  if (threadIdx.x == 0) store_scalars(scal, carry, wgs ? scale_for(mx) : 1.f, wgs ? scale_for(mw) : 1.f);
 }
 
 // Eight elements of a row as they lie in a packed operand: float16, scaled (P == 2: split); RAW: as they are.
@@ -612,27 +607,71 @@ __device__ __forceinline__ void pack_rows(const T* src, int to, int d, int kp, l
 }
 
 // Packed rows of x (and of w unless it is read as it lies), the bias in log2 units.  Workgroups [0, xwgs): 16 rows of x each; the next
-// 16: the zeros behind the last packed row; the rest: 16 rows of w a step, and the bias.
+// 16: the zeros behind the last packed row; the rest: 16 rows of w a step, and the bias.  Few rows (`planned` == 0): every workgroup
+// counts the rows before its own and takes the scale from the partial maxima itself, which saves a launch.
 constexpr int kPackRows = 16;
 template <typename T, int P, bool RAW>
 __global__ __launch_bounds__(256) void ce_pack_kernel(int n, int v, int d, int kp, int vp, const T* __restrict__ x, long long ldx,
                                                       const T* __restrict__ w, long long ldw, const T* __restrict__ bias,
-                                                      const void* __restrict__ target, int idx64, long long ignore, int xwgs,
-                                                      const int* __restrict__ blocks, const float* __restrict__ scal,
-                                                      char* __restrict__ xp, long long np, char* __restrict__ wp,
+                                                      const void* __restrict__ target, int idx64, long long ignore, int xwgs, int planned,
+                                                      int ax, int aw, const float* __restrict__ amax, const int* __restrict__ blocks,
+                                                      float* __restrict__ scal, char* __restrict__ xp, long long np, char* __restrict__ wp,
                                                       float* __restrict__ bias2, int* __restrict__ rowmap, int* __restrict__ inverse,
                                                       int* __restrict__ tgt, float* __restrict__ row_loss) {
-  __shared__ int flag[4];
+  __shared__ int flag[4], sums[2][4];
   __shared__ int where[256];
+  __shared__ float most[2][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wg = blockIdx.x;
+  const int block = wg < xwgs ? wg / (256 / kPackRows) : 0;
+  int before = 0, count = 0;
+  float sx = 1.f, sw = 1.f;
+  if (planned) {
+    before = wg < xwgs ? blocks[block] : 0;
+    count = (int)scal[kCount];
+    sx = scal[kXScale];
+    sw = scal[kWScale];
+  } else {
+    if (wg < xwgs + kPad / kPackRows) {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n; i += 256) {
+        const int c = row_counts(target, i, idx64, ignore);
+        count += c;
+        before += i < block * 256 ? c : 0;
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) {
+        count += __shfl_xor(count, o);
+        before += __shfl_xor(before, o);
+      }
+    }
+    float mx = 0.f, mw = 0.f;
+    for (int i = threadIdx.x; i < ax; i += 256) mx = fmaxf(mx, amax[i]);
+    for (int i = threadIdx.x; i < aw; i += 256) mw = fmaxf(mw, amax[ax + i]);
+    mx = wave_max(mx);
+    mw = wave_max(mw);
+    if (lane == 0) {
+      sums[0][wave] = count;
+      sums[1][wave] = before;
+      most[0][wave] = mx;
+      most[1][wave] = mw;
+    }
+    __syncthreads();
+    count = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+    before = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+    if (aw) {
+      sx = scale_for(fmaxf(fmaxf(most[0][0], most[0][1]), fmaxf(most[0][2], most[0][3])));
+      sw = scale_for(fmaxf(fmaxf(most[1][0], most[1][1]), fmaxf(most[1][2], most[1][3])));
+    }
+    if (wg == 0 && threadIdx.x == 0) store_scalars(scal, count, sx, sw);
+  }
   if (wg < xwgs) {
-    const int block = wg / (256 / kPackRows), i = block * 256 + threadIdx.x;
+    const int i = block * 256 + threadIdx.x;
     const long long t = i < n ? load_index(target, i, idx64) : ignore;
     const bool on = i < n && t != ignore;
     const uint64_t m = __ballot(on);
     if (lane == 0) flag[wave] = __popcll(m);
     __syncthreads();
-    int at = blocks[block] + __popcll(m & ((1ull << lane) - 1));
+    int at = before + __popcll(m & ((1ull << lane) - 1));
     for (int j = 0; j < wave; ++j) at += flag[j];
     where[threadIdx.x] = on ? at : -1;
     const int r0 = (wg % (256 / kPackRows)) * kPackRows;
@@ -647,9 +686,9 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(int n, int v, int d, int k
     }
     __syncthreads();
     const int r = r0 + (lane >> 2), to = where[r];
-    pack_rows<T, P, RAW>(to < 0 ? nullptr : x + (long long)(block * 256 + r) * ldx, to, d, kp, np, scal[kXScale], xp, np * kp * 2);
+    pack_rows<T, P, RAW>(to < 0 ? nullptr : x + (long long)(block * 256 + r) * ldx, to, d, kp, np, sx, xp, np * kp * 2);
   } else if (wg < xwgs + kPad / kPackRows) {
-    const int count = (int)scal[kCount], end = (count + kPad - 1) / kPad * kPad, r = count + (wg - xwgs) * kPackRows + (lane >> 2);
+    const int end = (count + kPad - 1) / kPad * kPad, r = count + (wg - xwgs) * kPackRows + (lane >> 2);
     pack_rows<T, P, RAW>(nullptr, r < end ? r : -1, d, kp, np, 1.f, xp, np * kp * 2);
     if (r < end && wave == 0 && (lane & 3) == 0) tgt[r] = -2;
   } else {
@@ -659,7 +698,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(int n, int v, int d, int k
     if (wp)
       for (int r0 = first * kPackRows; r0 < v; r0 += wgs * kPackRows) {
         const int r = r0 + (lane >> 2);
-        pack_rows<T, P, RAW>(w + (long long)(r < v ? r : 0) * ldw, r < v ? r : -1, d, kp, v, scal[kWScale], wp, (long long)v * kp * 2);
+        pack_rows<T, P, RAW>(w + (long long)(r < v ? r : 0) * ldw, r < v ? r : -1, d, kp, v, sw, wp, (long long)v * kp * 2);
       }
   }
 }
@@ -866,7 +905,16 @@ __global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chu
 
 // ---- sizes and launches ------------------------------------------------------------------------------------------------------
 
-constexpr int kMT = 256, kNT = 128;
+constexpr int kNT = 128;
+// the other side of a tile: 256, or less where that covers the classes / the features with less to spare
+inline int tile_v(int v) { return v <= 64 ? 64 : v <= 128 ? 128 : 256; }
+inline int tile_d(int d) { return d <= 64 ? 64 : (d + 127) / 128 * 128 < (d + 255) / 256 * 256 ? 128 : 256; }
+#define CE_TILE(size, MT, ...)                                    \
+  do {                                                            \
+    if ((size) == 256) { constexpr int MT = 256; __VA_ARGS__; }   \
+    else if ((size) == 128) { constexpr int MT = 128; __VA_ARGS__; } \
+    else { constexpr int MT = 64; __VA_ARGS__; }                  \
+  } while (0)
 constexpr long long kPieceBytes = 512ll << 20;           // memory of one piece of p - t
 constexpr int kMostSplits = 128;
 constexpr double kSmallProducts = 1 << 26;
@@ -896,7 +944,7 @@ inline Keep keep_plan(long long n, int d, int v, int dtype, bool direct) {
   k.planes = dtype == ISTNET_VOCAB_F32 ? 2 : 1;
   k.np = round_up(n, kPad) + kPad;      // zeros are written up to the next whole tile behind the last row
   k.kp = round_up(d, BK);
-  k.vp = round_up(v, kMT);
+  k.vp = round_up(v, tile_v(v));
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
   k.xp = take(2 * k.planes * k.np * k.kp);
@@ -911,9 +959,9 @@ inline Keep keep_plan(long long n, int d, int v, int dtype, bool direct) {
   return k;
 }
 struct Forward { long long part, zt, loss, blocks, amax, bytes; int tiles; };
-inline Forward forward_plan(const Keep& k) {
+inline Forward forward_plan(const Keep& k, int v) {
   Forward f = {};
-  f.tiles = (int)(k.vp / kMT);
+  f.tiles = (int)(k.vp / tile_v(v));
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
   f.part = take(8ll * f.tiles * k.np);
@@ -931,14 +979,15 @@ struct Backward {
 inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtype, int reduction) {
   Backward b = {};
   const long long planes = dtype == ISTNET_VOCAB_BF16 ? 1 : 2;      // of p - t
-  b.ld = round_up(d, kMT);
-  const long long dt = b.ld / kMT, seg = dtype == ISTNET_VOCAB_F32 ? 3 : planes;
+  const int mtv = tile_v(v);
+  b.ld = round_up(d, tile_d(d));
+  const long long dt = b.ld / tile_d(d), seg = dtype == ISTNET_VOCAB_F32 ? 3 : planes;
   // As few rounds of 512 workgroups for dw over all pieces as pieces of that memory allow, and as few pieces as that takes: 65536 classes
   // of 1024 features are four pieces of one full round each, not three of a round and a third.
-  const long long most = std::max<long long>(kMT, kPieceBytes / (2 * planes * k.np) / kMT * kMT), least = (k.vp + most - 1) / most;
+  const long long most = std::max<long long>(mtv, kPieceBytes / (2 * planes * k.np) / mtv * mtv), least = (k.vp + most - 1) / most;
   long long best = -1;
   for (long long p = least; p <= least + 3; ++p) {
-    const long long piece = round_up((k.vp + p - 1) / p, kMT), full = v / piece, rest = v - full * piece;
+    const long long piece = round_up((k.vp + p - 1) / p, mtv), full = v / piece, rest = v - full * piece;
     const long long rounds = full * ((dt * (piece / kNT) + 511) / 512) + (dt * ((rest + kNT - 1) / kNT) + 511) / 512;
     if (best < 0 || rounds < best) {
       best = rounds;
@@ -992,7 +1041,7 @@ extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
   if (small_ce(n, d, v)) return 0;
   const Keep k = keep_plan(n, d, v, dtype, false);
-  return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k).bytes) + 1023) / 1024);
+  return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k, v).bytes) + 1023) / 1024);
 }
 
 extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, int train, const void* x, long long ldx,
@@ -1005,26 +1054,19 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
     return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, st);
   const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
-  const Forward f = forward_plan(k);
+  const Forward f = forward_plan(k, v);
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = direct ? nullptr : kb + k.wp;
   float *scal = (float*)(kb + k.scal), *bias2 = (float*)(kb + k.bias2), *zt = (float*)(wb + f.zt);
   float *amax = (float*)(wb + f.amax), *packed_loss = (float*)(wb + f.loss), *row_loss = reduction == 0 ? loss : nullptr;
   RowStat* stat = (RowStat*)(kb + k.stat);
   int *blocks = (int*)(wb + f.blocks), *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse), *tgt = (int*)(kb + k.tgt);
-  const int ax = (int)std::min<long long>(256, (n + 3) / 4), aw = (int)std::min<long long>(768, (v + 3ll) / 4);
-  if (scaled) {
-    if (dtype == ISTNET_VOCAB_F32)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_amax_kernel<float>), dim3(ax + aw), dim3(256), 0, st, (int)n, v, d, (const float*)x, ldx,
-                         (const float*)w, ldw, target, idx64, ignore, ax, amax);
-    else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_amax_kernel<bf16>), dim3(ax + aw), dim3(256), 0, st, (int)n, v, d, (const bf16*)x, ldx,
-                         (const bf16*)w, ldw, target, idx64, ignore, ax, amax);
-  }
-  const int counted = n > 16384;      // up to here one workgroup counts the rows while it is at it
-  if (counted)
-    hipLaunchKernelGGL(ce_count_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, (int)n, target, idx64, ignore, blocks);
-  hipLaunchKernelGGL(ce_plan_kernel, dim3(1), dim3(1024), 0, st, (int)n, counted, target, idx64, ignore, (int)scaled, ax, ax + aw, amax,
-                     blocks, scal);
+  const int ax = scaled ? (int)std::min<long long>(256, (n + 15) / 16) : 0, aw = scaled ? (int)std::min<long long>(768, (v + 15ll) / 16) : 0;
+  const bool planned = n > 8192;
+  const int cw = planned ? (int)((n + 255) / 256) : 0;
+  if (ax + aw + cw)
+    VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_scan_kernel<T>), dim3(ax + aw + cw), dim3(256), 0, st, (int)n, v, d,
+                                                (const T*)x, ldx, (const T*)w, ldw, target, idx64, ignore, ax, aw, amax, blocks));
+  if (planned) hipLaunchKernelGGL(ce_plan_kernel, dim3(1), dim3(1024), 0, st, (int)n, ax, ax + aw, amax, blocks, scal);
   const int xwgs = (int)((n + 255) / 256 * (256 / kPackRows));
   const int wwgs = direct ? (bias ? (int)std::min<long long>(256, (k.vp + 255) / 256) : 0)
                           : (int)std::min<long long>(4096, (v + kPackRows - 1ll) / kPackRows);
@@ -1048,12 +1090,13 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
     typedef Matrix<T> X;
     const auto pack = [&](auto raw) {
       launch_pack<T, decltype(raw)::value>(xwgs + kPad / kPackRows + wwgs, st, (int)n, v, d, (int)k.kp, (int)k.vp, (const T*)x, ldx,
-                                           (const T*)w, ldw, (const T*)bias, target, idx64, ignore, xwgs, (const int*)blocks,
-                                           (const float*)scal, xp, k.np, wp, bias2, rowmap, inverse, tgt, row_loss);
+                                           (const T*)w, ldw, (const T*)bias, target, idx64, ignore, xwgs, (int)planned, ax, aw,
+                                           (const float*)amax, (const int*)blocks, scal, xp, k.np, wp, bias2, rowmap, inverse, tgt, row_loss);
     };
     const auto product = [&](auto m) {
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<decltype(m), X::LOGIT, 1, false, false, kMT, kNT, kLse, f16>),
-                         dim3(f.tiles * tn), dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), 0, 1, 0, e);
+      CE_TILE(tile_v(v), MT,
+              hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<decltype(m), X::LOGIT, 1, false, false, MT, kNT, kLse, f16>),
+                                 dim3(f.tiles * tn), dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), 0, 1, 0, e));
     };
     if (__is_same(T, bf16) && direct) {
       pack(std::true_type{});
@@ -1082,7 +1125,7 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = kb + k.wp, *dz = wb + b.dz, *xb = xp;
   float* scal = (float*)(kb + k.scal);
   int *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse);
-  const int tn = (int)((n + kNT - 1) / kNT), dt = (int)(b.ld / kMT);
+  const int tn = (int)((n + kNT - 1) / kNT), mtv = tile_v(v), mtd = tile_d(d), dt = (int)(b.ld / mtd);
   // weights of the rows' losses: taken into the rows of x that dw is formed from, which rounds them once more to 22 bits (float32) or
   // 11 (bfloat16); for float16 that would be the result's own precision, there they are taken into p - t
   const bool weighted = reduction == 0, folded = weighted && dtype == ISTNET_VOCAB_F16;
@@ -1116,8 +1159,9 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
       e.weights = folded ? gout : nullptr;
       e.v = v;
       e.v0 = v0;
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::LOGIT, PD, false, false, kMT, kNT, kDz, f16>), dim3(width / kMT * tn),
-                         dim3(256), 0, st, W, Xl, width / kMT, tn, (int)(k.kp / BK), 0, 1, 0, e);
+      CE_TILE(mtv, MT,
+              hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::LOGIT, PD, false, false, MT, kNT, kDz, f16>),
+                                 dim3(width / MT * tn), dim3(256), 0, st, W, Xl, width / MT, tn, (int)(k.kp / BK), 0, 1, 0, e));
       if (dx) {
         Epilogue s = {};
         s.scal = scal;
@@ -1125,8 +1169,9 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
         s.slab_stride = b.dx_rows * b.ld;
         s.ld_slab = b.ld;
         s.accumulate = piece > 0;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, false, kMT, kNT, kSlab, f16>),
-                           dim3(dt * tn * b.dx_splits), dim3(256), 0, st, W, D, dt, tn, (rows + BK - 1) / BK, b.dx_per, 1, 0, s);
+        CE_TILE(mtd, MT,
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, false, MT, kNT, kSlab, f16>),
+                                   dim3(dt * tn * b.dx_splits), dim3(256), 0, st, W, D, dt, tn, (rows + BK - 1) / BK, b.dx_per, 1, 0, s));
       }
       if (dw) {
         Epilogue s = {};
@@ -1142,11 +1187,13 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
         s.gout = gout;
         const int vt = (rows + kNT - 1) / kNT;
         if (b.dw_splits == 1) {
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kOut, T>), dim3(dt * vt), dim3(256), 0,
-                             st, Xw, D, dt, vt, 0, 0, 0, 1, s);
+          CE_TILE(mtd, MT,
+                  hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, MT, kNT, kOut, T>), dim3(dt * vt),
+                                     dim3(256), 0, st, Xw, D, dt, vt, 0, 0, 0, 1, s));
         } else {
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, kMT, kNT, kSlab, f16>),
-                             dim3(dt * vt * b.dw_splits), dim3(256), 0, st, Xw, D, dt, vt, 0, b.dw_per, 0, 1, s);
+          CE_TILE(mtd, MT,
+                  hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, MT, kNT, kSlab, f16>),
+                                     dim3(dt * vt * b.dw_splits), dim3(256), 0, st, Xw, D, dt, vt, 0, b.dw_per, 0, 1, s));
           hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dw_kernel<T>), dim3((unsigned)(((long long)rows * ((d + 3) / 4) + 63) / 64)), dim3(256),
                              0, st, rows, d, b.dw_splits, s.slab, s.slab_stride, b.ld, gout, reduction, scal, dw0);
         }
