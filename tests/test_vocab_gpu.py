@@ -527,3 +527,246 @@ def test_linear_ce_refusals():
     (dx,) = torch.autograd.grad(losses.LinearCrossEntropy(x, w, t, b), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,d,v", [(1, 1024, 5000), (1, 96, 70001), (200, 64, 9000), (130, 100, 5000), (5000, 32, 700), (40, 24, 50)])
+def test_linear_ce_without_a_backward(n, d, v, dtype):
+    x, w, b, t = _ce_inputs(n, d, v, dtype, n + d, ignored=0.2 if n > 1 else 0.0)
+    for bias in (b, None):
+        for reduction in ("none", "mean"):
+            with torch.no_grad():
+                loss = losses.LinearCrossEntropy(x, w, t, bias, IGNORE, reduction)
+            gout = torch.ones_like(loss)
+            want, bound, *_ = _ce_reference(x, w, bias, t, reduction, gout)
+            _within(loss, want, bound, "loss")
+            assert not loss.requires_grad
+    wide = torch.cat((w, w[:, :8]), 1)                                 # rows that are read as they lie, with a stride
+    with torch.no_grad():
+        strided = losses.LinearCrossEntropy(x, wide[:, :d], t, b, IGNORE, "none")
+        plain = losses.LinearCrossEntropy(x, w, t, b, IGNORE, "none")
+    want, bound, *_ = _ce_reference(x, w, b, t, "none", torch.ones(n, device=DEV))
+    _within(strided, plain.double(), 2 * bound, "strided")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d,v", [(384, 128), (128, 64), (64, 100), (130, 40), (640, 129)])
+def test_linear_ce_few_classes_many_rows(d, v, dtype):
+    """Past the four launches of small problems: every tile shape."""
+    n = 9000
+    for reduction in ("mean", "none"):
+        x, w, b, t = _ce_inputs(n, d, v, dtype, d + v, ignored=0.3)
+        _check_ce(x, w, b, t, reduction)
+
+
+# ---- used together, and as programs use them ---------------------------------------------------------------------------
+
+def _step(table, head, hb, ids, target, top, idx, dtype):
+    """Tokens in, a small body, a loss over the vocabulary with the table as its weight, and a distilled category head."""
+    h = pointnet2_utils.embedding_operation(table, ids, 4.0, 0)
+    h = torch.tanh(h.float()).to(dtype)
+    ce = losses.LinearCrossEntropy(h, table, target, ignore_index=0)
+    z = h.float() @ head.float().t() + hb.float()
+    kd = losses.TopLogitsDistill(z.to(dtype), top, idx, temperature=2.0)
+    return ce + 0.5 * kd
+
+
+def _step_reference(table, head, hb, ids, target, top, idx, dtype):
+    table, head, hb = (a.detach().double().cpu().requires_grad_() for a in (table, head, hb))
+    ids, target, idx, top = ids.long().cpu(), target.cpu(), idx.cpu(), top.double().cpu()
+    looked = table[ids] * 4.0
+    looked = looked * (ids != 0).unsqueeze(-1) + (looked * (ids == 0).unsqueeze(-1)).detach()      # the padding row gets no gradient here
+    h = torch.tanh(looked)
+    ce = losses.LinearCrossEntropy(h, table, target, ignore_index=0)
+    kd = losses.TopLogitsDistill(h @ head.t() + hb, top, idx, temperature=2.0)
+    loss = ce + 0.5 * kd
+    return loss.detach(), torch.autograd.grad(loss, (table, head, hb))
+
+
+def _step_inputs(dtype, seed, n=300, v=700, d=48, c=6):
+    g = _gen(seed)
+    table = (0.3 * torch.randn(v, d, device=DEV, generator=g)).to(dtype)
+    head, hb = (torch.randn(c, d, device=DEV, generator=g)).to(dtype), torch.randn(c, device=DEV, generator=g).to(dtype)
+    ids = torch.randint(0, v, (n,), device=DEV, generator=g)
+    target = torch.roll(ids, -1)
+    ids[::9] = 0
+    target[5::11] = 0
+    idx = torch.stack([torch.randperm(c, device=DEV, generator=g)[:3] for _ in range(n)])
+    idx[::4, 2] = -1
+    idx[::7] = -1
+    top = torch.randn(n, 3, device=DEV, generator=g).to(dtype)
+    return table, head, hb, ids, target, top, idx
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(300, 700), (5000, 6000)])
+def test_lookup_loss_and_distillation_together(dtype, n, v):
+    """Gradients of a step with all three, the table shared by the lookup and the loss.  bfloat16: the looked-up rows, the body's output
+    and the logits are each rounded (3 roundings on the way in, as many on the way back, the result once), float32 a few units."""
+    args = _step_inputs(dtype, 1, n, v)
+    leaves = [a.detach().requires_grad_() for a in args[:3]]
+    loss = _step(*leaves, *args[3:], dtype)
+    grads = torch.autograd.grad(loss, leaves)
+    want, wgrads = _step_reference(*args, dtype)
+    tol = 64 * U if dtype == F32 else 8 * _round(BF16)
+    assert abs(float(loss.detach()) - float(want)) <= tol * abs(float(want))
+    for got, ref in zip(grads, wgrads):
+        ref = ref.to(DEV)
+        assert float((got.double() - ref).norm()) <= tol * float(ref.norm())
+
+
+def test_training_loop_with_the_flat_optimizer():
+    """A few steps under optim.FlatAdam against torch.optim.Adam on the same native gradients."""
+    from istnet_amd.optim import FlatAdam
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.table = pointnet2_utils.ScaledEmbedding(300, 32, padding_idx=0)
+            self.head = torch.nn.Linear(32, 300)
+
+        def forward(self, ids, target):
+            return losses.LinearCrossEntropy(torch.tanh(self.table(ids)), self.head.weight, target, self.head.bias)
+
+    torch.manual_seed(3)
+    one, two = Net().to(DEV), Net().to(DEV)
+    two.load_state_dict(one.state_dict())
+    opts = FlatAdam(one.parameters(), lr=1e-2), torch.optim.Adam(two.parameters(), lr=1e-2)
+    ids = torch.randint(0, 300, (4, 64), device=DEV)
+    target = torch.roll(ids, -1, 1)
+    for _ in range(4):
+        for net, opt in zip((one, two), opts):
+            opt.zero_grad()
+            net(ids, target).backward()
+            opt.step()
+    for (name, p), q in zip(one.named_parameters(), two.parameters()):
+        assert p.grad is not None and torch.isfinite(p).all(), name
+        # Adam divides by the root of the second moment: equal gradients give updates that differ by a few units of the step
+        assert float((p - q).abs().max()) <= 1e-4 * 1e-2 * 4 + 4 * U * float(q.abs().max()), name
+
+
+@pytest.mark.parametrize("n,v", [(300, 700), (2500, 6000)])
+def test_captured_steps_replay_with_new_inputs(n, v):
+    """Two captured steps alternate with eager work on the same sizes; every replay gives the eager step's bits."""
+    dtype = F32
+    sets = [_step_inputs(dtype, 40 + i, n, v) for i in range(3)]
+    want = []
+    for s in sets:
+        leaves = [a.detach().requires_grad_() for a in s[:3]]
+        loss = _step(*leaves, *s[3:], dtype)
+        want.append([loss.detach().clone(), *[g.clone() for g in torch.autograd.grad(loss, leaves)]])
+    held = []
+    for k in range(2):
+        static = [a.clone() for a in sets[k]]
+        leaves = [a.requires_grad_() for a in static[:3]]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                torch.autograd.grad(_step(*leaves, *static[3:], dtype), leaves)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = _step(*leaves, *static[3:], dtype)
+            out = [loss.detach(), *torch.autograd.grad(loss, leaves)]
+        held.append((graph, static, out))
+    for turn in range(4):
+        for k, (graph, static, out) in enumerate(held):
+            pick = (turn + k) % 3
+            with torch.no_grad():
+                for dst, src in zip(static, sets[pick]):
+                    dst.copy_(src)
+            graph.replay()
+            leaves = [a.detach().requires_grad_() for a in sets[(pick + 1) % 3][:3]]
+            eager = torch.autograd.grad(_step(*leaves, *sets[(pick + 1) % 3][3:], dtype), leaves)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[pick])), (turn, k)
+            assert all(torch.equal(a, b) for a, b in zip(eager, want[(pick + 1) % 3][1:])), (turn, k)
+
+
+def test_calls_on_several_streams():
+    args = _step_inputs(F32, 9, 3000, 5000)
+    leaves = [a.detach().requires_grad_() for a in args[:3]]
+    first = torch.autograd.grad(_step(*leaves, *args[3:], F32), leaves)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(2):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                own = [a.detach().clone().requires_grad_() for a in args[:3]]
+                got.append(torch.autograd.grad(_step(*own, *args[3:], F32), own))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, first))
+
+
+def test_backward_twice_and_changed_operands():
+    x, w, b, t = _ce_inputs(5000, 40, 600, F32, 8)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    loss = losses.LinearCrossEntropy(x, w, t, b)
+    one = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    two = torch.autograd.grad(loss, (x, w))
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+    loss = losses.LinearCrossEntropy(x, w, t, b)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(loss, (x, w))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows behind the 2^31st element of the logits, of a table and of a head, against the same rows alone."""
+    g = _gen(17)
+    n, v = 33000, 65600                                            # 2.16e9 logits
+    z = torch.empty(n, v, device=DEV, dtype=F16)
+    for a in range(0, n, 3000):
+        z[a:a + 3000].normal_(generator=g)
+    idx = torch.randint(0, v, (n, 4), device=DEV, generator=g)
+    top = torch.randn(n, 4, device=DEV, generator=g)
+    z.requires_grad_()
+    loss = losses.TopLogitsDistill(z, top, idx, reduction="none")
+    (dz,) = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    tail = z.detach()[-5:].clone().requires_grad_()
+    part = losses.TopLogitsDistill(tail, top[-5:], idx[-5:], reduction="none")
+    (dtail,) = torch.autograd.grad(part, tail, torch.ones_like(part))
+    torch.testing.assert_close(loss[-5:], part, rtol=256 * U, atol=256 * U)
+    torch.testing.assert_close(dz[-5:].float(), dtail.float(), rtol=2 * _round(F16) + 256 * U, atol=_tiny(F16) * 2)
+    del z, dz, loss
+    rows, d = 2_200_000, 1000                                      # 2.2e9 entries
+    table = torch.empty(rows, d, device=DEV, dtype=F16)
+    table[-1000:].normal_(generator=g)
+    table.requires_grad_()
+    ids = torch.cat((torch.tensor([0, rows - 1, rows - 2, rows - 1], device=DEV),
+                     torch.randint(rows - 900, rows, (3000,), device=DEV, generator=g)))
+    out = pointnet2_utils.embedding_operation(table, ids, 2.0)
+    assert torch.equal(out[1:], table.detach()[ids[1:]] * 2)
+    grad = torch.randn(out.shape, device=DEV, generator=g).to(F16)
+    for m in (4, ids.numel()):                                     # one launch, and the sort
+        (dw,) = torch.autograd.grad(pointnet2_utils.embedding_operation(table, ids[:m], 2.0), table, grad[:m])
+        small = table.detach()[-1000:].clone().requires_grad_()
+        (ds,) = torch.autograd.grad(pointnet2_utils.embedding_operation(small, ids[1:m] - (rows - 1000), 2.0), small, grad[1:m])
+        assert torch.equal(dw[-1000:], ds) and (dw[1:-1000:4001] == 0).all() and torch.equal(dw[0], grad[0] * 2)
+        del dw
+    del out, table
+    x = torch.randn(8, d, device=DEV, generator=g)
+    w = torch.empty(rows, d, device=DEV, dtype=F16)
+    for a in range(0, rows, 200_000):
+        w[a:a + 200_000].normal_(0.0, 0.01, generator=g)
+    w[-3:] *= 8.0
+    target = torch.tensor([rows - 1, rows - 2, 5, rows - 3, 7, rows - 1, 0, 1_500_000], device=DEV)
+    xh = x.to(F16).requires_grad_()
+    w.requires_grad_()
+    loss = losses.LinearCrossEntropy(xh, w, target, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (xh, w), torch.ones_like(loss))
+    logits = torch.empty(8, rows, device=DEV, dtype=torch.float64)
+    for a in range(0, rows, 200_000):
+        logits[:, a:a + 200_000] = xh.detach().double() @ w.detach()[a:a + 200_000].double().t()
+    want = torch.logsumexp(logits, 1) - logits.gather(1, target.unsqueeze(1)).squeeze(1)
+    torch.testing.assert_close(loss.double(), want, rtol=4096 * U, atol=4096 * U)
+    p = torch.exp(logits - torch.logsumexp(logits, 1, keepdim=True))
+    p.scatter_add_(1, target.unsqueeze(1), -torch.ones(8, 1, device=DEV, dtype=torch.float64))
+    tail = p[:, -2000:].t() @ xh.detach().double()
+    assert float((dw[-2000:].double() - tail).norm()) <= 4 * _round(F16) * float(tail.norm())
+    dxw = sum(p[:, a:a + 200_000] @ w.detach()[a:a + 200_000].double() for a in range(0, rows, 200_000))
+    assert float((dx.double() - dxw).norm()) <= 4 * _round(F16) * float(dxw.norm())
