@@ -200,15 +200,15 @@ enum { kLse = 0, kDz = 1, kSlab = 2, kOut = 3 };
 // that make one up, walked one after the other along K, small ones first (1: hi hi; 2: hi lo, hi hi; 3: lo hi, hi lo, hi hi);
 // PD: planes of p - t that are written; T: element type of the final output.  The lane of column n holds rows 8 j + 4 (lane / 32) + 0..3 of every 32 x 32 block.
 // ROWS_N / ROWS_K: the packed rows are the N dimension (tiles behind the last row leave) / the K dimension (it ends there).
+template <int MT, int NT> constexpr int kTileLds = kStages * (MT + NT) * 64;
 template <typename M, int SEGS, int PD, bool AKS, bool BKS, int MT, int NT, int EPI, typename T>
-__global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, int tm, int tn, int ksteps, int per_split, int rows_n,
-                                                         int rows_k, Epilogue e) {
+__device__ __forceinline__ void ce_tile(char* lds, int wg, int wgs, Operand a, Operand b, int tm, int tn, int ksteps, int per_split,
+                                        int rows_n, int rows_k, Epilogue e) {
   constexpr int WAVES = 4, MB = MT / 64, NB = NT / 64;
   constexpr int ABYTES = MT * 64, BBYTES = NT * 64, STAGE = ABYTES + BBYTES;
-  __shared__ __attribute__((aligned(1024))) char lds[kStages * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
   int mt, nt, split;
-  tile_of(blockIdx.x, gridDim.x, tm, tn, &mt, &nt, &split);
+  tile_of(wg, wgs, tm, tn, &mt, &nt, &split);
   const int count = (rows_n || rows_k) ? (int)e.scal[kCount] : 0;
   if (rows_n && nt * NT >= count) return;
   if (rows_k) ksteps = (count + BK - 1) / BK;
@@ -305,11 +305,12 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
           for (int r = 0; r < 4; ++r) acc[i][j][g * 4 + r] = __builtin_fmaf(acc[i][j][g * 4 + r], scale, bb[r]);
         }
     } else if (e.v0 + m0 + MT > e.v) {
+      const int left = e.v - e.v0 - mw - half * 4;      // classes from this lane's first row on
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (e.v0 + mw + i * 32 + (r >> 2) * 8 + half * 4 + (r & 3) >= e.v) acc[i][j][r] = -INFINITY;
+          if (i * 32 + (r >> 2) * 8 + (r & 3) >= left) acc[i][j][r] = -INFINITY;
     }
   };
   if constexpr (EPI == kLse) {
@@ -320,14 +321,19 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
       finish_logits(j);
       const int t = e.target[n] - mw;
       if (__any(t >= 0 && t < MT / 2)) {
+        const int mine = t - half * 4;
+        float z = 0.f;
+        bool here = false;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (t == i * 32 + (r >> 2) * 8 + half * 4 + (r & 3)) {
-              e.zt[n] = acc[i][j][r];
-              acc[i][j][r] = -INFINITY;
-            }
+          for (int r = 0; r < 16; ++r) {
+            const bool is = mine == i * 32 + (r >> 2) * 8 + (r & 3);
+            z = is ? acc[i][j][r] : z;
+            here |= is;
+            acc[i][j][r] = is ? -INFINITY : acc[i][j][r];
+          }
+        if (here) e.zt[n] = z;
       }
       float m = -INFINITY;
 #pragma unroll
@@ -351,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
   } else if constexpr (EPI == kDz) {
     // per wave NT / 2 rows of MT / 2 classes, written row by row: pitch MT / 2 + 8 elements keeps the rows' writes apart
     constexpr int PITCH = MT / 2 + 8, ROWS = NT / 2;
-    static_assert(4 * ROWS * PITCH * 2 <= kStages * STAGE, "the epilogue's rows fit the tiles' LDS");
+    static_assert(4 * ROWS * PITCH * 2 <= kTileLds<MT, NT>, "the epilogue's rows fit the tiles' LDS");
     uint16_t* mine = reinterpret_cast<uint16_t*>(lds) + wave * ROWS * PITCH;
 #pragma unroll
     for (int pl = 0; pl < PD; ++pl) {
@@ -371,10 +377,11 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
           const int t = e.target[n] - e.v0 - mw;
           if (__any(t >= 0 && t < MT / 2)) {
             const float x = one * st.at_target;
+            const int mine = t - half * 4;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) acc[i][j][r] = t == i * 32 + (r >> 2) * 8 + half * 4 + (r & 3) ? x : acc[i][j][r];
+              for (int r = 0; r < 16; ++r) acc[i][j][r] = mine == i * 32 + (r >> 2) * 8 + (r & 3) ? x : acc[i][j][r];
           }
         }
 #pragma unroll
@@ -461,6 +468,82 @@ __global__ __launch_bounds__(256, 2) void ce_gemm_kernel(Operand a, Operand b, i
       }
     }
   }
+}
+
+// The products with the logits: kLse, kDz.
+template <typename M, int SEGS, int PD, int MT, int NT, int EPI>
+__global__ __launch_bounds__(256, 2) void ce_logits_kernel(Operand w, Operand x, int tm, int tn, int ksteps, Epilogue e) {
+  __shared__ __attribute__((aligned(1024))) char lds[kTileLds<MT, NT>];
+  ce_tile<M, SEGS, PD, false, false, MT, NT, EPI, f16>(lds, blockIdx.x, gridDim.x, w, x, tm, tn, ksteps, 0, 1, 0, e);
+}
+
+// db: column sums of p - t over the packed rows.  A workgroup has one panel and `chunk` rows: sixteen rows times four chunks of eight
+// columns per wave, the lanes of a column added up in a fixed order.
+template <int PD>
+__device__ __forceinline__ void column_sums(float* tmp, int unit, int part_no, const Operand& dz, const float* weights, const int* rowmap,
+                                            const float* scal, int chunk, float* part, long long part_ld) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = (int)scal[kCount];
+  const int a = part_no * chunk, b = min(count, a + chunk);
+  const long long at = unit * dz.unit_stride + ((lane & 3) << 4);
+  float s[8] = {};
+#pragma unroll 4
+  for (int r = a + wave * 16 + (lane >> 2); r < b; r += 64) {
+    const float g = weights ? weights[rowmap[r]] : 1.f;
+    float f[8];
+    unpack<f16>(*reinterpret_cast<const u32x4*>(dz.plane[0] + at + r * 64ll), f);
+    if constexpr (PD == 2) {
+      float l[8];
+      unpack<f16>(*reinterpret_cast<const u32x4*>(dz.plane[1] + at + r * 64ll), l);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] += l[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] += g * f[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) s[i] += __shfl_xor(s[i], o);
+    if (lane < 4) tmp[wave * 32 + lane * 8 + i] = s[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 32)
+    part[part_no * part_ld + unit * 32 + threadIdx.x] =
+        tmp[threadIdx.x] + tmp[32 + threadIdx.x] + tmp[64 + threadIdx.x] + tmp[96 + threadIdx.x];
+}
+
+// What is formed from a piece of p - t, in one launch: tiles of dw (K: the packed rows), tiles of dx (K: the piece's classes), column
+// sums.  The counts are rounded up to a multiple of eight, so that each part meets the XCDs as a launch of its own would.
+struct Grads {
+  Operand w, x, dz;
+  Epilogue dw, dx;
+  int dt;                        // tiles of d
+  int dw_wgs, dw_tn, dw_per;
+  int dx_wgs, dx_tn, dx_per, dx_steps;
+  int col_units, chunk;
+  const float* col_weights;
+  const int* rowmap;
+  float* col;
+  long long col_ld;
+};
+template <int SEGS, int PD, int MT, int NT, int DW, typename T>
+__global__ __launch_bounds__(256, 2) void ce_grads_kernel(Grads g) {
+  __shared__ __attribute__((aligned(1024))) char lds[kTileLds<MT, NT>];
+  int wg = blockIdx.x;
+  if (wg < ((g.dw_wgs + 7) & ~7)) {
+    if (wg < g.dw_wgs)
+      ce_tile<f16, SEGS, 1, true, true, MT, NT, DW, T>(lds, wg, g.dw_wgs, g.x, g.dz, g.dt, g.dw_tn, 0, g.dw_per, 0, 1, g.dw);
+    return;
+  }
+  wg -= (g.dw_wgs + 7) & ~7;
+  if (wg < ((g.dx_wgs + 7) & ~7)) {
+    if (wg < g.dx_wgs)
+      ce_tile<f16, SEGS, 1, true, false, MT, NT, kSlab, T>(lds, wg, g.dx_wgs, g.w, g.dz, g.dt, g.dx_tn, g.dx_steps, g.dx_per, 1, 0, g.dx);
+    return;
+  }
+  wg -= (g.dx_wgs + 7) & ~7;
+  column_sums<PD>(reinterpret_cast<float*>(lds), wg % g.col_units, wg / g.col_units, g.dz, g.col_weights, g.rowmap, g.dw.scal, g.chunk,
+                  g.col, g.col_ld);
 }
 
 // ---- before and after the products -------------------------------------------------------------------------------------------
@@ -714,25 +797,32 @@ __global__ __launch_bounds__(256) void ce_weigh_kernel(int d, int kp, const T* _
                          i < 0 ? 0.f : gout[i] / scal[kGMax] * scal[kXScale], xp, np * kp * 2);
 }
 
-// statistics and loss of 16 packed rows per workgroup, from the tiles' partial sums
+// statistics and loss of ROWS packed rows per workgroup, from the tiles' partial sums: 256 / ROWS parts of the tiles side by side
+// (Adding the losses up is a launch of its own, 5 us: the last workgroup doing it instead cost 30 us for 460 workgroups and 95 for 1430 in
+// fences between the XCDs' caches.)
+template <int ROWS>
 __global__ __launch_bounds__(256) void ce_finish_kernel(int tiles, int parts_ld, int biased, const float2* __restrict__ part,
                                                         const float* __restrict__ zt, const int* __restrict__ tgt,
                                                         const int* __restrict__ rowmap, const float* __restrict__ scal,
                                                         RowStat* __restrict__ stat, float* __restrict__ packed_loss,
                                                         float* __restrict__ row_loss) {
-  __shared__ float2 tmp[16][17];
-  const int count = (int)scal[kCount], t = threadIdx.x & 15, j = threadIdx.x >> 4, row = blockIdx.x * 16 + t;
-  if (blockIdx.x * 16 >= (count + kPad - 1) / kPad * kPad) return;
+  constexpr int PARTS = 256 / ROWS;
+  __shared__ float2 tmp[PARTS][ROWS + 1];
+  const int count = (int)scal[kCount], t = threadIdx.x % ROWS, j = threadIdx.x / ROWS, row = blockIdx.x * ROWS + t;
+  if ((int)blockIdx.x * ROWS >= (count + kPad - 1) / kPad * kPad) return;
   float2 ms = make_float2(-INFINITY, 0.f);
   if (row < count) {
 #pragma unroll 4
-    for (int k = j; k < tiles; k += 16) ms = merge(ms, part[(long long)k * parts_ld + row]);
+    for (int k = j; k < tiles; k += PARTS) ms = merge(ms, part[(long long)k * parts_ld + row]);
   }
   tmp[j][t] = ms;
-  __syncthreads();
+#pragma unroll
+  for (int o = PARTS / 2; o; o >>= 1) {
+    __syncthreads();
+    if (j < o) tmp[j][t] = ms = merge(ms, tmp[j + o][t]);
+  }
   if (j == 0) {
     if (row < count) {
-      for (int k = 1; k < 16; ++k) ms = merge(ms, tmp[k][t]);
       // ms: the other classes.  d = target's logit above their largest; loss = log(1 + rest), rest = others over target
       RowStat r = {kNaN, kNaN, kNaN, 0.f};
       float loss = kNaN;
@@ -766,6 +856,7 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(int mean, const float* _
   __shared__ double tmp[16];
   const int count = (int)scal[kCount];
   double sum = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < count; i += 1024) sum += packed_loss[i];
   sum = wave_sum(sum);
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = sum;
@@ -793,114 +884,86 @@ __global__ __launch_bounds__(1024) void ce_gmax_kernel(const float* __restrict__
   }
 }
 
-// dx: slabs added in order, scaled, back to the rows they belong to; rows that do not count get zeros
+// What is left when all pieces are done, in one launch.  dx: slabs added in order, scaled, back to the rows they belong to (zeros in rows
+// that do not count).  dw where its product was split along the rows: four parts of the slabs side by side, each in order, joined in
+// order.  db: the chunks' sums in order.
+struct Final {
+  int n, d, v, reduction, folded;
+  const float *gout, *scal;
+  const int* inverse;
+  const float* dx_slab;
+  long long dx_stride, ld;
+  int dx_splits;
+  unsigned dx_wgs, dw_wgs;
+  const float* dw_slab;
+  long long dw_stride;
+  int dw_splits;
+  const float* col;
+  long long col_ld;
+  int chunks;
+  void *dx, *dw, *db;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void ce_dx_kernel(int n, int d, int splits, const float* __restrict__ slab, long long slab_stride,
-                                                    long long ld, const int* __restrict__ inverse, const float* __restrict__ gout,
-                                                    int reduction, int folded, const float* __restrict__ scal, T* __restrict__ dx) {
-  const int per = (d + 3) / 4;
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, i = id / per;
-  if (i >= n) return;
-  const int c = (int)(id % per) * 4, at = inverse[i];
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  if (at >= 0) {
-    const float* p = slab + at * ld + c;
-    x = *reinterpret_cast<const f32x4*>(p);
-    for (int s = 1; s < splits; ++s) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * slab_stride);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] += y[r];
-    }
-    const float g = (folded ? scal[kGMax] : reduction == 0 ? gout[i] : reduction == 1 ? gout[0] / scal[kCount] : gout[0]) / kDzScale /
-                    scal[kWScale];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] *= g;
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (c + r < d) dx[i * d + c + r] = from_f32<T>(x[r]);
-}
-
-// dw where its product was split along the rows: four parts of the slabs side by side, each in order, joined in order
-template <typename T>
-__global__ __launch_bounds__(256) void ce_dw_kernel(int rows, int d, int splits, const float* __restrict__ slab, long long slab_stride,
-                                                    long long ld, const float* __restrict__ gout, int reduction,
-                                                    const float* __restrict__ scal, T* __restrict__ dw) {
+__global__ __launch_bounds__(256) void ce_final_kernel(Final f) {
   __shared__ f32x4 tmp[256];
-  const int per = (d + 3) / 4, part = threadIdx.x >> 6, each = (splits + 3) / 4;
-  const long long id = (long long)blockIdx.x * 64 + (threadIdx.x & 63), i = id / per;
-  const int c = (int)(id % per) * 4;
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  if (i < rows) {
-    const float* p = slab + i * ld + c;
+  const int per = (f.d + 3) / 4;
+  const float rows = f.scal[kCount];
+  const float whole = rows == 0.f ? 0.f : f.reduction == 0 ? f.scal[kGMax] : f.reduction == 1 ? f.gout[0] / rows : f.gout[0];
+  if (blockIdx.x < f.dx_wgs) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, i = id / per;
+    if (i >= f.n) return;
+    const int c = (int)(id % per) * 4, at = f.inverse[i];
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (at >= 0) {
+      const float* p = f.dx_slab + at * f.ld + c;
 #pragma unroll 8
-    for (int s = part * each; s < min(splits, (part + 1) * each); ++s) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * slab_stride);
+      for (int s = 0; s < f.dx_splits; ++s) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * f.dx_stride);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] += y[r];
+        for (int r = 0; r < 4; ++r) x[r] += y[r];
+      }
+      const float g = (f.reduction == 0 && !f.folded ? f.gout[i] : whole) / kDzScale / f.scal[kWScale];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] *= g;
     }
-  }
-  tmp[threadIdx.x] = x;
-  __syncthreads();
-  if (part || i >= rows) return;
-  for (int s = 1; s < 4; ++s)
+    T* out = (T*)f.dx + i * f.d + c;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] += tmp[s * 64 + threadIdx.x][r];
-  const float n = scal[kCount];
-  const float g = n == 0.f ? 0.f : (reduction == 0 ? scal[kGMax] : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale / scal[kXScale];
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (c + r < d) dw[i * d + c + r] = from_f32<T>(g * x[r]);
-}
-
-// db: column sums of p - t over the packed rows.  A workgroup has one panel and `chunk` rows: sixteen rows times four chunks of eight
-// columns per wave, the lanes of a column added up in a fixed order.
-template <int PD>
-__global__ __launch_bounds__(256) void ce_colsum_kernel(const char* __restrict__ hi, const char* __restrict__ lo, long long unit_stride,
-                                                        int width, const float* __restrict__ gout, const int* __restrict__ rowmap,
-                                                        const float* __restrict__ scal, int chunk, float* __restrict__ part) {
-  __shared__ float tmp[4][32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = (int)scal[kCount];
-  const int a = blockIdx.y * chunk, b = min(count, a + chunk);
-  const long long at = blockIdx.x * unit_stride + ((lane & 3) << 4);
-  float s[8] = {};
-#pragma unroll 4
-  for (int r = a + wave * 16 + (lane >> 2); r < b; r += 64) {
-    const float g = gout ? gout[rowmap[r]] : 1.f;
-    float f[8];
-    unpack<f16>(*reinterpret_cast<const u32x4*>(hi + at + r * 64ll), f);
-    if constexpr (PD == 2) {
-      float l[8];
-      unpack<f16>(*reinterpret_cast<const u32x4*>(lo + at + r * 64ll), l);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] += l[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] += g * f[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) s[i] += __shfl_xor(s[i], o);
-    if (lane < 4) tmp[wave][lane * 8 + i] = s[i];
-  }
-  __syncthreads();
-  if (threadIdx.x < 32)
-    part[(long long)blockIdx.y * width + blockIdx.x * 32 + threadIdx.x] =
-        tmp[0][threadIdx.x] + tmp[1][threadIdx.x] + tmp[2][threadIdx.x] + tmp[3][threadIdx.x];
-}
-template <typename T>
-__global__ __launch_bounds__(256) void ce_db_kernel(int rows, int width, int chunks, const float* __restrict__ part,
-                                                    const float* __restrict__ gout, int reduction, int folded,
-                                                    const float* __restrict__ scal, T* __restrict__ db) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= rows) return;
-  double s = 0.0;
+    for (int r = 0; r < 4; ++r)
+      if (c + r < f.d) out[r] = from_f32<T>(x[r]);
+  } else if (blockIdx.x < f.dx_wgs + f.dw_wgs) {
+    const int part = threadIdx.x >> 6, each = (f.dw_splits + 3) / 4;
+    const long long id = (long long)(blockIdx.x - f.dx_wgs) * 64 + (threadIdx.x & 63), i = id / per;
+    const int c = (int)(id % per) * 4;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (i < f.v) {
+      const float* p = f.dw_slab + i * f.ld + c;
 #pragma unroll 8
-  for (int k = 0; k < chunks; ++k) s += part[(long long)k * width + c];
-  const float n = scal[kCount];
-  const float g = n == 0.f ? 0.f : (folded ? scal[kGMax] : reduction == 0 ? 1.f : reduction == 1 ? gout[0] / n : gout[0]) / kDzScale;
-  db[c] = from_f32<T>((float)(g * s));
+      for (int s = part * each; s < min(f.dw_splits, (part + 1) * each); ++s) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(p + s * f.dw_stride);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] += y[r];
+      }
+    }
+    tmp[threadIdx.x] = x;
+    __syncthreads();
+    if (part || i >= f.v) return;
+    for (int s = 1; s < 4; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] += tmp[s * 64 + threadIdx.x][r];
+    const float g = whole / kDzScale / f.scal[kXScale];
+    T* out = (T*)f.dw + i * f.d + c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (c + r < f.d) out[r] = from_f32<T>(g * x[r]);
+  } else {
+    const int c = (blockIdx.x - f.dx_wgs - f.dw_wgs) * 256 + threadIdx.x;
+    if (c >= f.v) return;
+    double s = 0.0;
+#pragma unroll 8
+    for (int k = 0; k < f.chunks; ++k) s += f.col[k * f.col_ld + c];
+    const float g = (f.reduction == 0 && !f.folded ? (rows == 0.f ? 0.f : 1.f) : whole) / kDzScale;
+    ((T*)f.db)[c] = from_f32<T>((float)(g * s));
+  }
 }
 
 // ---- sizes and launches ------------------------------------------------------------------------------------------------------
@@ -917,6 +980,7 @@ inline int tile_d(int d) { return d <= 64 ? 64 : (d + 127) / 128 * 128 < (d + 25
   } while (0)
 constexpr long long kPieceBytes = 512ll << 20;           // memory of one piece of p - t
 constexpr int kMostSplits = 128;
+constexpr int kScanWgs = 2048;                           // workgroups at most that look for the largest entry of x, and of w
 constexpr double kSmallProducts = 1 << 26;
 
 inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
@@ -968,13 +1032,13 @@ inline Forward forward_plan(const Keep& k, int v) {
   f.zt = take(4 * k.np);
   f.loss = take(4 * k.np);
   f.blocks = take(4 * (k.np / 256 + 1));
-  f.amax = take(4 * 1024);
+  f.amax = take(4 * 2 * kScanWgs);
   f.bytes = at;
   return f;
 }
 struct Backward {
   int pieces, dx_splits, dx_per, dw_splits, dw_per, chunk, chunks;
-  long long piece, dz, xg, dx_slab, dx_rows, dw_slab, dw_rows, col, ld, bytes;
+  long long piece, dz, xg, dx_slab, dx_rows, dw_slab, dw_rows, col, ld, bytes;      // dw_rows: all classes, in whole tiles
 };
 inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtype, int reduction) {
   Backward b = {};
@@ -1001,10 +1065,10 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtyp
   };
   const long long most_rows = std::min<long long>(v, b.piece), dx_steps = (most_rows + BK - 1) / BK * seg, dw_steps = (n + BK - 1) / BK * seg;
   b.dx_rows = round_up(n, kNT);
-  b.dw_rows = round_up(most_rows, kNT);
+  b.dw_rows = round_up(v, std::max(mtv, kNT));
   b.dx_splits = (int)splits(dt * (b.dx_rows / kNT), dx_steps);
   b.dx_per = (int)((dx_steps + b.dx_splits - 1) / b.dx_splits);
-  b.dw_splits = (int)splits(dt * (b.dw_rows / kNT), dw_steps);
+  b.dw_splits = (int)splits(dt * ((most_rows + kNT - 1) / kNT), dw_steps);
   b.dw_per = (int)((dw_steps + b.dw_splits - 1) / b.dw_splits);
   b.chunk = (int)std::max<long long>(256, round_up((n + 127) / 128, 64));      // rows of one part of a bias gradient: 128 parts at most
   b.chunks = (int)((n + b.chunk - 1) / b.chunk);
@@ -1014,7 +1078,7 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtyp
   b.xg = reduction == 0 && dtype != ISTNET_VOCAB_F16 ? take(2 * k.planes * k.np * k.kp) : 0;
   b.dx_slab = take(4 * b.dx_splits * b.dx_rows * b.ld);
   b.dw_slab = b.dw_splits > 1 ? take(4 * b.dw_splits * b.dw_rows * b.ld) : 0;
-  b.col = take(4ll * b.chunks * b.piece);
+  b.col = take(4ll * b.chunks * k.vp);
   b.bytes = at;
   return b;
 }
@@ -1060,7 +1124,7 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   float *amax = (float*)(wb + f.amax), *packed_loss = (float*)(wb + f.loss), *row_loss = reduction == 0 ? loss : nullptr;
   RowStat* stat = (RowStat*)(kb + k.stat);
   int *blocks = (int*)(wb + f.blocks), *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse), *tgt = (int*)(kb + k.tgt);
-  const int ax = scaled ? (int)std::min<long long>(256, (n + 15) / 16) : 0, aw = scaled ? (int)std::min<long long>(768, (v + 15ll) / 16) : 0;
+  const int ax = scaled ? (int)std::min<long long>(kScanWgs, (n + 15) / 16) : 0, aw = scaled ? (int)std::min<long long>(kScanWgs, (v + 15ll) / 16) : 0;
   const bool planned = n > 8192;
   const int cw = planned ? (int)((n + 255) / 256) : 0;
   if (ax + aw + cw)
@@ -1095,8 +1159,8 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
     };
     const auto product = [&](auto m) {
       CE_TILE(tile_v(v), MT,
-              hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<decltype(m), X::LOGIT, 1, false, false, MT, kNT, kLse, f16>),
-                                 dim3(f.tiles * tn), dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), 0, 1, 0, e));
+              hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_logits_kernel<decltype(m), X::LOGIT, 1, MT, kNT, kLse>), dim3(f.tiles * tn),
+                                 dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), e));
     };
     if (__is_same(T, bf16) && direct) {
       pack(std::true_type{});
@@ -1106,7 +1170,9 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
       product(f16{});
     }
   });
-  hipLaunchKernelGGL(ce_finish_kernel, dim3((unsigned)(round_up(n, kPad) / 16)), dim3(256), 0, st, f.tiles, (int)k.np,
+  // few rows: more parts of the tiles, many: runs of rows in each read
+  const auto finish = n <= 1024 ? ce_finish_kernel<4> : ce_finish_kernel<16>;
+  hipLaunchKernelGGL(finish, dim3((unsigned)(round_up(n, kPad) / (n <= 1024 ? 4 : 16))), dim3(256), 0, st, f.tiles, (int)k.np,
                      bias != nullptr, (const float2*)(wb + f.part), zt, tgt, rowmap, scal, stat, packed_loss, row_loss);
   if (reduction != 0)
     hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, st, reduction == 1, packed_loss, scal, loss);
@@ -1119,6 +1185,7 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   if (!ce_ok(n, d, v, dtype) || !x || !w || !gout || !keep || (!ws && !small_ce(n, d, v)) || ldx < d || ldw < d || reduction < 0 || reduction > 2)
     return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
+  if (!dx && !dw && !db) return 0;
   if (small_ce(n, d, v)) return vocab_small_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, dx, dw, db, st);
   const Keep k = keep_plan(n, d, v, dtype, false);
   const Backward b = backward_plan(k, n, d, v, dtype, reduction);
@@ -1160,56 +1227,79 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
       e.v = v;
       e.v0 = v0;
       CE_TILE(mtv, MT,
-              hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::LOGIT, PD, false, false, MT, kNT, kDz, f16>),
-                                 dim3(width / MT * tn), dim3(256), 0, st, W, Xl, width / MT, tn, (int)(k.kp / BK), 0, 1, 0, e));
-      if (dx) {
-        Epilogue s = {};
-        s.scal = scal;
-        s.slab = (float*)(wb + b.dx_slab);
-        s.slab_stride = b.dx_rows * b.ld;
-        s.ld_slab = b.ld;
-        s.accumulate = piece > 0;
-        CE_TILE(mtd, MT,
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, false, MT, kNT, kSlab, f16>),
-                                   dim3(dt * tn * b.dx_splits), dim3(256), 0, st, W, D, dt, tn, (rows + BK - 1) / BK, b.dx_per, 1, 0, s));
-      }
+              hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_logits_kernel<f16, X::LOGIT, PD, MT, kNT, kDz>), dim3(width / MT * tn), dim3(256), 0,
+                                 st, W, Xl, width / MT, tn, (int)(k.kp / BK), e));
+      Grads g = {};
+      g.w = W;
+      g.x = Xw;
+      g.dz = D;
+      g.dt = dt;
+      g.dw.scal = g.dx.scal = scal;
+      g.dw.ld_slab = g.dx.ld_slab = b.ld;
       if (dw) {
-        Epilogue s = {};
-        s.scal = scal;
-        s.slab = (float*)(wb + b.dw_slab);
-        s.slab_stride = b.dw_rows * b.ld;
-        s.ld_slab = b.ld;
-        T* dw0 = (T*)dw + (long long)v0 * d;
-        s.out = dw0;
-        s.out_rows = rows;
-        s.d = d;
-        s.reduction = reduction;
-        s.gout = gout;
-        const int vt = (rows + kNT - 1) / kNT;
-        if (b.dw_splits == 1) {
-          CE_TILE(mtd, MT,
-                  hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, MT, kNT, kOut, T>), dim3(dt * vt),
-                                     dim3(256), 0, st, Xw, D, dt, vt, 0, 0, 0, 1, s));
-        } else {
-          CE_TILE(mtd, MT,
-                  hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_gemm_kernel<f16, X::GRAD, 1, true, true, MT, kNT, kSlab, f16>),
-                                     dim3(dt * vt * b.dw_splits), dim3(256), 0, st, Xw, D, dt, vt, 0, b.dw_per, 0, 1, s));
-          hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dw_kernel<T>), dim3((unsigned)(((long long)rows * ((d + 3) / 4) + 63) / 64)), dim3(256),
-                             0, st, rows, d, b.dw_splits, s.slab, s.slab_stride, b.ld, gout, reduction, scal, dw0);
-        }
+        g.dw_tn = (rows + kNT - 1) / kNT;
+        g.dw_wgs = dt * g.dw_tn * b.dw_splits;
+        g.dw_per = b.dw_splits > 1 ? b.dw_per : 0;
+        g.dw.slab = (float*)(wb + b.dw_slab) + v0 * b.ld;
+        g.dw.slab_stride = b.dw_rows * b.ld;
+        g.dw.out = (T*)dw + (long long)v0 * d;
+        g.dw.out_rows = rows;
+        g.dw.d = d;
+        g.dw.reduction = reduction;
+        g.dw.gout = gout;
+      }
+      if (dx) {
+        g.dx_tn = tn;
+        g.dx_wgs = dt * tn * b.dx_splits;
+        g.dx_per = b.dx_per;
+        g.dx_steps = (rows + BK - 1) / BK;
+        g.dx.slab = (float*)(wb + b.dx_slab);
+        g.dx.slab_stride = b.dx_rows * b.ld;
+        g.dx.accumulate = piece > 0;
       }
       if (db) {
-        float* col = (float*)(wb + b.col);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_colsum_kernel<PD>), dim3(width / 32, b.chunks), dim3(256), 0, st, dz, dz + dzplane,
-                           k.np * 64, width, weighted && !folded ? gout : nullptr, rowmap, scal, b.chunk, col);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_db_kernel<T>), dim3((rows + 255) / 256), dim3(256), 0, st, rows, width, b.chunks, col, gout,
-                           reduction, folded, scal, (T*)db + v0);
+        g.col_units = width / 32;
+        g.chunk = b.chunk;
+        g.col_weights = weighted && !folded ? gout : nullptr;
+        g.rowmap = rowmap;
+        g.col = (float*)(wb + b.col) + v0;
+        g.col_ld = k.vp;
       }
+      const int wgs = ((g.dw_wgs + 7) & ~7) + ((g.dx_wgs + 7) & ~7) + g.col_units * b.chunks;
+      if (b.dw_splits == 1)
+        CE_TILE(mtd, MT,
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_grads_kernel<X::GRAD, PD, MT, kNT, kOut, T>), dim3(wgs), dim3(256), 0, st, g));
+      else
+        CE_TILE(mtd, MT,
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_grads_kernel<X::GRAD, PD, MT, kNT, kSlab, T>), dim3(wgs), dim3(256), 0, st, g));
     }
-    if (dx)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_dx_kernel<T>), dim3((unsigned)((n * ((d + 3) / 4) + 255) / 256)), dim3(256), 0, st, (int)n, d,
-                         b.dx_splits, (const float*)(wb + b.dx_slab), b.dx_rows * b.ld, b.ld, inverse, gout, reduction, folded, scal,
-                         (T*)dx);
+    Final f = {};
+    f.n = (int)n;
+    f.d = d;
+    f.v = v;
+    f.reduction = reduction;
+    f.folded = folded;
+    f.gout = gout;
+    f.scal = scal;
+    f.inverse = inverse;
+    f.dx_slab = (float*)(wb + b.dx_slab);
+    f.dx_stride = b.dx_rows * b.ld;
+    f.ld = b.ld;
+    f.dx_splits = b.dx_splits;
+    f.dw_slab = (float*)(wb + b.dw_slab);
+    f.dw_stride = b.dw_rows * b.ld;
+    f.dw_splits = b.dw_splits;
+    f.col = (float*)(wb + b.col);
+    f.col_ld = k.vp;
+    f.chunks = b.chunks;
+    f.dx = dx;
+    f.dw = dw;
+    f.db = db;
+    const long long per = (d + 3) / 4;
+    f.dx_wgs = dx ? (unsigned)((n * per + 255) / 256) : 0;
+    f.dw_wgs = dw && b.dw_splits > 1 ? (unsigned)((v * per + 63) / 64) : 0;
+    const unsigned final_wgs = f.dx_wgs + f.dw_wgs + (db ? (unsigned)((v + 255) / 256) : 0);
+    if (final_wgs) hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_final_kernel<T>), dim3(final_wgs), dim3(256), 0, st, f);
   });
   return launch_status();
 }
