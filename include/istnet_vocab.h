@@ -56,7 +56,7 @@ ISTNET_PN2_API int istnet_distill_backward(long long n, int v, int k, int dtype,
  * Rows whose target is `ignore` do not count (loss 0; they are not looked at); any other target outside [0, v) makes the row NaN.
  * The logits are formed piece by piece and never kept.  keep (istnet_linear_ce_keep_kib, for the same w and ldw) carries the packed
  * operands and row statistics from the forward to the backward of the same call; train == 0: there will be none.  ws
- * (istnet_linear_ce_scratch_kib) is scratch.  n <= 2^22, d <= 2^20, v <= 2^28, n v <= 2^38. */
+ * (istnet_linear_ce_scratch_kib) is scratch.  n <= 2^22, d <= 2^20, v <= 2^28, n v <= 2^38, n d and v d <= 2^33. */
 ISTNET_PN2_API int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, int train, const void *w, long long ldw);
 ISTNET_PN2_API int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward);
 ISTNET_PN2_API int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, int train, const void *x,

@@ -601,7 +601,7 @@ __device__ __forceinline__ float scale_for(float amax) {      // power of two th
   if (!(amax > 0.f) || amax > 3.4e38f) return 1.f;
   int ex;
   frexpf(amax, &ex);                                          // amax = f 2^ex, f in [1/2, 1)
-  return ldexpf(1.f, max(-126, min(126, 15 - ex)));
+  return ldexpf(1.f, min(100, 15 - ex));                      // (100: what is divided out again stays a normal number)
 }
 
 __device__ __forceinline__ void store_scalars(float* scal, int count, float sx, float sw) {
@@ -868,13 +868,16 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(int mean, const float* _
   }
 }
 
-// largest |g| over the counted rows (weights of the rows' losses)
+// largest finite |g| over the counted rows (weights of the rows' losses)
 __global__ __launch_bounds__(1024) void ce_gmax_kernel(const float* __restrict__ gout, const int* __restrict__ rowmap,
                                                        float* __restrict__ scal) {
   __shared__ float tmp[16];
   const int count = (int)scal[kCount];
   float m = 0.f;
-  for (int i = threadIdx.x; i < count; i += 1024) m = fmaxf(m, fabsf(gout[rowmap[i]]));
+  for (int i = threadIdx.x; i < count; i += 1024) {
+    const float g = fabsf(gout[rowmap[i]]);
+    m = g < INFINITY ? fmaxf(m, g) : m;      // a row of weight infinity spoils itself, not the others
+  }
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = m;
   __syncthreads();
@@ -969,8 +972,13 @@ __global__ __launch_bounds__(256) void ce_final_kernel(Final f) {
 // ---- sizes and launches ------------------------------------------------------------------------------------------------------
 
 constexpr int kNT = 128;
-// the other side of a tile: 256, or less where that covers the classes / the features with less to spare
-inline int tile_v(int v) { return v <= 64 ? 64 : v <= 128 ? 128 : 256; }
+// The other side of a tile: 256, or less where that covers the classes / the features with less to spare -- or where the tiles are no
+// more than half the compute units: a step of a tile of 64 takes 0.34 us when it has a unit to itself, one of 256 takes 0.55 us.
+inline int tile_v(long long n, int v) {
+  int t = v <= 64 ? 64 : v <= 128 ? 128 : 256;
+  while (t > 64 && (n + 127) / 128 * ((v + t - 1) / t) <= 128) t /= 2;
+  return t;
+}
 inline int tile_d(int d) { return d <= 64 ? 64 : (d + 127) / 128 * 128 < (d + 255) / 256 * 256 ? 128 : 256; }
 #define CE_TILE(size, MT, ...)                                    \
   do {                                                            \
@@ -981,12 +989,13 @@ inline int tile_d(int d) { return d <= 64 ? 64 : (d + 127) / 128 * 128 < (d + 25
 constexpr long long kPieceBytes = 512ll << 20;           // memory of one piece of p - t
 constexpr int kMostSplits = 128;
 constexpr int kScanWgs = 2048;                           // workgroups at most that look for the largest entry of x, and of w
-constexpr double kSmallProducts = 1 << 26;
+constexpr long long kSmallSide = 1024, kSmallProducts = 1 << 28;      // see linear_ce_small.hip
 
 inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
 inline bool ce_ok(long long n, int d, int v, int dtype) {
   return n >= 1 && n <= (1ll << 22) && d >= 1 && d <= (1 << 20) && v >= 1 && v <= (1 << 28) && dtype >= 0 && dtype <= 2 &&
-         ((n + 127) / 128) * ((v + 255ll) / 256) <= (1ll << 23);      // a launch holds fewer than 2^32 threads
+         // a launch holds fewer than 2^32 threads
+         ((n + 127) / 128) * ((v + 255ll) / 256) <= (1ll << 23) && n * d <= (1ll << 33) && (long long)v * d <= (1ll << 33);
 }
 // Without a backward and for few rows, 16-bit rows of w are read as they lie: packing them costs three passes over w (81 us of
 // 65536 x 1024), which the products of panels win back from about 4000 rows on.
@@ -994,9 +1003,9 @@ inline bool direct_w(long long n, int d, int dtype, int train, const void* w, lo
   return !train && n <= 4096 && dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
 }
 
-// Problems that the four launches of linear_ce_small.hip serve: see there.
+// Problems that the four launches of linear_ce_small.hip serve.
 inline bool small_ce(long long n, int d, int v) {
-  return n <= 4096 && v <= 4096 && n * v <= (1ll << 21) && (double)n * v * d <= kSmallProducts;
+  return n <= kSmallSide && v <= kSmallSide && n * v * d <= kSmallProducts;
 }
 
 struct Keep {      // what the backward needs, in the caller's `keep`
@@ -1008,7 +1017,7 @@ inline Keep keep_plan(long long n, int d, int v, int dtype, bool direct) {
   k.planes = dtype == ISTNET_VOCAB_F32 ? 2 : 1;
   k.np = round_up(n, kPad) + kPad;      // zeros are written up to the next whole tile behind the last row
   k.kp = round_up(d, BK);
-  k.vp = round_up(v, tile_v(v));
+  k.vp = round_up(v, tile_v(n, v));
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
   k.xp = take(2 * k.planes * k.np * k.kp);
@@ -1023,9 +1032,9 @@ inline Keep keep_plan(long long n, int d, int v, int dtype, bool direct) {
   return k;
 }
 struct Forward { long long part, zt, loss, blocks, amax, bytes; int tiles; };
-inline Forward forward_plan(const Keep& k, int v) {
+inline Forward forward_plan(const Keep& k, long long n, int v) {
   Forward f = {};
-  f.tiles = (int)(k.vp / tile_v(v));
+  f.tiles = (int)(k.vp / tile_v(n, v));
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
   f.part = take(8ll * f.tiles * k.np);
@@ -1043,16 +1052,19 @@ struct Backward {
 inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtype, int reduction) {
   Backward b = {};
   const long long planes = dtype == ISTNET_VOCAB_BF16 ? 1 : 2;      // of p - t
-  const int mtv = tile_v(v);
+  const int mtv = tile_v(n, v);
   b.ld = round_up(d, tile_d(d));
   const long long dt = b.ld / tile_d(d), seg = dtype == ISTNET_VOCAB_F32 ? 3 : planes;
   // As few rounds of 512 workgroups for dw over all pieces as pieces of that memory allow, and as few pieces as that takes: 65536 classes
   // of 1024 features are four pieces of one full round each, not three of a round and a third.
-  const long long most = std::max<long long>(mtv, kPieceBytes / (2 * planes * k.np) / mtv * mtv), least = (k.vp + most - 1) / most;
+  // A piece is whole tiles of both products, unless it is the only one: what dw writes of it must not reach into the next.
+  const long long unit = std::max(mtv, kNT), most = std::max<long long>(unit, kPieceBytes / (2 * planes * k.np) / unit * unit);
+  const long long least = (k.vp + most - 1) / most;
   long long best = -1;
   for (long long p = least; p <= least + 3; ++p) {
-    const long long piece = round_up((k.vp + p - 1) / p, mtv), full = v / piece, rest = v - full * piece;
-    const long long rounds = full * ((dt * (piece / kNT) + 511) / 512) + (dt * ((rest + kNT - 1) / kNT) + 511) / 512;
+    const long long piece = p == 1 ? k.vp : round_up((k.vp + p - 1) / p, unit), full = v / piece, rest = v - full * piece;
+    const auto rounds_of = [&](long long classes) { return (dt * ((classes + kNT - 1) / kNT) + 511) / 512; };
+    const long long rounds = full * rounds_of(piece) + (rest ? rounds_of(rest) : 0);
     if (best < 0 || rounds < best) {
       best = rounds;
       b.piece = piece;
@@ -1069,6 +1081,7 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtyp
   b.dx_splits = (int)splits(dt * (b.dx_rows / kNT), dx_steps);
   b.dx_per = (int)((dx_steps + b.dx_splits - 1) / b.dx_splits);
   b.dw_splits = (int)splits(dt * ((most_rows + kNT - 1) / kNT), dw_steps);
+  if ((long long)v * d > (1ll << 28)) b.dw_splits = 1;      // joining the slabs of that many rows would not be one launch
   b.dw_per = (int)((dw_steps + b.dw_splits - 1) / b.dw_splits);
   b.chunk = (int)std::max<long long>(256, round_up((n + 127) / 128, 64));      // rows of one part of a bias gradient: 128 parts at most
   b.chunks = (int)((n + b.chunk - 1) / b.chunk);
@@ -1105,7 +1118,7 @@ extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
   if (small_ce(n, d, v)) return 0;
   const Keep k = keep_plan(n, d, v, dtype, false);
-  return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k, v).bytes) + 1023) / 1024);
+  return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k, n, v).bytes) + 1023) / 1024);
 }
 
 extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, int idx64, int train, const void* x, long long ldx,
@@ -1118,7 +1131,7 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
     return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, st);
   const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
-  const Forward f = forward_plan(k, v);
+  const Forward f = forward_plan(k, n, v);
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = direct ? nullptr : kb + k.wp;
   float *scal = (float*)(kb + k.scal), *bias2 = (float*)(kb + k.bias2), *zt = (float*)(wb + f.zt);
   float *amax = (float*)(wb + f.amax), *packed_loss = (float*)(wb + f.loss), *row_loss = reduction == 0 ? loss : nullptr;
@@ -1158,7 +1171,7 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
                                            (const float*)amax, (const int*)blocks, scal, xp, k.np, wp, bias2, rowmap, inverse, tgt, row_loss);
     };
     const auto product = [&](auto m) {
-      CE_TILE(tile_v(v), MT,
+      CE_TILE(tile_v(n, v), MT,
               hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_logits_kernel<decltype(m), X::LOGIT, 1, MT, kNT, kLse>), dim3(f.tiles * tn),
                                  dim3(256), 0, st, A, B, f.tiles, tn, (int)(k.kp / BK), e));
     };
@@ -1192,7 +1205,7 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = kb + k.wp, *dz = wb + b.dz, *xb = xp;
   float* scal = (float*)(kb + k.scal);
   int *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse);
-  const int tn = (int)((n + kNT - 1) / kNT), mtv = tile_v(v), mtd = tile_d(d), dt = (int)(b.ld / mtd);
+  const int tn = (int)((n + kNT - 1) / kNT), mtv = tile_v(n, v), mtd = tile_d(d), dt = (int)(b.ld / mtd);
   // weights of the rows' losses: taken into the rows of x that dw is formed from, which rounds them once more to 22 bits (float32) or
   // 11 (bfloat16); for float16 that would be the result's own precision, there they are taken into p - t
   const bool weighted = reduction == 0, folded = weighted && dtype == ISTNET_VOCAB_F16;

@@ -16,7 +16,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 struct __attribute__((packed, aligned(2))) Raw8 { u32x2 v; };
 
 constexpr float kNaN = __builtin_nanf("");
-constexpr int kWaves = 8, kTM = 64, kTN = 32;      // tile of a workgroup: every wave has all of it for its part of K
+constexpr int kWaves = 16, kTM = 64, kTN = 32;      // tile of a workgroup: every wave has all of it for its part of K
 constexpr int kPitch = kTM + 4;
 
 // four elements from p, those at or behind `left` as zeros
@@ -82,6 +82,7 @@ __device__ __forceinline__ f32x4 join(const Tile& t, float* lds) {
     }
   __syncthreads();
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (threadIdx.x >= kTM * kTN / 4) return s;
   const float* at = lds + (threadIdx.x >> 4) * kPitch + (threadIdx.x & 15) * 4;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(64 * kWaves) void ce_small_logits_kernel(int n, int
   });
   const f32x4 s = join(t, lds);
   const int r = n0 + (threadIdx.x >> 4), c = v0 + (threadIdx.x & 15) * 4;
-  if (r < n && c < vp) {
+  if (threadIdx.x < kTM * kTN / 4 && r < n && c < vp) {
     f32x4 y = s;
     if (bias) {
 #pragma unroll
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves) void ce_small_grads_kernel(int n, int 
     }
     const f32x4 s = join(t, lds);
     const int r = c0 + (threadIdx.x >> 4), c = d0 + (threadIdx.x & 15) * 4;
-    if (r < (is_dx ? n : v)) {
+    if (threadIdx.x < kTM * kTN / 4 && r < (is_dx ? n : v)) {
       const float g = is_dx ? (reduction == 0 ? (on[r] ? gout[r] : 0.f) : on[r] ? whole : 0.f) : whole;
       T* out = (is_dx ? dx : dw) + (long long)r * d;
 #pragma unroll

@@ -127,7 +127,8 @@ def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, r
     n = x.shape[0]
     if features.is_cuda and n:
         vn.check_float(features, "features")
-        if n > 1 << 22 or d > 1 << 20 or v > 1 << 28 or -(-n // 128) * -(-v // 256) > 1 << 23:
+        if (n > 1 << 22 or d > 1 << 20 or v > 1 << 28 or -(-n // 128) * -(-v // 256) > 1 << 23 or n * d > 1 << 33
+                or v * d > 1 << 33):
             raise ValueError(f"{n} rows of {d} features and {v} classes are too many for one call")
         train = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
         loss = vn.LinearCEFunction.apply(x, weight, bias, t, ignore_index, vn.REDUCTIONS[reduction], train)
