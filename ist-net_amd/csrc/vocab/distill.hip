@@ -127,7 +127,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k
     if (tid == 0) { stats[2 * row] = 0.f; stats[2 * row + 1] = -1.f; row_loss[row] = 0.f; }
     return;
   }
-  // rows short enough for one wave are looked at once more (they are in the caches); in longer ones the rest is no small number
+  // rows short enough for one wave are looked at once more (they are in the caches); longer ones keep the rounding of 1 + rest, 2^-24
   const float rest = fabsf(st.m) == INFINITY ? kNaN : THREADS == 64 && v <= kShortRow ? rest_of_row<T, THREADS>(z, v, st.m, kLog2e / temp, tmp)
                                                                                 : st.s - 1.f;
   float tm = -INFINITY, bad = 0.f;
@@ -145,6 +145,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k
   }
   bad = block_max<THREADS>(bad, tmp);
   tm = block_max<THREADS>(tm, tmp);
+  if (fabsf(tm) == INFINITY) bad = 1.f;      // no softmax of the teacher's
   float ts = 0.f;
   for (int j = tid; j < k; j += THREADS) ts += lidx[j] >= 0 ? expf(lq[j] - tm) : 0.f;
   ts = block_sum<THREADS>(ts, tmp);
@@ -221,6 +222,7 @@ __global__ __launch_bounds__(1024) void distill_total_kernel(long long n, int me
                                                              float* __restrict__ count) {
   __shared__ double tmp[2][16];
   double sum = 0.0, rows = 0.0;
+#pragma unroll 8
   for (long long i = threadIdx.x; i < n; i += 1024) {
     sum += row_loss[i];
     rows += stats[2 * i + 1] == -1.f ? 0.0 : 1.0;
@@ -303,8 +305,8 @@ inline DistillPlan distill_plan(long long n, int v, int elt) {
   return p;
 }
 inline bool distill_ok(long long n, int v, int k) {
-  // a launch holds fewer than 2^32 threads
-  return n >= 1 && n <= (1ll << 23) && v >= 1 && v < 0x7fffffff - 65536 && k >= 1 && k <= kMaxSlots;
+  // a launch holds fewer than 2^32 threads, and the end of a row's last part is an int: parts take up to 2048 x 4096 bytes too many
+  return n >= 1 && n <= (1ll << 23) && v >= 1 && v <= 0x7fffffff - (1 << 24) && k >= 1 && k <= kMaxSlots;
 }
 
 }  // namespace

@@ -154,26 +154,30 @@ __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(int n, int v, 
   for (int d = threadIdx.x; d < radix; d += kSortThreads) hist[nb <= kFewBlocks ? (long long)b * radix + d : (long long)d * nb + b] = cnt[d];
 }
 
-__global__ __launch_bounds__(1024) void embed_scan_kernel(long long count, int* __restrict__ hist) {
-  __shared__ int tmp[16];
+// many workgroups: workgroup d scans its digit's counts over the workgroups of the sort; the digits' totals follow behind all counts
+// (64 M tokens: one workgroup over all counts was the longest kernel of the sort)
+__global__ __launch_bounds__(256) void embed_scan_kernel(int nb, int* __restrict__ hist) {
+  __shared__ int tmp[4];
+  int* mine = hist + (long long)blockIdx.x * nb;
   int carry = 0;
-  for (long long base = 0; base < count; base += 4096) {
-    const long long i = base + 4 * threadIdx.x;
+  for (int base = 0; base < nb; base += 1024) {
+    const int i = base + 4 * threadIdx.x;
     int x[4], sum = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[j] = i + j < count ? hist[i + j] : 0;
+      x[j] = i + j < nb ? mine[i + j] : 0;
       sum += x[j];
     }
     int all;
-    int at = carry + block_exclusive<1024>(sum, tmp, &all);
+    int at = carry + block_exclusive<256>(sum, tmp, &all);
     carry += all;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (i + j < count) hist[i + j] = at;
+      if (i + j < nb) mine[i + j] = at;
       at += x[j];
     }
   }
+  if (threadIdx.x == 0) hist[(long long)gridDim.x * nb + blockIdx.x] = carry;
 }
 
 __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int v, const void* __restrict__ ids, int idx64,
@@ -201,36 +205,32 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int 
   }
   __syncthreads();
   constexpr int PER = (1 << kDigit) / kSortThreads;      // digits of a thread: PER consecutive ones
-  int at[PER];
-  if (nb <= kFewBlocks) {
-    int before[PER] = {}, total[PER] = {};
+  int at[PER], before[PER] = {}, total[PER] = {};
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = threadIdx.x * PER + j;
-      if (d < radix) {
+  for (int j = 0; j < PER; ++j) {
+    const int d = threadIdx.x * PER + j;
+    if (d < radix) {
+      if (nb <= kFewBlocks) {
 #pragma unroll 8
         for (int o = 0; o < nb; ++o) {
           const int c = hist[(long long)o * radix + d];
           total[j] += c;
           before[j] += o < b ? c : 0;
         }
+      } else {
+        total[j] = hist[(long long)radix * nb + d];
+        before[j] = hist[(long long)d * nb + b];
       }
     }
-    int mine = 0, all;
+  }
+  int mine = 0, all;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) mine += total[j];
-    int from = block_exclusive<kSortThreads>(mine, tmp, &all);
+  for (int j = 0; j < PER; ++j) mine += total[j];
+  int from = block_exclusive<kSortThreads>(mine, tmp, &all);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      at[j] = from + before[j];
-      from += total[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = threadIdx.x * PER + j;
-      at[j] = d < radix ? hist[(long long)d * nb + b] : 0;
-    }
+  for (int j = 0; j < PER; ++j) {
+    at[j] = from + before[j];
+    from += total[j];
   }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -542,6 +542,9 @@ inline bool embed_ok(long long n, int v, int d, int dtype) {
   return n >= 1 && n <= (1ll << 30) && v >= 1 && v < 0x7fffffff - 256 && d >= 1 && dtype >= 0 && dtype <= 2;
 }
 
+// a table of more rows takes more workgroups of embed_few_kernel than one launch may hold
+inline bool embed_few(long long n, int v) { return n <= kFewTokens && v <= (1 << 28); }
+
 struct EmbedPlan {
   int bits, passes, items, nb, longest, pieces;
   long long keys[2], perm[2], hist, start, part, bytes;      // offsets into the scratch memory
@@ -560,7 +563,7 @@ inline EmbedPlan embed_plan(long long n, int v, int d) {
   auto take = [&](long long bytes) { const long long o = at; at += (bytes + 255) / 256 * 256; return o; };
   const bool small = n <= kSmallSort;
   for (int i = 0; i < (small ? 1 : 2); ++i) { p.keys[i] = take(4 * n); p.perm[i] = take(4 * n); }
-  p.hist = small ? 0 : take(4ll * p.nb << p.bits);
+  p.hist = small ? 0 : take(4ll * (p.nb + 1) << p.bits);
   p.start = take(4ll * (v + 1ll));
   p.part = p.pieces ? take(8ll * p.pieces * ((d + 7) / 8 * 8)) : 0;
   p.bytes = at;
@@ -581,16 +584,16 @@ extern "C" int istnet_embed_forward(long long n, int v, int d, int dtype, int id
 
 extern "C" int istnet_embed_scratch_kib(long long n, int v, int d) {
   if (!embed_ok(n, v, d, 0)) return -1;
-  if (n <= kFewTokens) return 0;
+  if (embed_few(n, v)) return 0;
   return (int)((embed_plan(n, v, d).bytes + 1023) / 1024);
 }
 
 extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int idx64, const void* grad, long long ldg,
                                      const void* ids, long long padding, float scale, void* ws, void* dw, void* stream) {
-  if (!embed_ok(n, v, d, dtype) || !grad || !ids || (!ws && n > kFewTokens) || !dw || ldg < d) return ISTNET_PN2_EINVAL;
+  if (!embed_ok(n, v, d, dtype) || !grad || !ids || (!ws && !embed_few(n, v)) || !dw || ldg < d) return ISTNET_PN2_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
   const int ll = lanes_log_of(d, dtype);
-  if (n <= kFewTokens) {
+  if (embed_few(n, v)) {
     // rows per workgroup: enough workgroups for the chip, few enough that reading all indices in each of them stays cheap
     const int rows = v <= 4096 ? 16 : kFewRows;
     VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_few_kernel<T>), dim3((unsigned)((v + rows - 1ll) / rows)), dim3(256),
@@ -616,7 +619,7 @@ extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int i
       hipLaunchKernelGGL(embed_hist_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, i * p.bits,
                          p.bits, p.items, p.nb, hist);
       if (p.nb > kFewBlocks)
-        hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, st, (long long)p.nb << p.bits, hist);
+        hipLaunchKernelGGL(embed_scan_kernel, dim3(1u << p.bits), dim3(256), 0, st, p.nb, hist);
       hipLaunchKernelGGL(embed_scatter_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, pin,
                          i * p.bits, p.bits, p.items, p.nb, hist, keys[to], perm[to]);
       last = to;

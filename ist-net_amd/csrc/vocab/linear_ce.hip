@@ -552,8 +552,8 @@ __device__ __forceinline__ bool row_counts(const void* target, long long i, int 
   return load_index(target, i, idx64) != ignore;
 }
 
-// Workgroups [0, xwgs): the largest magnitude of the rows of x that count; [xwgs, xwgs + wwgs): of w (infinities as they come, NaN
-// passed over), one value per workgroup; the rest: counted rows per block of 256.  A wave has four rows' loads in flight.
+// Workgroups [0, xwgs): the largest finite magnitude of the rows of x that count (what is not finite spoils its own row, not the scale
+// of the others); [xwgs, xwgs + wwgs): of w, one value per workgroup; the rest: counted rows per block of 256.  A wave has four rows' loads in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_scan_kernel(int n, int v, int d, const T* __restrict__ x, long long ldx,
                                                       const T* __restrict__ w, long long ldw, const void* __restrict__ target,
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(256) void ce_scan_kernel(int n, int v, int d, const
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) m = on[j] ? fmaxf(m, fabsf(f[j][i])) : m;
+        for (int i = 0; i < kVec<T>; ++i) m = on[j] && fabsf(f[j][i]) < INFINITY ? fmaxf(m, fabsf(f[j][i])) : m;
     }
   }
   m = wave_max(m);
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256) void ce_scan_kernel(int n, int v, int d, const
 }
 
 __device__ __forceinline__ float scale_for(float amax) {      // power of two that takes amax to [2^14, 2^15)
-  if (!(amax > 0.f) || amax > 3.4e38f) return 1.f;
+  if (!(amax > 0.f)) return 1.f;
   int ex;
   frexpf(amax, &ex);                                          // amax = f 2^ex, f in [1/2, 1)
   return ldexpf(1.f, min(100, 15 - ex));                      // (100: what is divided out again stays a normal number)
@@ -856,7 +856,7 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(int mean, const float* _
   __shared__ double tmp[16];
   const int count = (int)scal[kCount];
   double sum = 0.0;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = threadIdx.x; i < count; i += 1024) sum += packed_loss[i];
   sum = wave_sum(sum);
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = sum;
@@ -869,14 +869,14 @@ __global__ __launch_bounds__(1024) void ce_total_kernel(int mean, const float* _
 }
 
 // largest finite |g| over the counted rows (weights of the rows' losses)
-__global__ __launch_bounds__(1024) void ce_gmax_kernel(const float* __restrict__ gout, const int* __restrict__ rowmap,
+__global__ __launch_bounds__(1024) void ce_gmax_kernel(int n, const float* __restrict__ gout, const int* __restrict__ inverse,
                                                        float* __restrict__ scal) {
   __shared__ float tmp[16];
-  const int count = (int)scal[kCount];
   float m = 0.f;
-  for (int i = threadIdx.x; i < count; i += 1024) {
-    const float g = fabsf(gout[rowmap[i]]);
-    m = g < INFINITY ? fmaxf(m, g) : m;      // a row of weight infinity spoils itself, not the others
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float g = fabsf(gout[i]);
+    m = inverse[i] >= 0 && g < INFINITY ? fmaxf(m, g) : m;      // a row of weight infinity spoils itself, not the others
   }
   m = wave_max(m);
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = m;
@@ -1209,7 +1209,7 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   // weights of the rows' losses: taken into the rows of x that dw is formed from, which rounds them once more to 22 bits (float32) or
   // 11 (bfloat16); for float16 that would be the result's own precision, there they are taken into p - t
   const bool weighted = reduction == 0, folded = weighted && dtype == ISTNET_VOCAB_F16;
-  if (weighted) hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, st, gout, rowmap, scal);
+  if (weighted) hipLaunchKernelGGL(ce_gmax_kernel, dim3(1), dim3(1024), 0, st, (int)n, gout, inverse, scal);
   VOCAB_DISPATCH(dtype, T, {
     typedef Matrix<T> X;
     constexpr int P = X::P, PD = X::PD;

@@ -3,7 +3,7 @@
 //
 // Four launches: the logits (kept: a few megabytes here), row statistics and p - t in their place, the loss, and ONE launch for dx, dw
 // and db.  Products on the float32 matrix instructions (v_mfma_f32_32x32x2_f32), operands straight from memory into registers whatever
-// their type, stride or alignment; eight waves split K and join through LDS in a fixed order.  Everything is float32, rounded once.
+// their type, stride or alignment; sixteen waves split K and join through LDS in a fixed order.  Everything is float32, rounded once.
 #include <algorithm>
 
 #include "vocab_common.h"
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void ce_small_rows_kernel(int n, int v, int vp
     at_target = d == -INFINITY ? -1.f : -1.f + 0.f * loss;
     top = m;
   } else {
-    const float rest = d > 0.f ? s * expf(-d) : s / expf(d);
+    const float rest = d == INFINITY ? kNaN : d > 0.f ? s * expf(-d) : s / expf(d);
     loss = log1pf(rest);
     at_target = -rest / (1.f + rest);
     top = fmaxf(m, zt);

@@ -49,14 +49,14 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
 
     float32 loss: per row ("none"), their "sum" or their "mean" over the rows that count.  Slots with index -1 are unused
     (their logits are not looked at); a row without a used slot does not count: loss 0, gradient 0, its logits are not looked at;
-    the mean over no row is NaN.  Slots may repeat a class.  A row with an index outside [-1, V) or with a NaN among its used
-    logits is NaN, loss and gradient.  Differentiable w.r.t. ``logits`` (once).  ``logits`` may be a slice with a row stride, of
+    the mean over no row is NaN.  Slots may repeat a class.  A row with an index outside [-1, V), with a NaN among its used
+    logits or without a finite largest one is NaN, loss and gradient.  T: 1e-4 to 1e4.  Differentiable w.r.t. ``logits`` (once).  ``logits`` may be a slice with a row stride, of
     float32, bfloat16 or float16; the gradient has its type, everything between is float32."""
     from . import vocab_native as vn
     vn.check_reduction(reduction)
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-4 <= temperature <= 1e4:
+        raise ValueError(f"temperature must be between 1e-4 and 1e4, got {temperature}")
     if (logits.dim() < 1 or top_index.dim() < 1 or logits.shape[:-1] != top_index.shape[:-1]
             or top_logits.shape != top_index.shape):
         raise ValueError(f"shapes do not agree: logits {tuple(logits.shape)}, top_logits {tuple(top_logits.shape)}, "
@@ -75,7 +75,7 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
     if logits.is_cuda and n:
         vn.check_float(logits, "logits")
         vn.check_float(top_logits, "top_logits")
-        if n > 1 << 23 or v >= 2 ** 31 - 65536:
+        if n > 1 << 23 or v >= 2 ** 31 - 2 ** 24:
             raise ValueError(f"{n} rows of {v} classes are too many for one call")
         loss = vn.DistillFunction.apply(z, top, idx, temperature, vn.REDUCTIONS[reduction])
     else:                                            # host: the definition as it is written

@@ -87,6 +87,21 @@ def test_distill_refusals():
         call(z, top.requires_grad_(), idx)
 
 
+@pytest.mark.parametrize("temperature", [1e-5, 1e5, 1e-40])
+def test_distill_refuses_temperatures_without_a_meaning_in_float32(temperature):
+    with pytest.raises(ValueError, match="temperature"):
+        losses.TopLogitsDistill(torch.randn(4, 10), torch.randn(4, 3), torch.zeros(4, 3, dtype=torch.int64), temperature)
+
+
+def test_distill_teachers_without_a_finite_largest_logit():
+    z = torch.randn(3, 6, dtype=torch.float64, requires_grad=True)
+    top = torch.tensor([[INF, 0.0], [-INF, -INF], [1.0, 2.0]], dtype=torch.float64)
+    rows = losses.TopLogitsDistill(z, top, torch.tensor([[0, 1], [2, 3], [4, 5]]), reduction="none")
+    rows.sum().backward()
+    assert rows.isnan().tolist() == [True, True, False]
+    assert z.grad[:2].isnan().all() and z.grad[2].isfinite().all()
+
+
 def test_distill_without_rows():
     z = torch.zeros(0, 5, requires_grad=True)
     top, idx = torch.zeros(0, 2), torch.zeros(0, 2, dtype=torch.int32)

@@ -261,6 +261,16 @@ def test_distill_rows_that_cannot_be_right_are_nan(v):
     assert dz[:5].isnan().all() and dz[5].isfinite().all()
 
 
+@pytest.mark.parametrize("v", [50, 9000])
+def test_distill_teachers_without_a_finite_largest_logit(v):
+    z, top, idx = _distill_inputs(4, v, 4, F32, v + 1)
+    top[0, 1], top[1] = INF, -INF
+    idx[1, 3] = -1
+    loss, dz = _check_distill(z, top, idx, 1.0, "none")
+    assert loss[:2].isnan().all() and loss[2:].isfinite().all()
+    assert dz[:2].isnan().all() and dz[2:].isfinite().all()
+
+
 def test_distill_mean_over_no_row():
     z, top, idx = _distill_inputs(5, 40, 3, F32, 1)
     z = z.detach().requires_grad_()
@@ -483,6 +493,42 @@ def test_linear_ce_rows_that_cannot_be_right_are_nan(dtype):
     assert losses.LinearCrossEntropy(x2, w, t.clamp(min=0, max=299), b, reduction="none").isnan()[0]
     none = losses.LinearCrossEntropy(x[:0], w, t[:0], b)
     assert none.isnan()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,d,v", [(12, 40, 300), (40, 64, 5000)])
+def test_linear_ce_infinite_features_spoil_their_own_row(n, d, v, dtype):
+    """float32 and bfloat16 rows share a scale: what is not finite must not become it."""
+    x, w, b, t = _ce_inputs(n, d, v, dtype, 24, ignored=0.0)
+    whole = x.detach().clone()
+    whole[3, 5], whole[7, 0] = INF, NAN
+    whole.requires_grad_()
+    others = [i for i in range(n) if i not in (3, 7)]
+    loss = losses.LinearCrossEntropy(whole, w, t, b, reduction="none")
+    gout = 0.5 + torch.rand(n, device=DEV, generator=_gen(13))
+    (dx,) = torch.autograd.grad(loss, whole, gout)
+    assert loss[7].isnan() and not loss[3].isfinite() and dx[7].isnan().all() and dx[3].isnan().any()
+    want, bound, (ref, gb, _), *_ = _ce_reference(x[others], w, b, t[others], "none", gout[others])
+    _within(loss[others], want, bound, "loss")
+    _within(dx[others], ref, gb, "dx")
+
+
+@pytest.mark.parametrize("n,v", [(6, 300), (40, 5000)])
+def test_linear_ce_infinite_logits(n, v):
+    """As in the definition: a target of +inf is NaN, a target that the bias excludes costs infinitely much."""
+    x, w, b, t = _ce_inputs(n, 32, v, F32, 25, ignored=0.0)
+    t[:] = torch.arange(n, device=DEV)
+    b[1], b[2] = INF, -INF
+    for rows in ([1], [2], [0, 2, 3]):
+        xr = x[rows].detach().requires_grad_()
+        bias = b.clone()
+        if 1 not in rows:
+            bias[1] = 0.0
+        loss = losses.LinearCrossEntropy(xr, w, t[rows], bias, reduction="none")
+        (dx,) = torch.autograd.grad(loss, xr, torch.ones_like(loss))
+        ref = torch.nn.functional.cross_entropy(x[rows].double() @ w.double().t() + bias.double(), t[rows], reduction="none")
+        assert torch.equal(loss.isnan(), ref.isnan()) and torch.equal(loss.isinf(), ref.isinf()), rows
+        assert torch.equal(dx.isfinite().all(1), ~ref.isnan())
 
 
 def test_linear_ce_large_logits_offsets_and_outliers():
@@ -713,6 +759,28 @@ def test_backward_twice_and_changed_operands():
         w.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(loss, (x, w))
+
+
+def test_few_indices_into_a_table_of_very_many_rows():
+    v = (1 << 28) + 3
+    table = torch.zeros(v, 1, device=DEV, dtype=BF16)
+    table[-2:] = 3.0
+    table.requires_grad_()
+    ids = torch.tensor([v - 1, 5, v - 2, v - 1], device=DEV)
+    out = pointnet2_utils.embedding_operation(table, ids, 2.0)
+    assert out.flatten().tolist() == [6.0, 0.0, 6.0, 6.0]
+    (dw,) = torch.autograd.grad(out, table, torch.tensor([[1.0], [2.0], [4.0], [8.0]], device=DEV, dtype=BF16))
+    assert dw[[v - 1, v - 2, 5], 0].tolist() == [18.0, 8.0, 4.0] and dw.count_nonzero() == 3
+
+
+@pytest.mark.parametrize("v", [40, 70000])
+def test_lookup_gradient_of_many_indices(v):
+    """More workgroups than one reads the digit counts of by itself, an odd number of them."""
+    n = 300_001
+    ids = torch.randint(0, v, (n,), device=DEV, generator=_gen(v))
+    ids[ids % 5 == 1] = 3
+    w = torch.zeros(v, 3, device=DEV)
+    _check_lookup(w, ids, 1.5, 7)
 
 
 def test_offsets_beyond_32_bits():
