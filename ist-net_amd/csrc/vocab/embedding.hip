@@ -19,7 +19,7 @@ constexpr int kSmallDigit = 6;        // bits of a digit there: 64 digits x 16 w
 constexpr int kDigit = 9;             // most bits of a digit of the sort over many workgroups
 constexpr int kSortThreads = 256;
 constexpr int kFewBlocks = 64;        // workgroups up to which the scatter adds up the digit counts of all of them (saves a launch)
-constexpr int kSortItems = 16;        // tokens per thread and workgroup of that sort
+constexpr int kFewItems = 4, kSortItems = 16;      // tokens per thread of that sort, up to 2^18 tokens and above
 
 __device__ __forceinline__ uint32_t key_of(const void* ids, long long i, int idx64, int v, long long padding) {
   const long long id = load_index(ids, i, idx64);
@@ -142,6 +142,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_hist_kernel(int n, int v, 
   for (int d = threadIdx.x; d < radix; d += kSortThreads) cnt[d] = 0;
   __syncthreads();
   const long long base = (long long)b * kSortThreads * items;
+#pragma unroll 4
   for (int r = 0; r < items; ++r) {
     const long long i = base + r * kSortThreads + threadIdx.x;
     if (i < n) {
@@ -180,46 +181,51 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(int nb, int* __restrict
   if (threadIdx.x == 0) hist[(long long)gridDim.x * nb + blockIdx.x] = carry;
 }
 
+template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int v, const void* __restrict__ ids, int idx64,
                                                                      long long padding, const uint32_t* __restrict__ keys_in,
-                                                                     const uint32_t* __restrict__ perm_in, int shift, int bits,
-                                                                     int items, int nb, const int* __restrict__ hist,
-                                                                     uint32_t* __restrict__ keys_out, uint32_t* __restrict__ perm_out) {
+                                                                     const uint32_t* __restrict__ perm_in, int shift, int bits, int nb,
+                                                                     const int* __restrict__ hist, uint32_t* __restrict__ keys_out,
+                                                                     uint32_t* __restrict__ perm_out) {
   constexpr int WAVES = kSortThreads / 64;
   __shared__ int cnt[WAVES][1 << kDigit];
   __shared__ int tmp[WAVES];
   const int radix = 1 << bits, b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int d = lane; d < radix; d += 64) cnt[wave][d] = 0;
   __syncthreads();
-  const long long first = ((long long)b * WAVES + wave) * 64 * items;
-  int rank[kSortItems];
-  uint32_t key[kSortItems];
+  const long long first = ((long long)b * WAVES + wave) * 64 * ITEMS;
+  int rank[ITEMS];
+  uint32_t key[ITEMS], from_token[ITEMS];
 #pragma unroll
-  for (int r = 0; r < kSortItems; ++r) {
-    if (r < items) {
-      const long long i = first + r * 64 + lane;
-      const bool active = i < n;
-      key[r] = active ? (keys_in ? keys_in[i] : key_of(ids, i, idx64, v, padding)) : 0u;
-      rank[r] = rank_and_count((key[r] >> shift) & (uint32_t)(radix - 1), bits, active, cnt[wave], lane);
-    }
+  for (int r = 0; r < ITEMS; ++r) {      // all loads on their way before the first is counted
+    const long long i = first + r * 64 + lane;
+    const bool active = i < n;
+    key[r] = active ? (keys_in ? keys_in[i] : key_of(ids, i, idx64, v, padding)) : 0u;
+    from_token[r] = active && perm_in ? perm_in[i] : (uint32_t)i;
   }
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r)
+    rank[r] = rank_and_count((key[r] >> shift) & (uint32_t)(radix - 1), bits, first + r * 64 + lane < n, cnt[wave], lane);
   __syncthreads();
   constexpr int PER = (1 << kDigit) / kSortThreads;      // digits of a thread: PER consecutive ones
+  static_assert(PER == 2, "the counts of a thread's digits are one load");
   int at[PER], before[PER] = {}, total[PER] = {};
+  const int d0 = threadIdx.x * PER;
+  if (d0 < radix) {      // radix is even
+    if (nb <= kFewBlocks) {
+#pragma unroll 16
+      for (int o = 0; o < nb; ++o) {
+        const int2 c = *reinterpret_cast<const int2*>(hist + (long long)o * radix + d0);
+        total[0] += c.x;
+        total[1] += c.y;
+        before[0] += o < b ? c.x : 0;
+        before[1] += o < b ? c.y : 0;
+      }
+    } else {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int d = threadIdx.x * PER + j;
-    if (d < radix) {
-      if (nb <= kFewBlocks) {
-#pragma unroll 8
-        for (int o = 0; o < nb; ++o) {
-          const int c = hist[(long long)o * radix + d];
-          total[j] += c;
-          before[j] += o < b ? c : 0;
-        }
-      } else {
-        total[j] = hist[(long long)radix * nb + d];
-        before[j] = hist[(long long)d * nb + b];
+      for (int j = 0; j < PER; ++j) {
+        total[j] = hist[(long long)radix * nb + d0 + j];
+        before[j] = hist[(long long)(d0 + j) * nb + b];
       }
     }
   }
@@ -246,12 +252,12 @@ __global__ __launch_bounds__(kSortThreads) void embed_scatter_kernel(int n, int 
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kSortItems; ++r) {
+  for (int r = 0; r < ITEMS; ++r) {
     const long long i = first + r * 64 + lane;
-    if (r < items && i < n) {
+    if (i < n) {
       const int pos = cnt[wave][(key[r] >> shift) & (uint32_t)(radix - 1)] + rank[r];
       keys_out[pos] = key[r];
-      perm_out[pos] = perm_in ? perm_in[i] : (uint32_t)i;
+      perm_out[pos] = from_token[r];
     }
   }
 }
@@ -300,12 +306,12 @@ constexpr int kTeamRows = 4;      // table rows per team of lanes
 
 // The rows of a team are far apart: frequent indices are often neighbours, and one team would have to add up several of them.
 template <typename T>
-__global__ __launch_bounds__(256) void embed_rows_kernel(int v, int d, int lanes_log, int longest, const T* __restrict__ grad,
-                                                         long long ldg, const uint32_t* __restrict__ perm,
-                                                         const int* __restrict__ start, float scale, T* __restrict__ dw) {
+__device__ __forceinline__ void sum_rows(long long wg, long long wgs, int v, int d, int lanes_log, int longest,
+                                         const T* __restrict__ grad, long long ldg, const uint32_t* __restrict__ perm,
+                                         const int* __restrict__ start, float scale, T* __restrict__ dw) {
   const int lanes = 1 << lanes_log, at = threadIdx.x & (lanes - 1);
-  const long long teams = (long long)gridDim.x << (8 - lanes_log);
-  for (long long row0 = ((long long)blockIdx.x << (8 - lanes_log)) + (threadIdx.x >> lanes_log); row0 < v; row0 += teams * kTeamRows) {
+  const long long teams = wgs << (8 - lanes_log);
+  for (long long row0 = (wg << (8 - lanes_log)) + (threadIdx.x >> lanes_log); row0 < v; row0 += teams * kTeamRows) {
     int s[kTeamRows], e[kTeamRows];
 #pragma unroll
     for (int r = 0; r < kTeamRows; ++r) {
@@ -347,11 +353,9 @@ __device__ __forceinline__ void join_teams(float (&acc)[kVec<T>], float* lds, in
 // Piece p holds sorted tokens [p L, (p + 1) L).  At most two runs longer than L touch it: the one of its first token (slot 0) and
 // the one of its last (slot 1, if that is another one).
 template <typename T>
-__global__ __launch_bounds__(256) void embed_pieces_kernel(int n, int v, int d, int lanes_log, int longest, const T* __restrict__ grad,
-                                                           long long ldg, const uint32_t* __restrict__ keys,
-                                                           const uint32_t* __restrict__ perm, const int* __restrict__ start,
-                                                           float* __restrict__ part) {
-  __shared__ float lds[256 * kVec<T>];
+__device__ __forceinline__ void sum_piece(float* lds, int n, int v, int d, int lanes_log, int longest, const T* __restrict__ grad,
+                                          long long ldg, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ perm,
+                                          const int* __restrict__ start, float* __restrict__ part) {
   const int lanes = 1 << lanes_log, teams = 256 >> lanes_log, at = threadIdx.x & (lanes - 1), team = threadIdx.x >> lanes_log;
   const int p0 = blockIdx.x * longest, p1 = min(n, p0 + longest);
   const uint32_t ka = keys[p0], kb = keys[p1 - 1];
@@ -374,6 +378,20 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(int n, int v, int d, 
       }
     }
   }
+}
+
+// Short runs and the pieces of long ones do not meet: one launch, the pieces first because one takes longer.  (32768 tokens of a table of
+// 65536 x 1024 bfloat16: 55 us for both, 48 and 15 us in launches of their own.)
+template <typename T>
+__global__ __launch_bounds__(256) void embed_sums_kernel(int n, int v, int d, int lanes_log, int longest, int pieces,
+                                                         const T* __restrict__ grad, long long ldg, const uint32_t* __restrict__ keys,
+                                                         const uint32_t* __restrict__ perm, const int* __restrict__ start, float scale,
+                                                         float* __restrict__ part, T* __restrict__ dw) {
+  __shared__ float lds[256 * kVec<T>];
+  if ((int)blockIdx.x < pieces)
+    sum_piece(lds, n, v, d, lanes_log, longest, grad, ldg, keys, perm, start, part);
+  else
+    sum_rows<T>(blockIdx.x - pieces, gridDim.x - pieces, v, d, lanes_log, longest, grad, ldg, perm, start, scale, dw);
 }
 
 // the run longer than L that STARTS in piece p (there is at most one, that of the piece's last token): its partial sums in order
@@ -554,7 +572,7 @@ inline EmbedPlan embed_plan(long long n, int v, int d) {
   const int key_bits = log2_ceil((long long)v + 1), most = n <= kSmallSort ? kSmallDigit : kDigit;
   p.passes = (key_bits + most - 1) / most;
   p.bits = (key_bits + p.passes - 1) / p.passes;
-  p.items = n <= 256 * 1024 ? 4 : kSortItems;
+  p.items = n <= 256 * 1024 ? kFewItems : kSortItems;
   p.nb = (int)((n + kSortThreads * p.items - 1) / (kSortThreads * p.items));
   // pieces short enough that one is a few rounds of loads, long enough that the partial sums of one row do not become many
   p.longest = std::max(32, (1 << ((log2_ceil(n) + 1) / 2)) / 8);
@@ -620,22 +638,20 @@ extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int i
                          p.bits, p.items, p.nb, hist);
       if (p.nb > kFewBlocks)
         hipLaunchKernelGGL(embed_scan_kernel, dim3(1u << p.bits), dim3(256), 0, st, p.nb, hist);
-      hipLaunchKernelGGL(embed_scatter_kernel, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, pin,
-                         i * p.bits, p.bits, p.items, p.nb, hist, keys[to], perm[to]);
+      const auto scatter = p.items == kFewItems ? embed_scatter_kernel<kFewItems> : embed_scatter_kernel<kSortItems>;
+      hipLaunchKernelGGL(scatter, dim3(p.nb), dim3(kSortThreads), 0, st, (int)n, v, ids, idx64, padding, kin, pin, i * p.bits, p.bits,
+                         p.nb, hist, keys[to], perm[to]);
       last = to;
     }
   }
   hipLaunchKernelGGL(embed_starts_kernel, dim3((unsigned)(v / 256 + 1)), dim3(256), 0, st, (int)n, v, keys[last], start);
   const long long rows = (256 >> ll) * (long long)kTeamRows, grid = std::min((v + rows - 1) / rows, kMaxGrid);
   VOCAB_DISPATCH(dtype, T, {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, st, v, d, ll, p.longest,
-                       (const T*)grad, ldg, perm[last], start, scale, (T*)dw);
-    if (p.pieces) {
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_pieces_kernel<T>), dim3(p.pieces), dim3(256), 0, st, (int)n, v, d, ll, p.longest,
-                         (const T*)grad, ldg, keys[last], perm[last], start, part);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_sums_kernel<T>), dim3((unsigned)(p.pieces + grid)), dim3(256), 0, st, (int)n, v, d, ll,
+                       p.longest, p.pieces, (const T*)grad, ldg, keys[last], perm[last], start, scale, part, (T*)dw);
+    if (p.pieces)
       hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_join_kernel<T>), dim3(p.pieces), dim3(256), 0, st, (int)n, v, d, ll, p.longest,
                          keys[last], start, part, scale, (T*)dw);
-    }
   });
   return launch_status();
 }
