@@ -679,6 +679,7 @@ __device__ __forceinline__ void pack8(const T* src, int left, float scale, u32x4
 template <typename T, int P, bool RAW>
 __device__ __forceinline__ void pack_rows(const T* src, int to, int d, int kp, long long rows, float scale, char* out, long long plane) {
   if (to < 0) return;
+#pragma unroll 4
   for (int u = threadIdx.x >> 6; u < kp / 32; u += 4) {
     const int c = u * 32 + (threadIdx.x & 3) * 8;
     u32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
@@ -887,6 +888,24 @@ __global__ __launch_bounds__(1024) void ce_gmax_kernel(int n, const float* __res
   }
 }
 
+// four elements at any element boundary, of which `left` belong to the row
+template <typename T> __device__ __forceinline__ void store4(T* p, int left, const f32x4& x) {
+  if (left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      store16(p, u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])});
+    } else {
+      uint32_t h[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) h[r] = __builtin_bit_cast(uint16_t, from_f32<T>(x[r]));
+      reinterpret_cast<Raw8*>(p)->v = u32x2{h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 3; ++r)
+      if (r < left) p[r] = from_f32<T>(x[r]);
+  }
+}
+
 // What is left when all pieces are done, in one launch.  dx: slabs added in order, scaled, back to the rows they belong to (zeros in rows
 // that do not count).  dw where its product was split along the rows: four parts of the slabs side by side, each in order, joined in
 // order.  db: the chunks' sums in order.
@@ -909,13 +928,14 @@ struct Final {
 template <typename T>
 __global__ __launch_bounds__(256) void ce_final_kernel(Final f) {
   __shared__ f32x4 tmp[256];
-  const int per = (f.d + 3) / 4;
+  const unsigned per = (f.d + 3) / 4;      // fours of a row; all of them are fewer than 2^32
   const float rows = f.scal[kCount];
   const float whole = rows == 0.f ? 0.f : f.reduction == 0 ? f.scal[kGMax] : f.reduction == 1 ? f.gout[0] / rows : f.gout[0];
   if (blockIdx.x < f.dx_wgs) {
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, i = id / per;
+    const unsigned id = blockIdx.x * 256 + threadIdx.x;
+    const long long i = id / per;
     if (i >= f.n) return;
-    const int c = (int)(id % per) * 4, at = f.inverse[i];
+    const int c = (int)(id - (unsigned)i * per) * 4, at = f.inverse[i];
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
       const float* p = f.dx_slab + at * f.ld + c;
@@ -929,14 +949,12 @@ __global__ __launch_bounds__(256) void ce_final_kernel(Final f) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] *= g;
     }
-    T* out = (T*)f.dx + i * f.d + c;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (c + r < f.d) out[r] = from_f32<T>(x[r]);
+    store4((T*)f.dx + i * f.d + c, f.d - c, x);
   } else if (blockIdx.x < f.dx_wgs + f.dw_wgs) {
     const int part = threadIdx.x >> 6, each = (f.dw_splits + 3) / 4;
-    const long long id = (long long)(blockIdx.x - f.dx_wgs) * 64 + (threadIdx.x & 63), i = id / per;
-    const int c = (int)(id % per) * 4;
+    const unsigned id = (blockIdx.x - f.dx_wgs) * 64 + (threadIdx.x & 63);
+    const long long i = id / per;
+    const int c = (int)(id - (unsigned)i * per) * 4;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     if (i < f.v) {
       const float* p = f.dw_slab + i * f.ld + c;
@@ -954,10 +972,9 @@ __global__ __launch_bounds__(256) void ce_final_kernel(Final f) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] += tmp[s * 64 + threadIdx.x][r];
     const float g = whole / kDzScale / f.scal[kXScale];
-    T* out = (T*)f.dw + i * f.d + c;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (c + r < f.d) out[r] = from_f32<T>(g * x[r]);
+    for (int r = 0; r < 4; ++r) x[r] *= g;
+    store4((T*)f.dw + i * f.d + c, f.d - c, x);
   } else {
     const int c = (blockIdx.x - f.dx_wgs - f.dw_wgs) * 256 + threadIdx.x;
     if (c >= f.v) return;

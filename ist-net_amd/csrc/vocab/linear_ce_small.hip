@@ -12,8 +12,6 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-struct __attribute__((packed, aligned(2))) Raw8 { u32x2 v; };
 
 constexpr float kNaN = __builtin_nanf("");
 constexpr int kWaves = 16, kTM = 64, kTN = 32;      // tile of a workgroup: every wave has all of it for its part of K

@@ -20,9 +20,11 @@ namespace {
 typedef _Float16 f16;
 struct bf16 { uint16_t u; };
 
-// sixteen bytes at any element boundary: gfx950 loads and stores them with one instruction whatever the address
+// sixteen and eight bytes at any element boundary: gfx950 loads and stores them with one instruction whatever the address
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 struct __attribute__((packed, aligned(2))) Raw16 { u32x4 v; };
+struct __attribute__((packed, aligned(2))) Raw8 { u32x2 v; };
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(f16 x) { return (float)x; }

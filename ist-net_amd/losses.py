@@ -50,8 +50,9 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
     float32 loss: per row ("none"), their "sum" or their "mean" over the rows that count.  Slots with index -1 are unused
     (their logits are not looked at); a row without a used slot does not count: loss 0, gradient 0, its logits are not looked at;
     the mean over no row is NaN.  Slots may repeat a class.  A row with an index outside [-1, V), with a NaN among its used
-    logits or without a finite largest one is NaN, loss and gradient.  T: 1e-4 to 1e4.  Differentiable w.r.t. ``logits`` (once).  ``logits`` may be a slice with a row stride, of
-    float32, bfloat16 or float16; the gradient has its type, everything between is float32."""
+    logits or without a finite largest one is NaN, loss and gradient.  T: 1e-4 to 1e4.  Differentiable w.r.t. ``logits`` (once).
+    ``logits`` may be a slice with a row stride, of float32, bfloat16 or float16; the gradient has its type, everything between
+    is float32."""
     from . import vocab_native as vn
     vn.check_reduction(reduction)
     temperature = float(temperature)
@@ -70,7 +71,10 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
     vn.check_device(logits, "logits", top_logits, "top_logits")
     vn.check_device(logits, "logits", top_index, "top_index")
     lead = logits.shape[:-1]
-    z, top, idx = logits.reshape(-1, v), top_logits.reshape(-1, k), top_index.reshape(-1, k)
+    flat = logits.dim() == 2                         # (a view costs a node of the graph)
+    z, top, idx = logits, top_logits, top_index
+    if not flat:
+        z, top, idx = logits.reshape(-1, v), top_logits.reshape(-1, k), top_index.reshape(-1, k)
     n = z.shape[0]
     if logits.is_cuda and n:
         vn.check_float(logits, "logits")
@@ -92,7 +96,7 @@ def TopLogitsDistill(logits, top_logits, top_index, temperature=1.0, reduction="
         rows = temperature ** 2 * torch.where(used & (q != 0), q * (log_q - log_p), 0.0).sum(1)
         rows = rows * torch.where(bad, float("nan"), 1.0)
         loss = _reduce_rows(rows, counted, reduction)
-    return loss.reshape(lead) if reduction == "none" else loss
+    return loss if flat or reduction != "none" else loss.reshape(lead)
 
 
 def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, reduction="mean"):
@@ -123,7 +127,8 @@ def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, r
     if bias is not None:
         vn.check_device(features, "features", bias, "bias")
     ignore_index = int(ignore_index)
-    x, t = features.reshape(-1, d), target.reshape(-1)
+    flat = features.dim() == 2                       # (a view costs a node of the graph)
+    x, t = (features, target) if flat else (features.reshape(-1, d), target.reshape(-1))
     n = x.shape[0]
     if features.is_cuda and n:
         vn.check_float(features, "features")
@@ -141,7 +146,7 @@ def LinearCrossEntropy(features, weight, target, bias=None, ignore_index=-100, r
         rows = -torch.log_softmax(z, 1).gather(1, t.long().clamp(0, v - 1).unsqueeze(1)).squeeze(1)
         rows = torch.where(counted, rows, 0.0) * torch.where(bad, float("nan"), 1.0)
         loss = _reduce_rows(rows, counted, reduction)
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    return loss if flat or reduction != "none" else loss.reshape(target.shape)
 
 
 class _WeightedSumFn(torch.autograd.Function):
