@@ -4,7 +4,9 @@
 //   row = T^2 sum_k q_k (log q_k - log p_idx(k))          dz_v = T g (p_v - sum_{k: idx(k) = v} q_k)
 //
 // Bound by bytes: z is read once forward (one pass with a running maximum and sum), read once and dz written once backward; the
-// teacher's k values are noise beside a row.  A row is one workgroup's, or several workgroups' where there are few rows.
+// teacher's k values are noise beside a row.  A row is one workgroup's, or several workgroups' where there are few rows.  8192 rows of
+// 65536 bfloat16 classes, 5% of them without a teacher: forward 230 us = 4.4 TB/s, backward 428 us = 4.9 TB/s, where a copy of a large
+// tensor runs at 5.15 TB/s.  Four 16-byte loads in flight per thread forward, two beside as many stores backward.
 #include <algorithm>
 
 #include "vocab_common.h"
@@ -291,15 +293,16 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
 }
 
 struct DistillPlan { int threads, splits, width; };
-// One wave per row up to 4 KB, four waves above; parts of a row (of whole 4 KB blocks) where the rows alone are too few workgroups
-// for the chip's 256 compute units.
+// One wave per row up to 4 KB, four waves above (forward and backward, 8000 rows of 4 KB: 40 us with one, 49 us with four; of 8 KB: 63 and
+// 60 us).  Up to 256 rows of more than 64 KB, too few for the chip's 256 compute units, are cut into parts of 16 KB at least (4 rows of
+// 256 KB: 20 us cut, 29 us whole; 64: 24 and 32 us; 512: 76 and 74 us; one row of 64 KB: 20 and 18 us).
 inline DistillPlan distill_plan(long long n, int v, int elt) {
   DistillPlan p;
   const long long bytes = (long long)v * elt;
   p.threads = bytes <= 4096 ? 64 : 256;
   const int block = 4096 / elt;
   const long long blocks = (v + block - 1) / block;
-  p.splits = (int)std::min(blocks, std::max(1ll, 2048 / n));
+  p.splits = n <= 256 && blocks > 16 ? (int)std::min(blocks / 4, 1024 / n) : 1;
   p.width = (int)((blocks + p.splits - 1) / p.splits) * block;
   p.splits = (int)((v + (long long)p.width - 1) / p.width);
   return p;

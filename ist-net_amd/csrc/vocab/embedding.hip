@@ -7,6 +7,10 @@
 // are sorted by index (stable, least significant digit first), every table row then owns a run of the sorted list and one team of
 // lanes adds it up in registers -- no atomics, dw written once.  A run longer than L tokens would leave one team with a long chain
 // of loads; it is cut where the sorted list is cut into pieces of L, the pieces are summed side by side and joined in order.
+//
+// 32768 tokens of a table of 65536 x 1024 bfloat16: lookup 25 us (67 MB written, 20 to 40 MB of rows read: 4 TB/s), gradient 97 us of
+// which the sums take 56 us (67 MB read, 134 MB written: 3.6 TB/s) and the sort 41 us: six launches of 4 to 11 us that wait for memory
+// and for each other, whatever the width of the rows.
 #include <algorithm>
 
 #include "vocab_common.h"
@@ -19,7 +23,8 @@ constexpr int kSmallDigit = 6;        // bits of a digit there: 64 digits x 16 w
 constexpr int kDigit = 9;             // most bits of a digit of the sort over many workgroups
 constexpr int kSortThreads = 256;
 constexpr int kFewBlocks = 64;        // workgroups up to which the scatter adds up the digit counts of all of them (saves a launch)
-constexpr int kFewItems = 4, kSortItems = 16;      // tokens per thread of that sort, up to 2^18 tokens and above
+// tokens per thread of that sort, up to 2^20 tokens (lookup and gradient of 2^18: 90 us with 4, 120 us with 16) and above (2^23: 840 and 790 us)
+constexpr int kFewItems = 4, kSortItems = 16;
 
 __device__ __forceinline__ uint32_t key_of(const void* ids, long long i, int idx64, int v, long long padding) {
   const long long id = load_index(ids, i, idx64);
@@ -430,7 +435,8 @@ __global__ __launch_bounds__(256) void embed_join_kernel(int n, int v, int d, in
 
 // Few tokens: one launch.  A workgroup owns `rows` (<= 64) consecutive table rows, picks their tokens out of all n in order, sorts them
 // by row in LDS and adds them up; a run longer than kShortRun is shared by its teams.  (77 x 99 into 1000 rows: 5 launches of 2 to 5 us
-// each became one of 6 us, and what they cost the host is gone.)
+// each became one of 6 us, and what they cost the host is gone: 20 us.  2048 tokens into 1000 rows: lookup and gradient 38 us in a graph,
+// 29 us with the sort, 4096: 56 and 34 us; launched one by one both wait for the host up to some 60 us.)
 constexpr int kFewTokens = 2048, kFewRows = 64, kShortRun = 32;
 template <typename T>
 __global__ __launch_bounds__(256) void embed_few_kernel(int n, int v, int d, int rows, int lanes_log, const T* __restrict__ grad,
@@ -572,7 +578,7 @@ inline EmbedPlan embed_plan(long long n, int v, int d) {
   const int key_bits = log2_ceil((long long)v + 1), most = n <= kSmallSort ? kSmallDigit : kDigit;
   p.passes = (key_bits + most - 1) / most;
   p.bits = (key_bits + p.passes - 1) / p.passes;
-  p.items = n <= 256 * 1024 ? kFewItems : kSortItems;
+  p.items = n <= 1024 * 1024 ? kFewItems : kSortItems;
   p.nb = (int)((n + kSortThreads * p.items - 1) / (kSortThreads * p.items));
   // pieces short enough that one is a few rounds of loads, long enough that the partial sums of one row do not become many
   p.longest = std::max(32, (1 << ((log2_ceil(n) + 1) / 2)) / 8);
@@ -612,8 +618,9 @@ extern "C" int istnet_embed_backward(long long n, int v, int d, int dtype, int i
   const hipStream_t st = (hipStream_t)stream;
   const int ll = lanes_log_of(d, dtype);
   if (embed_few(n, v)) {
-    // rows per workgroup: enough workgroups for the chip, few enough that reading all indices in each of them stays cheap
-    const int rows = v <= 4096 ? 16 : kFewRows;
+    // rows per workgroup: enough workgroups for the chip, few enough that reading all indices in each of them stays cheap (1000 tokens,
+    // table of 65536 x 256: 30 us with 16, 43 us with 64; 2000 tokens, 2^20 x 16: 230 and 108 us)
+    const int rows = v <= 65536 ? 16 : kFewRows;
     VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(embed_few_kernel<T>), dim3((unsigned)((v + rows - 1ll) / rows)), dim3(256),
                                                 0, st, (int)n, v, d, rows, ll, (const T*)grad, ldg, ids, idx64, padding, scale, (T*)dw));
     return launch_status();

@@ -194,6 +194,10 @@ __device__ __forceinline__ void tile_of(int wg, int total, int tm, int tn, int* 
   *n = in / gm;
 }
 
+// 7424 rows that count of 8192 x 1024 against 65536 classes, bfloat16: logits with their statistics 960 us = 1040 TFLOP/s (matrix cores busy
+// 0.62 of the time, no LDS conflict), again with p - t written 4 x 267 us = 930 TFLOP/s (0.53), dx and dw 4 x 512 us = 970 TFLOP/s
+// (0.59).  A library's product of the same sizes without the epilogues: x w^T 927, z w 1142, z^T x 1024 us.  Two workgroups per compute
+// unit overlap the epilogue of one with the products of the other: one tile of 256 x 256 per unit took 1320 us for the logits.
 enum { kLse = 0, kDz = 1, kSlab = 2, kOut = 3 };
 
 // C (M x N) = A (M x K) B (N x K)^T, tile MT x NT, four waves of MT / 2 x NT / 2.  M: matrix element type; SEGS: products of planes
@@ -486,7 +490,7 @@ __device__ __forceinline__ void column_sums(float* tmp, int unit, int part_no, c
   const int a = part_no * chunk, b = min(count, a + chunk);
   const long long at = unit * dz.unit_stride + ((lane & 3) << 4);
   float s[8] = {};
-#pragma unroll 4
+#pragma unroll 8
   for (int r = a + wave * 16 + (lane >> 2); r < b; r += 64) {
     const float g = weights ? weights[rowmap[r]] : 1.f;
     float f[8];
@@ -1006,7 +1010,11 @@ inline int tile_d(int d) { return d <= 64 ? 64 : (d + 127) / 128 * 128 < (d + 25
 constexpr long long kPieceBytes = 512ll << 20;           // memory of one piece of p - t
 constexpr int kMostSplits = 128;
 constexpr int kScanWgs = 2048;                           // workgroups at most that look for the largest entry of x, and of w
-constexpr long long kSmallSide = 1024, kSmallProducts = 1 << 28;      // see linear_ce_small.hip
+// Problems that the four launches of linear_ce_small.hip serve.  Forward and backward in a graph, float32 / bfloat16, there and here:
+// 32 x 512, 6 classes 24 / 25 and 64 / 44 us; 512 x 256, 512 classes 38 / 39 and 59 / 46 us; 1024 x 256, 1024 classes (2^28 products)
+// 64 / 65 and 66 / 51 us; 1024 x 1024, 1024 classes 133 / 138 and 137 / 72 us.  Launched one by one, the five launches that are saved
+// are 20 us of the host's besides.
+constexpr long long kSmallSide = 1024, kSmallProducts = 1 << 28;
 
 inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
 inline bool ce_ok(long long n, int d, int v, int dtype) {
@@ -1014,13 +1022,13 @@ inline bool ce_ok(long long n, int d, int v, int dtype) {
          // a launch holds fewer than 2^32 threads
          ((n + 127) / 128) * ((v + 255ll) / 256) <= (1ll << 23) && n * d <= (1ll << 33) && (long long)v * d <= (1ll << 33);
 }
-// Without a backward and for few rows, 16-bit rows of w are read as they lie: packing them costs three passes over w (81 us of
-// 65536 x 1024), which the products of panels win back from about 4000 rows on.
+// Without a backward and for few rows, 16-bit rows of w are read as they lie: packing them costs three passes over w, which the products
+// of panels win back with the rows (65536 classes x 1024 bfloat16: 1 row 47 us as they lie, 113 us packed; 2048 rows 275 and 339;
+// 4096 rows 525 and 572; 8192 rows 1055 and 1043).
 inline bool direct_w(long long n, int d, int dtype, int train, const void* w, long long ldw) {
-  return !train && n <= 4096 && dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
+  return !train && n <= 8192 && dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
 }
 
-// Problems that the four launches of linear_ce_small.hip serve.
 inline bool small_ce(long long n, int d, int v) {
   return n <= kSmallSide && v <= kSmallSide && n * v * d <= kSmallProducts;
 }
@@ -1100,7 +1108,8 @@ inline Backward backward_plan(const Keep& k, long long n, int d, int v, int dtyp
   b.dw_splits = (int)splits(dt * ((most_rows + kNT - 1) / kNT), dw_steps);
   if ((long long)v * d > (1ll << 28)) b.dw_splits = 1;      // joining the slabs of that many rows would not be one launch
   b.dw_per = (int)((dw_steps + b.dw_splits - 1) / b.dw_splits);
-  b.chunk = (int)std::max<long long>(256, round_up((n + 127) / 128, 64));      // rows of one part of a bias gradient: 128 parts at most
+  // rows of one part of a bias gradient: 128 parts at most, and some 2048 workgroups of a panel's part where there are more panels
+  b.chunk = (int)std::max<long long>({256, round_up((n + 127) / 128, 64), round_up(n * (b.piece / 32) / 2048, 64)});
   b.chunks = (int)((n + b.chunk - 1) / b.chunk);
   long long at = 0;
   auto take = [&](long long bytes) { const long long o = at; at += round_up(bytes, 256); return o; };
@@ -1155,6 +1164,7 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   RowStat* stat = (RowStat*)(kb + k.stat);
   int *blocks = (int*)(wb + f.blocks), *rowmap = (int*)(kb + k.rowmap), *inverse = (int*)(kb + k.inverse), *tgt = (int*)(kb + k.tgt);
   const int ax = scaled ? (int)std::min<long long>(kScanWgs, (n + 15) / 16) : 0, aw = scaled ? (int)std::min<long long>(kScanWgs, (v + 15ll) / 16) : 0;
+  // more rows: counted once (8000 rows x 128, 1100 classes: 112 us either way; 32000: 243 us counted once, 270 us by every workgroup)
   const bool planned = n > 8192;
   const int cw = planned ? (int)((n + 255) / 256) : 0;
   if (ax + aw + cw)

@@ -235,7 +235,7 @@ def test_distill(n, v, k, dtype):
 
 
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
-@pytest.mark.parametrize("n,v", [(9, 50), (9, 9000)])
+@pytest.mark.parametrize("n,v", [(9, 50), (9, 9000), (9, 40000)])
 def test_distill_masks_and_repeats(n, v, reduction):
     """Rows without a teacher (their NaN logits are not looked at), slots without one, repeated classes, weights of zero, classes the
     student excludes."""
@@ -252,7 +252,7 @@ def test_distill_masks_and_repeats(n, v, reduction):
     _check_distill(z, top, idx, 1.5, reduction)
 
 
-@pytest.mark.parametrize("v", [50, 9000])
+@pytest.mark.parametrize("v", [50, 9000, 40000])
 def test_distill_rows_that_cannot_be_right_are_nan(v):
     z, top, idx = _distill_inputs(6, v, 4, F32, v)
     idx[0, 2], idx[1, 0], top[2, 1], z[3, 7], z[4, 8] = v, -2, NAN, NAN, INF
@@ -261,7 +261,7 @@ def test_distill_rows_that_cannot_be_right_are_nan(v):
     assert dz[:5].isnan().all() and dz[5].isfinite().all()
 
 
-@pytest.mark.parametrize("v", [50, 9000])
+@pytest.mark.parametrize("v", [50, 9000, 40000])
 def test_distill_teachers_without_a_finite_largest_logit(v):
     z, top, idx = _distill_inputs(4, v, 4, F32, v + 1)
     top[0, 1], top[1] = INF, -INF
@@ -773,10 +773,9 @@ def test_few_indices_into_a_table_of_very_many_rows():
     assert dw[[v - 1, v - 2, 5], 0].tolist() == [18.0, 8.0, 4.0] and dw.count_nonzero() == 3
 
 
-@pytest.mark.parametrize("v", [40, 70000])
-def test_lookup_gradient_of_many_indices(v):
+@pytest.mark.parametrize("n,v", [(300_001, 40), (300_001, 70000), (1_100_003, 70000)])
+def test_lookup_gradient_of_many_indices(n, v):
     """More workgroups than one reads the digit counts of by itself, an odd number of them."""
-    n = 300_001
     ids = torch.randint(0, v, (n,), device=DEV, generator=_gen(v))
     ids[ids % 5 == 1] = 3
     w = torch.zeros(v, 3, device=DEV)
