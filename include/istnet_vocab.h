@@ -1,12 +1,13 @@
 /*
  * istnet_vocab.h -- C ABI (library libistnet_pn2.so, conventions of istnet_pn2.h) of the operators at the two ends of a model
- * with discrete classes: a scaled table lookup and its gradient, and the distance to a teacher's top logits.
+ * with discrete classes: a scaled table lookup and its gradient, the distance to a teacher's top logits, and the cross entropy of
+ * a linear head without its logits.
  *
  * Element types: ISTNET_VOCAB_F32 / _BF16 / _F16 (`dtype`, all floating tensors of a call that are not said to be float).
  * Indices are int32 (idx64 == 0) or int64 (idx64 != 0).  Rows are contiguous (last stride 1); a leading dimension `ld*` is the
  * distance of two rows in elements.  Every function enqueues on `stream` and returns 0, a hipError_t or ISTNET_PN2_EINVAL; the
- * *_scratch_kib functions return the size of the caller's scratch memory `ws` in KiB (-1 for invalid sizes; 0: ws may be NULL), which nothing
- * has to clear and which may be reused as soon as the call's work on `stream` is done.  Sums are float or double, in an order that the
+ * *_scratch_kib functions return the size of the caller's scratch memory `ws` in KiB (-1 for invalid sizes; 0: ws may be NULL), which
+ * nothing has to clear and which may be reused as soon as the call's work on `stream` is done.  Sums are float or double, in an order that the
  * sizes alone decide: the same inputs give the same bits.
  */
 #ifndef ISTNET_VOCAB_H_
@@ -37,10 +38,11 @@ ISTNET_PN2_API int istnet_embed_backward(long long n, int v, int d, int dtype, i
  * top (n, k) of the classes idx (n, k); slots with idx == -1 are unused, rows without a used slot do not count:
  *   q = softmax over the used slots of top / T,  p = softmax over all classes of z / T,
  *   row = T^2 * sum_k q_k (log q_k - log p_idx(k)),  loss = per row (reduction 0), sum (2) or mean over the counted rows (1).
- * An index outside [-1, v) or a NaN among the used logits makes its row NaN.  Kept for the backward: stats (n, 2) = (row maximum,
- * sum of exp((z - maximum) / T) beside the largest itself, -1 where the row does not count), q (n, k) = the weight of a slot's class (the slots of a row
- * that name the same class all hold their sum) and count (1) = number of counted rows (written for reductions 1 and 2).
- * ttype: element type of top.  n <= 2^23. */
+ * An index outside [-1, v), a NaN among the used logits or none with a finite maximum makes its row NaN.  Kept for the backward:
+ * stats (n, 2) = (row maximum, sum of exp((z - maximum) / T) beside the largest itself, -1 where the row does not count), q (n, k) =
+ * the weight of a slot's class (the slots of a row that name the same class all hold their sum) and count (1) = number of counted
+ * rows (written for reductions 1 and 2).
+ * ttype: element type of top.  n <= 2^23, v < 2^31 - 2^24. */
 ISTNET_PN2_API int istnet_distill_scratch_kib(long long n, int v, int k);
 ISTNET_PN2_API int istnet_distill_forward(long long n, int v, int k, int dtype, int ttype, int idx64, const void *z,
                                           long long ldz, const void *top, const void *idx, float temperature, int reduction,
