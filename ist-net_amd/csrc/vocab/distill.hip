@@ -16,7 +16,6 @@ namespace {
 constexpr int kMaxSlots = 256;
 constexpr int kShortRow = 2048;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNaN = __builtin_nanf("");
 
 struct Stat { float m, s; };      // maximum, sum of exp2((x - maximum) c)
 

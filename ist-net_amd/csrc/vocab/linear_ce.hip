@@ -39,7 +39,6 @@ typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kNaN = __builtin_nanf("");
 constexpr int BK = 32;            // K per step: 64 bytes of a row
 constexpr int kStages = 3;        // steps in LDS: one being read, two on their way
 constexpr int kPad = 256;         // rows of packed operands are padded to whole tiles
@@ -1023,7 +1022,7 @@ inline bool ce_ok(long long n, int d, int v, int dtype) {
          ((n + 127) / 128) * ((v + 255ll) / 256) <= (1ll << 23) && n * d <= (1ll << 33) && (long long)v * d <= (1ll << 33);
 }
 // Without a backward and for few rows, 16-bit rows of w are read as they lie: packing them costs three passes over w, which the products
-// of panels win back with the rows (65536 classes x 1024 bfloat16: 1 row 47 us as they lie, 113 us packed; 2048 rows 275 and 339;
+// of panels win back with the rows (65536 classes x 1024 bfloat16: 512 rows 88 us as they lie, 159 us packed; 2048 rows 275 and 339;
 // 4096 rows 525 and 572; 8192 rows 1055 and 1043).
 inline bool direct_w(long long n, int d, int dtype, int train, const void* w, long long ldw) {
   return !train && n <= 8192 && dtype != ISTNET_VOCAB_F32 && d % BK == 0 && ldw % 8 == 0 && ldw <= (1 << 22) && ((uintptr_t)w & 15) == 0;
@@ -1032,6 +1031,10 @@ inline bool direct_w(long long n, int d, int dtype, int train, const void* w, lo
 inline bool small_ce(long long n, int d, int v) {
   return n <= kSmallSide && v <= kSmallSide && n * v * d <= kSmallProducts;
 }
+// Problems that linear_ce_few.hip serves.  65536 classes x 1024, forward alone / with backward, there and here: bfloat16, one row 33 / 93 and
+// 46 / 255 us, 32 rows 38 / 159 and 47 / 265 us (64 rows would take 53 / 421, and 48 / 274 here); float32, one row 57 / 186 and
+// 253 / 506 us, 32 rows 101 / 351 and 260 / 512 us.  8000 classes x 200, bfloat16, 32 rows with backward: 42 and 49 us.
+inline bool few_ce(long long n, int d, int v) { return !small_ce(n, d, v) && n <= kFewRowsCe && n * v <= (1ll << 28); }
 
 struct Keep {      // what the backward needs, in the caller's `keep`
   long long np, kp, vp, planes;
@@ -1138,11 +1141,13 @@ inline void launch_pack(int wgs, hipStream_t st, A... args) {
 extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, int train, const void* w, long long ldw) {
   if (!ce_ok(n, d, v, dtype)) return -1;
   if (small_ce(n, d, v)) return (int)((vocab_small_ce_keep(n, v) + 1023) / 1024);
+  if (few_ce(n, d, v)) return (int)((vocab_few_ce_keep(n, v, train) + 1023) / 1024);
   return (int)((keep_plan(n, d, v, dtype, direct_w(n, d, dtype, train, w, ldw)).bytes + 1023) / 1024);
 }
 extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward) {
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
   if (small_ce(n, d, v)) return 0;
+  if (few_ce(n, d, v)) return (int)((vocab_few_ce_scratch(n, d, v, dtype, backward) + 1023) / 1024);
   const Keep k = keep_plan(n, d, v, dtype, false);
   return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k, n, v).bytes) + 1023) / 1024);
 }
@@ -1155,6 +1160,8 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
   const hipStream_t st = (hipStream_t)stream;
   if (small_ce(n, d, v))
     return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, st);
+  if (few_ce(n, d, v))
+    return vocab_few_ce_forward((int)n, d, v, dtype, idx64, train, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, ws, st);
   const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
   const Forward f = forward_plan(k, n, v);
@@ -1227,6 +1234,7 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   const hipStream_t st = (hipStream_t)stream;
   if (!dx && !dw && !db) return 0;
   if (small_ce(n, d, v)) return vocab_small_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, dx, dw, db, st);
+  if (few_ce(n, d, v)) return vocab_few_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, ws, dx, dw, db, st);
   const Keep k = keep_plan(n, d, v, dtype, false);
   const Backward b = backward_plan(k, n, d, v, dtype, reduction);
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = kb + k.wp, *dz = wb + b.dz, *xb = xp;

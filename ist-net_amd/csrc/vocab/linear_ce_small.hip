@@ -14,7 +14,6 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kNaN = __builtin_nanf("");
 constexpr int kWaves = 16, kTM = 64, kTN = 32;      // tile of a workgroup: every wave has all of it for its part of K
 constexpr int kPitch = kTM + 4;
 
@@ -144,34 +143,16 @@ __global__ __launch_bounds__(256) void ce_small_rows_kernel(int n, int v, int vp
     if (lane == 0) { row_loss[i] = fill; on[i] = t != ignore; }
     return;
   }
-  // the other classes: largest logit and sum of exponentials, so that the loss and the target's derivative keep their relative
-  // precision where the target is almost certain
-  float m = -INFINITY;
+  float m = -INFINITY;      // of the other classes
   for (int c = lane; c < v; c += 64) m = c == t ? m : fmaxf(m, row[c]);
   m = wave_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
   float s = 0.f;
   for (int c = lane; c < v; c += 64) s += c == t ? 0.f : expf(row[c] - ref);
   s = wave_sum(s);
-  const float zt = row[t], d = zt - m;
-  float loss, at_target, top;
-  if (m == -INFINITY) {
-    loss = s + 0.f * zt;      // zero, or NaN
-    at_target = -loss;
-    top = zt;
-  } else if (d < -60.f) {
-    loss = logf(s) - d;
-    at_target = d == -INFINITY ? -1.f : -1.f + 0.f * loss;
-    top = m;
-  } else {
-    const float rest = d == INFINITY ? kNaN : d > 0.f ? s * expf(-d) : s / expf(d);
-    loss = log1pf(rest);
-    at_target = -rest / (1.f + rest);
-    top = fmaxf(m, zt);
-  }
-  const float inv = 1.f / ((m == -INFINITY ? s : s * expf(m - top)) + expf(zt - top));
-  for (int c = lane; c < vp; c += 64) row[c] = c >= v ? 0.f : c == t ? at_target : inv * expf(row[c] - top);
-  if (lane == 0) { row_loss[i] = loss; on[i] = 1; }
+  const Row r = row_of(m, s, row[t]);
+  for (int c = lane; c < vp; c += 64) row[c] = c >= v ? 0.f : c == t ? r.at_target : r.inv * expf(row[c] - r.top);
+  if (lane == 0) { row_loss[i] = r.loss; on[i] = 1; }
 }
 
 __global__ __launch_bounds__(1024) void ce_small_total_kernel(int n, int reduction, const float* __restrict__ row_loss,

@@ -8,7 +8,16 @@
 
 #include "../../../include/istnet_vocab.h"
 
-// The cross entropy of small problems (linear_ce_small.hip), called by the entry points of linear_ce.hip.
+// The cross entropy of few rows (linear_ce_few.hip) and of small problems (linear_ce_small.hip), called by the entry points of
+// linear_ce.hip.
+constexpr int kFewRowsCe = 32;
+long long vocab_few_ce_keep(long long n, int v, int train);
+long long vocab_few_ce_scratch(long long n, int d, int v, int dtype, int backward);
+int vocab_few_ce_forward(int n, int d, int v, int dtype, int idx64, int train, const void* x, long long ldx, const void* w,
+                         long long ldw, const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep,
+                         void* ws, hipStream_t st);
+int vocab_few_ce_backward(int n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw, int reduction,
+                          const float* gout, const void* keep, void* ws, void* dx, void* dw, void* db, hipStream_t st);
 long long vocab_small_ce_keep(long long n, int v);
 int vocab_small_ce_forward(int n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w, long long ldw,
                            const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, hipStream_t st);
@@ -16,6 +25,8 @@ int vocab_small_ce_backward(int n, int d, int v, int dtype, const void* x, long 
                             const float* gout, const void* keep, void* dx, void* dw, void* db, hipStream_t st);
 
 namespace {
+
+constexpr float kNaN = __builtin_nanf("");
 
 typedef _Float16 f16;
 struct bf16 { uint16_t u; };
@@ -118,6 +129,30 @@ __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
   return x;
+}
+
+// A row from its other classes (largest logit m, sum s of exp(z - m)) and its target's logit: probabilities inv exp(z - top), p - 1 of the
+// target from the sum over the others, so that it and the loss keep their relative precision where the target is almost certain.
+struct __attribute__((aligned(16))) Row { float top, inv, at_target, loss; };
+__device__ __forceinline__ Row row_of(float m, float s, float zt) {
+  const float d = zt - m;
+  Row r;
+  if (m == -INFINITY) {
+    r.loss = s + 0.f * zt;      // zero, or NaN
+    r.at_target = -r.loss;
+    r.top = zt;
+  } else if (d < -60.f) {
+    r.loss = logf(s) - d;
+    r.at_target = d == -INFINITY ? -1.f : -1.f + 0.f * r.loss;
+    r.top = m;
+  } else {
+    const float rest = d == INFINITY ? kNaN : d > 0.f ? s * expf(-d) : s / expf(d);
+    r.loss = log1pf(rest);
+    r.at_target = -rest / (1.f + rest);
+    r.top = fmaxf(m, zt);
+  }
+  r.inv = 1.f / ((m == -INFINITY ? s : s * expf(m - r.top)) + expf(zt - r.top));
+  return r;
 }
 
 inline int launch_status() {

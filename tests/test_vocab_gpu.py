@@ -596,6 +596,46 @@ def test_linear_ce_without_a_backward(n, d, v, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,d,v", [(1, 1024, 5000), (1, 31, 1025), (2, 33, 3001), (3, 1, 70001), (4, 7, 7000), (7, 130, 2049), (16, 1027, 5003),
+                                   (13, 2500, 1500), (16, 64, 66000), (17, 64, 3000), (32, 300, 4001), (33, 129, 2100), (64, 1024, 5000),
+                                   (64, 20, 40000), (65, 64, 3000)])
+def test_linear_ce_few_rows(n, d, v, dtype):
+    for i, reduction in enumerate(["mean", "none", "sum"]):
+        x, w, b, t = _ce_inputs(n, d, v, dtype, n + d + v + i, bias=i != 1, ignored=0.2 if n > 2 else 0.0,
+                                index=(torch.int32, torch.int64)[i % 2])
+        wide = torch.zeros(v, d + 5, device=DEV, dtype=dtype)
+        wide[:, 3:3 + d] = w
+        _check_ce(x, wide[:, 3:3 + d] if i == 2 else w, b, t, reduction)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_linear_ce_few_rows_masks(dtype, reduction):
+    x, w, b, t = _ce_inputs(11, 48, 2600, dtype, 27, ignored=0.0)
+    t[5], t[10], t[7], t[0] = IGNORE, IGNORE, 2599, 1
+    x[5], x[10] = NAN, INF
+    b[64:256], b[300] = -INF, -INF
+    t = torch.where(((t >= 64) & (t < 256)) | (t == 300), 450, t)
+    loss, grads = _check_ce(x, w, b, t, reduction)
+    assert all(g.isfinite().all() for g in grads) and (grads[0][[5, 10]] == 0).all()
+    loss, grads = _check_ce(x[:4], w, b, torch.full_like(t[:4], 7), reduction, ignore=7)      # nothing counts
+    assert (loss == 0).all() if reduction != "mean" else loss.isnan()
+    assert all((g == 0).all() for g in grads)
+    t[2], t[3] = 2600, -1
+    xr = x.detach().requires_grad_()
+    loss = losses.LinearCrossEntropy(xr, w, t, b, reduction=reduction)
+    (dx,) = torch.autograd.grad(loss, xr, torch.ones_like(loss))
+    assert dx.isnan().all(1).nonzero().flatten().tolist() == [2, 3] and dx[[0, 1, 4, 5, 10]].isfinite().all()
+    assert loss.isnan().sum() == (2 if reduction == "none" else 1)
+    first = losses.LinearCrossEntropy(xr[:2], w.requires_grad_(), t[:2], b, reduction=reduction)      # only one of the gradients
+    g = torch.ones_like(first)
+    (dw,) = torch.autograd.grad(first, w, g, retain_graph=True)
+    (dx,) = torch.autograd.grad(first, xr, g, retain_graph=True)
+    both = torch.autograd.grad(first, (xr, w), g)
+    assert torch.equal(both[0], dx) and torch.equal(both[1], dw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("d,v", [(384, 128), (128, 64), (64, 100), (130, 40), (640, 129)])
 def test_linear_ce_few_classes_many_rows(d, v, dtype):
     """Past the four launches of small problems: every tile shape."""
@@ -837,3 +877,10 @@ def test_offsets_beyond_32_bits():
     assert float((dw[-2000:].double() - tail).norm()) <= 4 * _round(F16) * float(tail.norm())
     dxw = sum(p[:, a:a + 200_000] @ w.detach()[a:a + 200_000].double() for a in range(0, rows, 200_000))
     assert float((dx.double() - dxw).norm()) <= 4 * _round(F16) * float(dxw.norm())
+    del dw, p, logits
+    xm = xh.detach().repeat(5, 1).requires_grad_()                 # more rows than are kept in registers
+    loss = losses.LinearCrossEntropy(xm, w, target.repeat(5), reduction="none")
+    dx, dw = torch.autograd.grad(loss, (xm, w), torch.ones_like(loss))
+    torch.testing.assert_close(loss.double(), want.repeat(5), rtol=4096 * U, atol=4096 * U)
+    assert float((dw[-2000:].double() - 5 * tail).norm()) <= 4 * _round(F16) * float(5 * tail.norm())
+    assert float((dx.double() - dxw.repeat(5, 1)).norm()) <= 4 * _round(F16) * float(dxw.repeat(5, 1).norm())
