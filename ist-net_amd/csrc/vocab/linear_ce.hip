@@ -1035,6 +1035,13 @@ inline bool small_ce(long long n, int d, int v) {
 // 46 / 255 us, 32 rows 38 / 159 and 47 / 265 us (64 rows would take 53 / 421, and 48 / 274 here); float32, one row 57 / 186 and
 // 253 / 506 us, 32 rows 101 / 351 and 260 / 512 us.  8000 classes x 200, bfloat16, 32 rows with backward: 42 and 49 us.
 inline bool few_ce(long long n, int d, int v) { return !small_ce(n, d, v) && n <= kFewRowsCe && n * v <= (1ll << 28); }
+// Problems that linear_ce_classes.hip serves: w in float32 within 64 KB.  Forward and backward in a graph, float32 / bfloat16, there and
+// here: 32768 x 128, 64 classes 50 / 54 and 76 / 62 us, 6 classes 29 / 28 and 74 / 60 us; 300000 x 64, 10 classes 78 / 90 and
+// 315 / 198 us; 8192 x 256, 40 classes 44 / 46 and 69 / 57 us; 4000 x 32, 33 classes 28 / 38 and 41 / 39 us; beyond it 8192 x 1024, 64
+// classes 161 / 124 and 149 / 85 us.  Four or five launches instead of nine.
+inline bool class_ce(long long n, int d, int v) {
+  return n > kSmallSide && v <= 64 && round_up(v, 16) * d <= 16384 && n * v <= (1ll << 28);
+}
 
 struct Keep {      // what the backward needs, in the caller's `keep`
   long long np, kp, vp, planes;
@@ -1142,12 +1149,14 @@ extern "C" int istnet_linear_ce_keep_kib(long long n, int d, int v, int dtype, i
   if (!ce_ok(n, d, v, dtype)) return -1;
   if (small_ce(n, d, v)) return (int)((vocab_small_ce_keep(n, v) + 1023) / 1024);
   if (few_ce(n, d, v)) return (int)((vocab_few_ce_keep(n, v, train) + 1023) / 1024);
+  if (class_ce(n, d, v)) return (int)((vocab_class_ce_keep(n, v, train) + 1023) / 1024);
   return (int)((keep_plan(n, d, v, dtype, direct_w(n, d, dtype, train, w, ldw)).bytes + 1023) / 1024);
 }
 extern "C" int istnet_linear_ce_scratch_kib(long long n, int d, int v, int dtype, int reduction, int backward) {
   if (!ce_ok(n, d, v, dtype) || reduction < 0 || reduction > 2) return -1;
   if (small_ce(n, d, v)) return 0;
   if (few_ce(n, d, v)) return (int)((vocab_few_ce_scratch(n, d, v, dtype, backward) + 1023) / 1024);
+  if (class_ce(n, d, v)) return (int)((vocab_class_ce_scratch(n, d, v, dtype, backward) + 1023) / 1024);
   const Keep k = keep_plan(n, d, v, dtype, false);
   return (int)(((backward ? backward_plan(k, n, d, v, dtype, reduction).bytes : forward_plan(k, n, v).bytes) + 1023) / 1024);
 }
@@ -1162,6 +1171,8 @@ extern "C" int istnet_linear_ce_forward(long long n, int d, int v, int dtype, in
     return vocab_small_ce_forward((int)n, d, v, dtype, idx64, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, st);
   if (few_ce(n, d, v))
     return vocab_few_ce_forward((int)n, d, v, dtype, idx64, train, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, ws, st);
+  if (class_ce(n, d, v))
+    return vocab_class_ce_forward((int)n, d, v, dtype, idx64, train, x, ldx, w, ldw, bias, target, ignore, reduction, loss, keep, ws, st);
   const bool direct = direct_w(n, d, dtype, train, w, ldw), scaled = dtype == ISTNET_VOCAB_F32 || (dtype == ISTNET_VOCAB_BF16 && !direct);
   const Keep k = keep_plan(n, d, v, dtype, direct);
   const Forward f = forward_plan(k, n, v);
@@ -1235,6 +1246,7 @@ extern "C" int istnet_linear_ce_backward(long long n, int d, int v, int dtype, c
   if (!dx && !dw && !db) return 0;
   if (small_ce(n, d, v)) return vocab_small_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, dx, dw, db, st);
   if (few_ce(n, d, v)) return vocab_few_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, ws, dx, dw, db, st);
+  if (class_ce(n, d, v)) return vocab_class_ce_backward((int)n, d, v, dtype, x, ldx, w, ldw, reduction, gout, keep, ws, dx, dw, db, st);
   const Keep k = keep_plan(n, d, v, dtype, false);
   const Backward b = backward_plan(k, n, d, v, dtype, reduction);
   char *kb = (char*)keep, *wb = (char*)ws, *xp = kb + k.xp, *wp = kb + k.wp, *dz = wb + b.dz, *xb = xp;

@@ -16,37 +16,12 @@
 // row of bfloat16, but 203 us for 16.
 #include <algorithm>
 
-#include "vocab_common.h"
+#include "linear_ce_direct.h"
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kClasses = 64;           // of a workgroup, forward
 constexpr int kPitch = kClasses + 4;
-
-// one step of K: 64 bytes of a row, lane group g = lane / 16 has sixteen of them; which K they are does not matter as long as both
-// operands agree
-template <typename T> constexpr int kStep = 64 / (int)sizeof(T);
-template <typename T> __device__ __forceinline__ f32x4 multiply(const u32x4& a, const u32x4& b, f32x4 c) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[k]), __uint_as_float(b[k]), c, 0, 0, 0);
-    return c;
-  } else if constexpr (__is_same(T, bf16)) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
-  }
-}
-// sixteen bytes of which `left` elements belong to the row, zeros behind them
-template <typename T> __device__ __forceinline__ u32x4 load_raw(const T* p, int left) {
-  float f[kVec<T>];
-  load_part(p, left, f);
-  return pack<T>(f);
-}
 
 struct Part { float m, s; };      // other classes' largest logit, sum of exp(z - m)
 __device__ __forceinline__ Part merge(Part p, Part q) {
@@ -139,7 +114,7 @@ __global__ __launch_bounds__(256) void ce_few_logits_kernel(int n, int d, int v,
     }
     if (bias) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += c + e < v ? to_f32(bias[c + e]) : 0.f;
+      for (int e = 0; e < 4; ++e) y[e] += to_f32(bias[min(c + e, v - 1)]);
     }
     if (z && row < n && c < ldz) *reinterpret_cast<f32x4*>(z + row * ldz + c) = y;
     const long long t = row < n ? load_index(target, row, idx64) : -1;
@@ -271,14 +246,17 @@ __global__ __launch_bounds__(256, 2) void ce_few_grads_kernel(FewGrads f) {
         const T* at = w + col;
         const int last = f.v - 1, by = 4 * f.teams;
         int c = team * 4;
-        if (mine == G && (first + G) * 16 * V <= f.d) {
+        if (mine > 0 && (f.d % V == 0 || (first + G) * 16 * V <= f.d)) {
           constexpr int U = 8 / G;
+          long long to[G];      // (lanes behind the last column read others, for sums that are not stored)
+#pragma unroll
+          for (int q = 0; q < G; ++q) to[q] = col + q * 16 * V < f.d ? q * 16 * V : -(long long)col;
           for (; c + (U - 1) * by < count; c += U * by) {
             u32x4 raw[U][G];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-              for (int q = 0; q < G; ++q) raw[u][q] = load16(at + min(c0 + c + u * by + g, last) * f.ldw + q * 16 * V);
+              for (int q = 0; q < G; ++q) raw[u][q] = load16(at + min(c0 + c + u * by + g, last) * f.ldw + to[q]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -379,8 +357,6 @@ __global__ __launch_bounds__(256) void ce_few_join_kernel(int n, int d, int slab
   for (int e = 0; e < 4; ++e)
     if (c + e < d) dx[(long long)i * d + c + e] = from_f32<T>(tgt[i] == -2 ? 0.f : x[e]);
 }
-
-inline long long round_up(long long x, long long m) { return (x + m - 1) / m * m; }
 
 struct FewKeep { long long ldz, z, stat, tgt, loss, bytes; };
 inline FewKeep few_keep(long long n, int v, int train) {

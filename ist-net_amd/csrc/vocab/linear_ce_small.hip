@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * kWaves) void ce_small_logits_kernel(int n, int
     f32x4 y = s;
     if (bias) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] += c + i < v ? to_f32(bias[c + i]) : 0.f;
+      for (int i = 0; i < 4; ++i) y[i] += to_f32(bias[min(c + i, v - 1)]);
     }
     *reinterpret_cast<f32x4*>(z + (long long)r * vp + c) = y;
   }

@@ -8,8 +8,8 @@
 
 #include "../../../include/istnet_vocab.h"
 
-// The cross entropy of few rows (linear_ce_few.hip) and of small problems (linear_ce_small.hip), called by the entry points of
-// linear_ce.hip.
+// The cross entropy of few rows (linear_ce_few.hip), of few classes (linear_ce_classes.hip) and of small problems
+// (linear_ce_small.hip), called by the entry points of linear_ce.hip.
 constexpr int kFewRowsCe = 32;
 long long vocab_few_ce_keep(long long n, int v, int train);
 long long vocab_few_ce_scratch(long long n, int d, int v, int dtype, int backward);
@@ -18,6 +18,13 @@ int vocab_few_ce_forward(int n, int d, int v, int dtype, int idx64, int train, c
                          void* ws, hipStream_t st);
 int vocab_few_ce_backward(int n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw, int reduction,
                           const float* gout, const void* keep, void* ws, void* dx, void* dw, void* db, hipStream_t st);
+long long vocab_class_ce_keep(long long n, int v, int train);
+long long vocab_class_ce_scratch(long long n, int d, int v, int dtype, int backward);
+int vocab_class_ce_forward(int n, int d, int v, int dtype, int idx64, int train, const void* x, long long ldx, const void* w,
+                           long long ldw, const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep,
+                           void* ws, hipStream_t st);
+int vocab_class_ce_backward(int n, int d, int v, int dtype, const void* x, long long ldx, const void* w, long long ldw, int reduction,
+                            const float* gout, const void* keep, void* ws, void* dx, void* dw, void* db, hipStream_t st);
 long long vocab_small_ce_keep(long long n, int v);
 int vocab_small_ce_forward(int n, int d, int v, int dtype, int idx64, const void* x, long long ldx, const void* w, long long ldw,
                            const void* bias, const void* target, long long ignore, int reduction, float* loss, void* keep, hipStream_t st);

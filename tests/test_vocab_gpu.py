@@ -609,6 +609,43 @@ def test_linear_ce_few_rows(n, d, v, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,d,v", [(1025, 1, 1), (1100, 33, 6), (2000, 64, 16), (4097, 130, 17), (1500, 520, 64), (5000, 67, 64), (30001, 16, 40),
+                                   (1281, 1030, 9), (70000, 128, 64), (3000, 20, 65)])
+def test_linear_ce_few_classes(n, d, v, dtype):
+    for i, reduction in enumerate(["mean", "none", "sum"]):
+        x, w, b, t = _ce_inputs(n, d, v, dtype, n + d + v + i, bias=i != 1, ignored=0.3, index=(torch.int32, torch.int64)[i % 2])
+        wide = torch.zeros(n, d + 3, device=DEV, dtype=dtype)
+        wide[:, 1:1 + d] = x
+        _check_ce(wide[:, 1:1 + d] if i == 2 else x, w, b, t, reduction)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_linear_ce_few_classes_masks(dtype, reduction):
+    x, w, b, t = _ce_inputs(1300, 48, 37, dtype, 28, ignored=0.2)
+    t[5], t[1299], t[7], t[0] = IGNORE, IGNORE, 36, 1
+    x[5], x[1299] = NAN, INF
+    b[16:32], b[3] = -INF, -INF
+    t = torch.where(((t >= 16) & (t < 32)) | (t == 3), 9, t)
+    loss, grads = _check_ce(x, w, b, t, reduction)
+    assert all(g.isfinite().all() for g in grads) and (grads[0][[5, 1299]] == 0).all()
+    loss, grads = _check_ce(x[:1200], w, b, torch.full_like(t[:1200], 7), reduction, ignore=7)      # nothing counts
+    assert (loss == 0).all() if reduction != "mean" else loss.isnan()
+    assert all((g == 0).all() for g in grads)
+    t[200], t[1000] = 37, -1
+    xr, wr, br = x.detach().requires_grad_(), w.detach().requires_grad_(), b.detach().requires_grad_()
+    loss = losses.LinearCrossEntropy(xr, w, t, b, reduction=reduction)
+    (dx,) = torch.autograd.grad(loss, xr, torch.ones_like(loss))
+    assert dx.isnan().all(1).nonzero().flatten().tolist() == [200, 1000] and dx[[0, 1, 4, 5, 1299]].isfinite().all()
+    assert loss.isnan().sum() == (2 if reduction == "none" else 1)
+    t[200], t[1000] = 5, 6
+    loss = losses.LinearCrossEntropy(xr, wr, t, br, reduction=reduction)      # only one of the gradients
+    g = torch.ones_like(loss)
+    alone = [torch.autograd.grad(loss, a, g, retain_graph=True)[0] for a in (xr, wr, br)]
+    assert all(torch.equal(p, q) for p, q in zip(alone, torch.autograd.grad(loss, (xr, wr, br), g)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 def test_linear_ce_few_rows_masks(dtype, reduction):
     x, w, b, t = _ce_inputs(11, 48, 2600, dtype, 27, ignored=0.0)
