@@ -15,13 +15,29 @@ namespace {
 
 constexpr int kMaxSlots = 256;
 constexpr int kShortRow = 2048;
-constexpr float kLog2e = 1.4426950408889634f;
 
-struct Stat { float m, s; };      // maximum, sum of exp2((x - maximum) c)
+// exp(x / T) = 2^(x c), c = log2(e) / T.  float32 logits: with what the product x c and c itself lose (a few 2^-24 of x c, 2e-6 of the result
+// where x / T is 20), because p - q cancels; 16-bit logits have roundings of their own and two instructions less.
+struct Expo { float hi, lo; };
+__device__ __forceinline__ Expo expo_of(float temp) {
+  const double c = 1.4426950408889634 / (double)temp;
+  const float hi = (float)c;
+  return {hi, (float)(c - (double)hi)};
+}
+template <typename T> __device__ __forceinline__ float exp_of(float x, Expo c) {
+  const float y = x * c.hi;
+  if constexpr (sizeof(T) == 4) {
+    const float lo = __builtin_fmaf(x, c.lo, __builtin_fmaf(x, c.hi, -y)), e = exp2_raw(y);
+    return y > -INFINITY ? __builtin_fmaf(e, lo * 0.6931471805599453f, e) : e;      // (x = -inf: lo is NaN)
+  }
+  return exp2_raw(y);
+}
 
-__device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
-  const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;      // nothing seen yet: exp2(-inf) = 0, not NaN
-  return {m, a.s * exp2_raw((a.m - ref) * c) + b.s * exp2_raw((b.m - ref) * c)};
+struct Stat { float m, s; };      // maximum, sum of exp((x - maximum) / T)
+
+template <typename T> __device__ __forceinline__ Stat merge(Stat a, Stat b, Expo c) {
+  const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;      // nothing seen yet: exp(-inf) = 0, not NaN
+  return {m, a.s * exp_of<T>(a.m - ref, c) + b.s * exp_of<T>(b.m - ref, c)};
 }
 
 template <int THREADS> __device__ __forceinline__ float block_max(float x, float* tmp) {
@@ -49,6 +65,19 @@ template <int THREADS> __device__ __forceinline__ float block_sum(float x, float
   return x;
 }
 
+template <int THREADS> __device__ __forceinline__ double block_sum(double x, double* tmp) {
+  x = wave_sum(x);
+  if constexpr (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = tmp[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) x += tmp[w];
+    __syncthreads();
+  }
+  return x;
+}
+
 // any used slot in the row?  (every thread gets the answer)
 template <int THREADS>
 __device__ __forceinline__ bool row_counts(const void* idx, long long row, int k, int idx64, float* tmp) {
@@ -59,7 +88,7 @@ __device__ __forceinline__ bool row_counts(const void* idx, long long row, int k
 
 // running maximum and sum of z[a, e) over the workgroup's threads
 template <typename T, int THREADS>
-__device__ __forceinline__ Stat scan_row(const T* __restrict__ z, int a, int e, float c, float* tmp) {
+__device__ __forceinline__ Stat scan_row(const T* __restrict__ z, int a, int e, Expo c, float* tmp) {
   constexpr int V = kVec<T>, U = 4;      // four sixteen-byte loads in flight per thread
   Stat st = {-INFINITY, 0.f};
   int at = a + threadIdx.x * V;
@@ -73,11 +102,11 @@ __device__ __forceinline__ Stat scan_row(const T* __restrict__ z, int a, int e, 
 #pragma unroll
       for (int i = 0; i < V; ++i) m = fmaxf(m, f[u][i]);
     const float ref = m == -INFINITY ? 0.f : m;
-    float s = st.s * exp2_raw((st.m - ref) * c);
+    float s = st.s * exp_of<T>(st.m - ref, c);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < V; ++i) s += exp2_raw((f[u][i] - ref) * c);
+      for (int i = 0; i < V; ++i) s += exp_of<T>(f[u][i] - ref, c);
     st = {m, s};
   }
   for (; at < e; at += THREADS * V) {
@@ -88,18 +117,18 @@ __device__ __forceinline__ Stat scan_row(const T* __restrict__ z, int a, int e, 
 #pragma unroll
     for (int i = 0; i < V; ++i) m = i < left ? fmaxf(m, f[i]) : m;
     const float ref = m == -INFINITY ? 0.f : m;
-    float s = st.s * exp2_raw((st.m - ref) * c);
+    float s = st.s * exp_of<T>(st.m - ref, c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s += i < left ? exp2_raw((f[i] - ref) * c) : 0.f;
+    for (int i = 0; i < V; ++i) s += i < left ? exp_of<T>(f[i] - ref, c) : 0.f;
     st = {m, s};
   }
   const float m = block_max<THREADS>(st.m, tmp), ref = m == -INFINITY ? 0.f : m;
-  return {m, block_sum<THREADS>(st.s * exp2_raw((st.m - ref) * c), tmp)};
+  return {m, block_sum<THREADS>(st.s * exp_of<T>(st.m - ref, c), tmp)};
 }
 
 // sum of exponentials of a row beside ONE of its largest logits, m: what 1 + rest rounds away where the largest is almost certain
 template <typename T, int THREADS>
-__device__ __forceinline__ float rest_of_row(const T* __restrict__ z, int v, float m, float c, float* tmp) {
+__device__ __forceinline__ float rest_of_row(const T* __restrict__ z, int v, float m, Expo c, float* tmp) {
   constexpr int V = kVec<T>;
   float rest = 0.f, largest = 0.f;
   for (int at = threadIdx.x * V; at < v; at += THREADS * V) {
@@ -108,7 +137,7 @@ __device__ __forceinline__ float rest_of_row(const T* __restrict__ z, int v, flo
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       if (at + i < v) {
-        if (f[i] == m) largest += 1.f; else rest += exp2_raw((f[i] - m) * c);
+        if (f[i] == m) largest += 1.f; else rest += exp_of<T>(f[i] - m, c);
       }
     }
   }
@@ -116,12 +145,14 @@ __device__ __forceinline__ float rest_of_row(const T* __restrict__ z, int v, flo
   return rest + (block_sum<THREADS>(largest, tmp) - 1.f);
 }
 
-// the row's loss from its statistics: teacher's softmax, the k picked logits, weights of the slots for the backward
+// the row's loss from its statistics: teacher's softmax, the k picked logits, weights of the slots for the backward.  The logarithms
+// cancel in q (log q - log p): what there are k of is held in double.
+struct Slots { double t[kMaxSlots], tmp[4]; float q[kMaxSlots]; int idx[kMaxSlots]; };
 template <typename T, int THREADS>
 __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k, int ttype, int idx64, const void* __restrict__ top,
                                            const void* __restrict__ idx, long long row, float temp, Stat st, bool counts,
                                            float* __restrict__ row_loss, float* __restrict__ stats, float* __restrict__ q, float* tmp,
-                                           float* lq, int* lidx) {
+                                           Slots& sl) {
   const int tid = threadIdx.x;
   if (!counts) {
     for (int j = tid; j < k; j += THREADS) q[row * k + j] = 0.f;
@@ -129,50 +160,54 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ z, int v, int k
     return;
   }
   // rows short enough for one wave are looked at once more (they are in the caches); longer ones keep the rounding of 1 + rest, 2^-24
-  const float rest = fabsf(st.m) == INFINITY ? kNaN : THREADS == 64 && v <= kShortRow ? rest_of_row<T, THREADS>(z, v, st.m, kLog2e / temp, tmp)
-                                                                                : st.s - 1.f;
+  float rest = st.s - 1.f;
+  if (fabsf(st.m) == INFINITY) rest = kNaN;
+  else if (THREADS == 64 && v <= kShortRow) rest = rest_of_row<T, THREADS>(z, v, st.m, expo_of(temp), tmp);
   float tm = -INFINITY, bad = 0.f;
   for (int j = tid; j < k; j += THREADS) {
     const long long id = load_index(idx, row * k + j, idx64);
     float t = -INFINITY;
     if (id != -1) {
-      t = (ttype == ISTNET_VOCAB_F32 ? ((const float*)top)[row * k + j]
-           : ttype == ISTNET_VOCAB_BF16 ? to_f32(((const bf16*)top)[row * k + j]) : (float)((const f16*)top)[row * k + j]) / temp;
+      t = ttype == ISTNET_VOCAB_F32 ? ((const float*)top)[row * k + j]
+          : ttype == ISTNET_VOCAB_BF16 ? to_f32(((const bf16*)top)[row * k + j]) : (float)((const f16*)top)[row * k + j];
       if (id < -1 || id >= v || t != t) bad = 1.f;
     }
-    lq[j] = t;
-    lidx[j] = (id < 0 || id >= v) ? -1 : (int)id;
+    sl.t[j] = t;
+    sl.idx[j] = (id < 0 || id >= v) ? -1 : (int)id;
     tm = fmaxf(tm, t);
   }
   bad = block_max<THREADS>(bad, tmp);
   tm = block_max<THREADS>(tm, tmp);
   if (fabsf(tm) == INFINITY) bad = 1.f;      // no softmax of the teacher's
-  float ts = 0.f;
-  for (int j = tid; j < k; j += THREADS) ts += lidx[j] >= 0 ? expf(lq[j] - tm) : 0.f;
-  ts = block_sum<THREADS>(ts, tmp);
-  const float log_ts = logf(ts), log_s = log1pf(rest);
-  float loss = 0.f;
-  for (int j = tid; j < k; j += THREADS) {
-    const float t = lq[j];
-    float qj = 0.f;
-    if (lidx[j] >= 0) {
-      qj = expf(t - tm) / ts;
-      // a slot of the teacher's logit -inf weighs nothing, whatever the student says
-      if (!(qj == 0.f)) loss += qj * ((t - tm - log_ts) - ((to_f32(z[lidx[j]]) - st.m) / temp - log_s));
-    }
-    lq[j] = qj;      // each thread overwrites only what it alone has read since the barrier
+  const double by = 1.0 / (double)temp;
+  double ts = 0.0;
+  for (int j = tid; j < k; j += THREADS) {      // each thread reads and writes its own slots until the barrier
+    sl.t[j] = (sl.t[j] - (double)tm) * by;
+    ts += sl.idx[j] >= 0 ? exp(sl.t[j]) : 0.0;
   }
-  loss = block_sum<THREADS>(loss, tmp);
+  ts = block_sum<THREADS>(ts, sl.tmp);
+  const double logs = log1p((double)rest) - log(ts);
+  double loss = 0.0;
+  for (int j = tid; j < k; j += THREADS) {
+    double qj = 0.0;
+    if (sl.idx[j] >= 0) {
+      qj = exp(sl.t[j]) / ts;
+      // a slot of the teacher's logit -inf weighs nothing, whatever the student says
+      if (!(qj == 0.0)) loss += qj * (sl.t[j] - ((double)to_f32(z[sl.idx[j]]) - (double)st.m) * by + logs);
+    }
+    sl.q[j] = (float)qj;
+  }
+  loss = block_sum<THREADS>(loss, sl.tmp);
   __syncthreads();
   for (int j = tid; j < k; j += THREADS) {      // slots of the same class share their weights' sum, in slot order
     float sum = 0.f;
-    for (int i = 0; i < k; ++i) sum += lidx[i] == lidx[j] ? lq[i] : 0.f;
-    q[row * k + j] = lidx[j] >= 0 ? sum : 0.f;
+    for (int i = 0; i < k; ++i) sum += sl.idx[i] == sl.idx[j] ? sl.q[i] : 0.f;
+    q[row * k + j] = sl.idx[j] >= 0 ? sum : 0.f;
   }
   if (tid == 0) {
     stats[2 * row] = st.m;
     stats[2 * row + 1] = bad > 0.f ? kNaN : rest;
-    row_loss[row] = bad > 0.f ? kNaN : temp * temp * loss;
+    row_loss[row] = bad > 0.f ? kNaN : (float)((double)temp * (double)temp * loss);
   }
 }
 
@@ -184,15 +219,14 @@ __global__ __launch_bounds__(THREADS) void distill_rows_kernel(int v, int k, int
                                                                Stat* __restrict__ part, float* __restrict__ row_loss,
                                                                float* __restrict__ stats, float* __restrict__ q) {
   __shared__ float tmp[THREADS / 64];
-  __shared__ float lq[kMaxSlots];
-  __shared__ int lidx[kMaxSlots];
+  __shared__ Slots sl;
   const long long row = blockIdx.x / splits;
   const int a = (int)(blockIdx.x % splits) * width, e = min(v, a + width);
   const bool counts = row_counts<THREADS>(idx, row, k, idx64, tmp);
   Stat st = {-INFINITY, 0.f};
-  if (counts) st = scan_row<T, THREADS>(z + row * ldz, a, e, kLog2e / temp, tmp);
+  if (counts) st = scan_row<T, THREADS>(z + row * ldz, a, e, expo_of(temp), tmp);
   if (splits == 1)
-    finish_row<T, THREADS>(z + row * ldz, v, k, ttype, idx64, top, idx, row, temp, st, counts, row_loss, stats, q, tmp, lq, lidx);
+    finish_row<T, THREADS>(z + row * ldz, v, k, ttype, idx64, top, idx, row, temp, st, counts, row_loss, stats, q, tmp, sl);
   else if (threadIdx.x == 0)
     part[blockIdx.x] = st;
 }
@@ -203,18 +237,17 @@ __global__ __launch_bounds__(64) void distill_join_kernel(int v, int k, int ttyp
                                                           int splits, const Stat* __restrict__ part, float* __restrict__ row_loss,
                                                           float* __restrict__ stats, float* __restrict__ q) {
   __shared__ float tmp[1];
-  __shared__ float lq[kMaxSlots];
-  __shared__ int lidx[kMaxSlots];
+  __shared__ Slots sl;
   const long long row = blockIdx.x;
-  const float c = kLog2e / temp;
+  const Expo c = expo_of(temp);
   const bool counts = row_counts<64>(idx, row, k, idx64, tmp);
   Stat st = {-INFINITY, 0.f};
   if (counts) {
-    for (int p = threadIdx.x; p < splits; p += 64) st = merge(st, part[row * splits + p], c);
+    for (int p = threadIdx.x; p < splits; p += 64) st = merge<T>(st, part[row * splits + p], c);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) st = merge(st, {__shfl_xor(st.m, o), __shfl_xor(st.s, o)}, c);
+    for (int o = 32; o; o >>= 1) st = merge<T>(st, {__shfl_xor(st.m, o), __shfl_xor(st.s, o)}, c);
   }
-  finish_row<T, 64>(z + row * ldz, v, k, ttype, idx64, top, idx, row, temp, st, counts, row_loss, stats, q, tmp, lq, lidx);
+  finish_row<T, 64>(z + row * ldz, v, k, ttype, idx64, top, idx, row, temp, st, counts, row_loss, stats, q, tmp, sl);
 }
 
 // sum of the rows' losses and number of counted rows, in double, one workgroup
@@ -249,7 +282,8 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
   constexpr int V = kVec<T>;
   const long long row = blockIdx.x / splits;
   const int a = (int)(blockIdx.x % splits) * width, e = min(v, a + width);
-  const float m = stats[2 * row], rest = stats[2 * row + 1], inv_s = 1.f / (1.f + rest), c = kLog2e / temp;
+  const float m = stats[2 * row], rest = stats[2 * row + 1], inv_s = 1.f / (1.f + rest);
+  const Expo c = expo_of(temp);
   T* out = dz + row * v;
   if (rest == -1.f) {      // a row without a teacher: its logits are not looked at
     const float zero[V] = {};
@@ -268,7 +302,7 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[u][i] = gp * exp2_raw((f[u][i] - m) * c);
+      for (int i = 0; i < V; ++i) f[u][i] = gp * exp_of<T>(f[u][i] - m, c);
       store16(out + at + u * THREADS * V, pack<T>(f[u]));
     }
   }
@@ -276,7 +310,7 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
     float f[V];
     load_part(in + at, e - at, f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = gp * exp2_raw((f[i] - m) * c);
+    for (int i = 0; i < V; ++i) f[i] = gp * exp_of<T>(f[i] - m, c);
     store_part(out + at, e - at, f);
   }
   // the teacher's classes: p - q is formed before it is rounded, as (e - q - q rest) / (1 + rest), which keeps its precision where
@@ -285,7 +319,7 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
   for (int j = threadIdx.x; j < k; j += THREADS) {
     const long long id = load_index(idx, row * k + j, idx64);
     if (id >= a && id < e) {
-      const float qj = q[row * k + j], ej = exp2_raw((to_f32(in[id]) - m) * c);
+      const float qj = q[row * k + j], ej = exp_of<T>(to_f32(in[id]) - m, c);
       out[id] = from_f32<T>(gp * __builtin_fmaf(-qj, rest, ej - qj));
     }
   }
