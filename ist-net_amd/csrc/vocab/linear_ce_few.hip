@@ -377,7 +377,9 @@ inline FewPlan few_plan(long long n, int d, int v, int dtype) {
   p.teams = p.groups == 1 ? 4 : p.groups == 2 ? 2 : 1;
   p.chunk = (int)std::min<long long>(kChunk, round_up((v + 511) / 512, 16));      // some 512 workgroups
   p.subs = (v + p.chunk - 1) / p.chunk;
-  p.dxs = std::min(p.subs, (n <= 16 ? 512 : 256) / p.teams);      // slabs that are small beside w
+  // slabs that are small beside w: 64 MB, or 32 of them where there are that many features
+  const long long most = std::max<long long>(32, (64ll << 20) / (4 * n * d * p.teams));
+  p.dxs = (int)std::min<long long>({p.subs, (n <= 16 ? 512 : 256) / p.teams, most});
   return p;
 }
 #define FEW_BLOCKS(n, NB, ...)                                           \

@@ -2,7 +2,8 @@
 // launches: below some 10^8 multiplications those launches, not the products, are what a call costs).  gfx950, wave64.
 //
 // Four launches: the logits (kept: a few megabytes here), row statistics and p - t in their place, the loss, and ONE launch for dx, dw
-// and db.  Products on the float32 matrix instructions (v_mfma_f32_32x32x2_f32), operands straight from memory into registers whatever
+// and db; three up to 64 rows, two where the logits are one tile (32 rows, 64 classes): a launch is 4 us of the host's, and while the
+// host is at it the engine's thread falls asleep.  Products on the float32 matrix instructions (v_mfma_f32_32x32x2_f32), operands straight from memory into registers whatever
 // their type, stride or alignment; sixteen waves split K and join through LDS in a fixed order.  Everything is float32, rounded once.
 // 32 x 512 float32, six classes: 8 + 4 + 3 + 7 us, each a few memory latencies; a call and its gradient take the host 120 us.
 #include <algorithm>
@@ -95,12 +96,58 @@ __device__ __forceinline__ bool counts(const void* target, long long i, int idx6
   return load_index(target, i, idx64) != ignore;
 }
 
-// z (n, vp) = x w^T + bias; a lane's K of one step of 8: 4 (lane / 32) .. + 3
+// one wave: loss of row i, and p - t in its logits' place (zeros behind the last class and in rows that do not count)
+__device__ __forceinline__ float small_row(int i, int v, int vp, const void* target, int idx64, long long ignore, float* z,
+                                           float* row_loss, int* on) {
+  const int lane = threadIdx.x & 63;
+  const long long t = load_index(target, i, idx64);
+  float* row = z + (long long)i * vp;
+  if (t == ignore || t < 0 || t >= v) {
+    const float fill = t == ignore ? 0.f : kNaN;
+    for (int c = lane; c < vp; c += 64) row[c] = c < v ? fill : 0.f;
+    if (lane == 0) { row_loss[i] = fill; on[i] = t != ignore; }
+    return fill;
+  }
+  float m = -INFINITY;      // of the other classes
+  for (int c = lane; c < v; c += 64) m = c == t ? m : fmaxf(m, row[c]);
+  m = wave_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int c = lane; c < v; c += 64) s += c == t ? 0.f : expf(row[c] - ref);
+  s = wave_sum(s);
+  const Row r = row_of(m, s, row[t]);
+  for (int c = lane; c < vp; c += 64) row[c] = c >= v ? 0.f : c == t ? r.at_target : r.inv * expf(row[c] - r.top);
+  if (lane == 0) { row_loss[i] = r.loss; on[i] = 1; }
+  return r.loss;
+}
+
+// sixteen waves: all rows, their sum and number
+__device__ __forceinline__ void small_finish(int n, int v, int vp, const void* target, int idx64, long long ignore, int reduction, float* z,
+                                             float* row_loss, int* on, float* loss, float* count, double (&tmp)[2][16]) {
+  const int wave = threadIdx.x >> 6;
+  double sum = 0.0, rows = 0.0;
+  for (int i = wave; i < n; i += 16) {
+    sum += small_row(i, v, vp, target, idx64, ignore, z, row_loss, on);
+    rows += counts(target, i, idx64, ignore);
+  }
+  if ((threadIdx.x & 63) == 0) { tmp[0][wave] = sum; tmp[1][wave] = rows; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = rows = 0.0;
+    for (int w = 0; w < 16; ++w) { sum += tmp[0][w]; rows += tmp[1][w]; }
+    if (reduction) *loss = (float)(reduction == 1 ? sum / rows : sum);
+    *count = (float)rows;
+  }
+}
+
+// z (n, vp) = x w^T + bias; a lane's K of one step of 8: 4 (lane / 32) .. + 3.  The only workgroup does the rest of the forward as well.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void ce_small_logits_kernel(int n, int d, int v, int vp, const T* __restrict__ x, long long ldx,
                                                                       const T* __restrict__ w, long long ldw, const T* __restrict__ bias,
                                                                       const void* __restrict__ target, int idx64, long long ignore,
-                                                                      float* __restrict__ z) {
+                                                                      int reduction, float* __restrict__ z,
+                                                                      float* __restrict__ row_loss, int* __restrict__ on_row,
+                                                                      float* __restrict__ loss, float* __restrict__ count) {
   __shared__ __attribute__((aligned(16))) float lds[kWaves * kTN * kPitch];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tv = (v + kTM - 1) / kTM;
   const int v0 = (int)(blockIdx.x % tv) * kTM, n0 = (int)(blockIdx.x / tv) * kTN;
@@ -127,32 +174,26 @@ __global__ __launch_bounds__(64 * kWaves) void ce_small_logits_kernel(int n, int
     }
     *reinterpret_cast<f32x4*>(z + (long long)r * vp + c) = y;
   }
+  if (gridDim.x > 1) return;
+  __shared__ double tmp[2][16];
+  __syncthreads();
+  small_finish(n, v, vp, target, idx64, ignore, reduction, z, row_loss, on_row, loss, count, tmp);
 }
 
-// one wave per row: loss, and p - t in the logits' place (zeros behind the last class and in rows that do not count)
 __global__ __launch_bounds__(256) void ce_small_rows_kernel(int n, int v, int vp, const void* __restrict__ target, int idx64,
                                                             long long ignore, float* __restrict__ z, float* __restrict__ row_loss,
                                                             int* __restrict__ on) {
-  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= n) return;
-  const long long t = load_index(target, i, idx64);
-  float* row = z + (long long)i * vp;
-  if (t == ignore || t < 0 || t >= v) {
-    const float fill = t == ignore ? 0.f : kNaN;
-    for (int c = lane; c < vp; c += 64) row[c] = c < v ? fill : 0.f;
-    if (lane == 0) { row_loss[i] = fill; on[i] = t != ignore; }
-    return;
-  }
-  float m = -INFINITY;      // of the other classes
-  for (int c = lane; c < v; c += 64) m = c == t ? m : fmaxf(m, row[c]);
-  m = wave_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  for (int c = lane; c < v; c += 64) s += c == t ? 0.f : expf(row[c] - ref);
-  s = wave_sum(s);
-  const Row r = row_of(m, s, row[t]);
-  for (int c = lane; c < vp; c += 64) row[c] = c >= v ? 0.f : c == t ? r.at_target : r.inv * expf(row[c] - r.top);
-  if (lane == 0) { row_loss[i] = r.loss; on[i] = 1; }
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i < n) small_row(i, v, vp, target, idx64, ignore, z, row_loss, on);
+}
+
+// up to 64 rows: rows and total in one launch
+__global__ __launch_bounds__(1024) void ce_small_finish_kernel(int n, int v, int vp, const void* __restrict__ target, int idx64,
+                                                               long long ignore, int reduction, float* __restrict__ z,
+                                                               float* __restrict__ row_loss, int* __restrict__ on,
+                                                               float* __restrict__ loss, float* __restrict__ count) {
+  __shared__ double tmp[2][16];
+  small_finish(n, v, vp, target, idx64, ignore, reduction, z, row_loss, on, loss, count, tmp);
 }
 
 __global__ __launch_bounds__(1024) void ce_small_total_kernel(int n, int reduction, const float* __restrict__ row_loss,
@@ -272,13 +313,20 @@ int vocab_small_ce_forward(int n, int d, int v, int dtype, int idx64, const void
   const SmallKeep k = small_keep(n, v);
   float *z = (float*)((char*)keep + k.z), *row_loss = reduction == 0 ? loss : (float*)((char*)keep + k.loss);
   int* on = (int*)((char*)keep + k.on);
-  VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_small_logits_kernel<T>),
-                                              dim3(((v + kTM - 1) / kTM) * ((n + kTN - 1) / kTN)), dim3(64 * kWaves), 0, st, n, d, v,
-                                              (int)k.vp, (const T*)x, ldx, (const T*)w, ldw, (const T*)bias, target, idx64, ignore, z));
-  hipLaunchKernelGGL(ce_small_rows_kernel, dim3((n + 3) / 4), dim3(256), 0, st, n, v, (int)k.vp, target, idx64, ignore, z, row_loss, on);
-  if (reduction != 0)
-    hipLaunchKernelGGL(ce_small_total_kernel, dim3(1), dim3(1024), 0, st, n, reduction, row_loss, on, loss,
-                       (float*)((char*)keep + k.count));
+  float* count = (float*)((char*)keep + k.count);
+  const int wgs = ((v + kTM - 1) / kTM) * ((n + kTN - 1) / kTN);
+  VOCAB_DISPATCH(dtype, T, hipLaunchKernelGGL(HIP_KERNEL_NAME(ce_small_logits_kernel<T>), dim3(wgs), dim3(64 * kWaves), 0, st, n, d, v,
+                                              (int)k.vp, (const T*)x, ldx, (const T*)w, ldw, (const T*)bias, target, idx64, ignore,
+                                              reduction, z, row_loss, on, loss, count));
+  if (wgs == 1) return launch_status();
+  if (n <= 64) {
+    hipLaunchKernelGGL(ce_small_finish_kernel, dim3(1), dim3(1024), 0, st, n, v, (int)k.vp, target, idx64, ignore, reduction, z, row_loss,
+                       on, loss, count);
+  } else {
+    hipLaunchKernelGGL(ce_small_rows_kernel, dim3((n + 3) / 4), dim3(256), 0, st, n, v, (int)k.vp, target, idx64, ignore, z, row_loss, on);
+    if (reduction != 0)
+      hipLaunchKernelGGL(ce_small_total_kernel, dim3(1), dim3(1024), 0, st, n, reduction, row_loss, on, loss, count);
+  }
   return launch_status();
 }
 

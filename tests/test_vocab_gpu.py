@@ -598,7 +598,7 @@ def test_linear_ce_without_a_backward(n, d, v, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("n,d,v", [(1, 1024, 5000), (1, 31, 1025), (2, 33, 3001), (3, 1, 70001), (4, 7, 7000), (7, 130, 2049), (16, 1027, 5003),
                                    (13, 2500, 1500), (16, 64, 66000), (17, 64, 3000), (32, 300, 4001), (33, 129, 2100), (64, 1024, 5000),
-                                   (64, 20, 40000), (65, 64, 3000)])
+                                   (64, 20, 40000), (65, 64, 3000), (5, 20001, 1100), (30, 9000, 1200)])
 def test_linear_ce_few_rows(n, d, v, dtype):
     for i, reduction in enumerate(["mean", "none", "sum"]):
         x, w, b, t = _ce_inputs(n, d, v, dtype, n + d + v + i, bias=i != 1, ignored=0.2 if n > 2 else 0.0,
@@ -610,7 +610,8 @@ def test_linear_ce_few_rows(n, d, v, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("n,d,v", [(1025, 1, 1), (1100, 33, 6), (2000, 64, 16), (4097, 130, 17), (1500, 520, 64), (5000, 67, 64), (30001, 16, 40),
-                                   (1281, 1030, 9), (70000, 128, 64), (3000, 20, 65)])
+                                   (1281, 1010, 9), (1500, 250, 64), (2000, 500, 30), (70000, 128, 64),
+                                   (3000, 20, 65)])
 def test_linear_ce_few_classes(n, d, v, dtype):
     for i, reduction in enumerate(["mean", "none", "sum"]):
         x, w, b, t = _ce_inputs(n, d, v, dtype, n + d + v + i, bias=i != 1, ignored=0.3, index=(torch.int32, torch.int64)[i % 2])
