@@ -544,6 +544,29 @@ def test_linear_ce_large_logits_offsets_and_outliers():
     _check_ce(x, w, None, t, "none", norms=False)
 
 
+@pytest.mark.parametrize("n,v", [(5, 2000), (40, 2000), (1500, 20), (40, 200)])
+def test_linear_ce_subnormal_half_features(n, v):
+    x, w, b, t = _ce_inputs(n, 64, v, F32, 33, ignored=0.0)
+    x, w = (2e-6 * x).to(F16), (2e4 * w).to(F16)
+    assert float(x.abs().max()) < 6e-5 and w.isfinite().all()
+    loss, _ = _check_ce(x, w, None, t, "none", norms=False)
+    assert float((loss - math.log(v)).abs().max()) > 1e-2      # the logits are not zeros
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(12, 3000), (300, 900), (1500, 60)])
+def test_a_table_that_is_the_head_as_well(n, v, dtype):
+    table = torch.randn(v, 32, device=DEV, generator=_gen(41)).to(dtype)
+    ids, target = (torch.randint(0, v, (n,), device=DEV, generator=_gen(42 + i)) for i in range(2))
+    one = table.clone().requires_grad_()
+    h = pointnet2_utils.embedding_operation(one, ids, 0.5)
+    (both,) = torch.autograd.grad(losses.LinearCrossEntropy(h, one, target), one)
+    first, second = table.clone().requires_grad_(), table.clone().requires_grad_()
+    h = pointnet2_utils.embedding_operation(first, ids, 0.5)
+    parts = torch.autograd.grad(losses.LinearCrossEntropy(h, second, target), (first, second))
+    assert torch.equal(both, parts[0] + parts[1])
+
+
 def test_linear_ce_gradient_against_differences():
     x, w, b, t = _ce_inputs(2, 5, 7, F32, 3, ignored=0.0)
     x, w, b = (a.detach().requires_grad_() for a in (x, w, b))
@@ -723,7 +746,7 @@ def _step_inputs(dtype, seed, n=300, v=700, d=48, c=6):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n,v", [(300, 700), (5000, 6000)])
+@pytest.mark.parametrize("n,v", [(300, 700), (5000, 6000), (20, 6000), (3000, 40)])
 def test_lookup_loss_and_distillation_together(dtype, n, v):
     """Gradients of a step with all three, the table shared by the lookup and the loss.  bfloat16: the looked-up rows, the body's output
     and the logits are each rounded (3 roundings on the way in, as many on the way back, the result once), float32 a few units."""
@@ -769,7 +792,7 @@ def test_training_loop_with_the_flat_optimizer():
         assert float((p - q).abs().max()) <= 1e-4 * 1e-2 * 4 + 4 * U * float(q.abs().max()), name
 
 
-@pytest.mark.parametrize("n,v", [(300, 700), (2500, 6000)])
+@pytest.mark.parametrize("n,v", [(300, 700), (2500, 6000), (20, 6000), (3000, 40), (30, 50)])
 def test_captured_steps_replay_with_new_inputs(n, v):
     """Two captured steps alternate with eager work on the same sizes; every replay gives the eager step's bits."""
     dtype = F32
