@@ -8,8 +8,8 @@
 // lanes adds it up in registers -- no atomics, dw written once.  A run longer than L tokens would leave one team with a long chain
 // of loads; it is cut where the sorted list is cut into pieces of L, the pieces are summed side by side and joined in order.
 //
-// 32768 tokens of a table of 65536 x 1024 bfloat16: lookup 25 us (67 MB written, 20 to 40 MB of rows read: 4 TB/s), gradient 97 us of
-// which the sums take 56 us (67 MB read, 134 MB written: 3.6 TB/s) and the sort 41 us: six launches of 4 to 11 us that wait for memory
+// 32768 tokens of a table of 65536 x 1024 bfloat16: lookup 25 us (67 MB written, 20 to 40 MB of rows read: 4 TB/s), gradient 85 us of
+// which the sums take 45 us (67 MB read, 134 MB written: 4.5 TB/s) and the sort 40 us: six launches of 4 to 11 us that wait for memory
 // and for each other, whatever the width of the rows.
 #include <algorithm>
 
@@ -279,11 +279,12 @@ __global__ __launch_bounds__(256) void embed_starts_kernel(int n, int v, const u
   start[t] = lo;
 }
 
-// sum of the gradient rows of sorted tokens [a, e), elements [col, col + left), eight loads in flight, added in order
+// sum of the gradient rows of sorted tokens [a, e), elements [col, col + left), added in order: four loads in flight, two where the run ends
+// (most runs are short; eight and one: 120 us for lookup and gradient of 32768 tokens of 65536 x 1024 bfloat16, this 110 us)
 template <typename T>
 __device__ __forceinline__ void sum_run(const T* __restrict__ grad, long long ldg, const uint32_t* __restrict__ perm, int a, int e,
                                         int col, int left, float (&acc)[kVec<T>]) {
-  constexpr int U = 8;
+  constexpr int U = 4;
   int p = a;
   if (left >= kVec<T>) {
     for (; p + U <= e; p += U) {
@@ -298,6 +299,21 @@ __device__ __forceinline__ void sum_run(const T* __restrict__ grad, long long ld
         for (int i = 0; i < kVec<T>; ++i) acc[i] += f[i];
       }
     }
+  }
+  if (left >= kVec<T>) {
+    for (; p < e; p += 2) {
+      u32x4 raw[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) raw[j] = load16(grad + (long long)perm[min(p + j, e - 1)] * ldg + col);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float f[kVec<T>];
+        unpack<T>(raw[j], f);
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) acc[i] = p + j < e ? acc[i] + f[i] : acc[i];
+      }
+    }
+    return;
   }
   for (; p < e; ++p) {
     float f[kVec<T>];
@@ -386,7 +402,7 @@ __device__ __forceinline__ void sum_piece(float* lds, int n, int v, int d, int l
 }
 
 // Short runs and the pieces of long ones do not meet: one launch, the pieces first because one takes longer.  (32768 tokens of a table of
-// 65536 x 1024 bfloat16: 55 us for both, 48 and 15 us in launches of their own.)
+// 65536 x 1024 bfloat16: 45 us for both, with 15 us more for the pieces in a launch of their own.)
 template <typename T>
 __global__ __launch_bounds__(256) void embed_sums_kernel(int n, int v, int d, int lanes_log, int longest, int pieces,
                                                          const T* __restrict__ grad, long long ldg, const uint32_t* __restrict__ keys,
