@@ -5,8 +5,8 @@
 //
 // Bound by bytes: z is read once forward (one pass with a running maximum and sum), read once and dz written once backward; the
 // teacher's k values are noise beside a row.  A row is one workgroup's, or several workgroups' where there are few rows.  8192 rows of
-// 65536 bfloat16 classes, 5% of them without a teacher: forward 230 us = 4.4 TB/s, backward 428 us = 4.9 TB/s, where a copy of a large
-// tensor runs at 5.15 TB/s.  Four 16-byte loads in flight per thread forward, two beside as many stores backward.
+// 65536 bfloat16 classes, 5% of them without a teacher: forward 230 us = 4.4 TB/s, backward 375 us = 5.6 TB/s, where a copy of a large
+// tensor runs at 5.15 TB/s.  Four 16-byte loads in flight per thread.
 #include <algorithm>
 
 #include "vocab_common.h"
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
   const float g = temp * (reduction == 0 ? gout[row] : reduction == 1 ? gout[0] / count[0] : gout[0]);
   const float gp = g * inv_s;
   const T* in = z + row * ldz;
-  constexpr int U = 2;
+  constexpr int U = THREADS == 1024 ? 4 : 2;
   int at = a + threadIdx.x * V;
   for (; at + (U - 1) * THREADS * V + V <= e; at += U * THREADS * V) {
     float f[U][V];
@@ -325,14 +325,16 @@ __global__ __launch_bounds__(THREADS) void distill_grad_kernel(int v, int k, int
   }
 }
 
-struct DistillPlan { int threads, splits, width; };
+struct DistillPlan { int threads, grad_threads, splits, width; };
 // One wave per row up to 4 KB, four waves above (forward and backward, 8000 rows of 4 KB: 40 us with one, 49 us with four; of 8 KB: 63 and
-// 60 us).  Up to 256 rows of more than 64 KB, too few for the chip's 256 compute units, are cut into parts of 16 KB at least (4 rows of
+// 60 us), sixteen waves backward from 30 KB on, which reads and writes a copy's 5.5 TB/s (forward and backward, 2000 rows of 256 KB: 332 us
+// with four waves, 317 us with sixteen; 8000 of 32 KB: 181 and 176 us, of 16 KB: 94 and 100 us).  Up to 256 rows of more than 64 KB, too few for the chip's 256 compute units, are cut into parts of 16 KB at least (4 rows of
 // 256 KB: 20 us cut, 29 us whole; 64: 24 and 32 us; 512: 76 and 74 us; one row of 64 KB: 20 and 18 us).
 inline DistillPlan distill_plan(long long n, int v, int elt) {
   DistillPlan p;
   const long long bytes = (long long)v * elt;
   p.threads = bytes <= 4096 ? 64 : 256;
+  p.grad_threads = bytes < (30 << 10) || n > (1 << 21) ? p.threads : 1024;      // (a launch holds fewer than 2^32 threads)
   const int block = 4096 / elt;
   const long long blocks = (v + block - 1) / block;
   p.splits = n <= 256 && blocks > 16 ? (int)std::min(blocks / 4, 1024 / n) : 1;
@@ -391,12 +393,11 @@ extern "C" int istnet_distill_backward(long long n, int v, int k, int dtype, int
   const DistillPlan p = distill_plan(n, v, dtype == ISTNET_VOCAB_F32 ? 4 : 2);
   const dim3 grid((unsigned)(n * p.splits));
   VOCAB_DISPATCH(dtype, T, {
-    if (p.threads == 64)
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_grad_kernel<T, 64>), grid, dim3(64), 0, st, v, k, idx64, (const T*)z, ldz, idx,
-                         temperature, reduction, gout, stats, q, count, p.splits, p.width, (T*)dz);
-    else
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_grad_kernel<T, 256>), grid, dim3(256), 0, st, v, k, idx64, (const T*)z, ldz, idx,
-                         temperature, reduction, gout, stats, q, count, p.splits, p.width, (T*)dz);
+    const auto grad = p.grad_threads == 64    ? distill_grad_kernel<T, 64>
+                      : p.grad_threads == 256 ? distill_grad_kernel<T, 256>
+                                              : distill_grad_kernel<T, 1024>;
+    hipLaunchKernelGGL(grad, grid, dim3(p.grad_threads), 0, st, v, k, idx64, (const T*)z, ldz, idx, temperature, reduction, gout, stats, q,
+                       count, p.splits, p.width, (T*)dz);
   });
   return launch_status();
 }
